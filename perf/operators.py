@@ -1,0 +1,488 @@
+"""The 4-bit paged KV cache's operators, as measured cases.
+
+Kinds of case, each one pass through the package's public entry points, or (`own` false) the same
+in elementary torch operations, in 32 bits, rounded once at the end:
+
+  append   kv_append_q4_hip then kv_read_q4_hip: new K/V rows are quantised into their slots, and the
+           same slots read back as the values that they now stand for
+  decode   paged_attention_decode_q4_hip: one query row per request over its 4-bit pages; with
+           "weights", every key's attention weight is added to its slot's running total
+  prefill  paged_attention_prefill_q4_hip: a causal chunk of query rows over 4-bit pages (the chunk's
+           own keys are in them), with or without the running totals
+  evict    evict_q4_hip: per request and KV head, the newest `window` keys and of the others those of
+           the largest totals, `keep` in all, moved in their order into fresh pages
+
+A page holds 16 tokens of one KV head: K and V each in their own pool, uint8 [blocks, heads, page
+bytes]. 64 consecutive values of a row share a half-precision scale s and centre z; the code c in
+0..15 stands for z + s (c - 7.5), with z = half((hi + lo) / 2), s = half((hi - lo) / 15) over the
+group's values (clamped to half's range) and c = (x - z) / s + 7.5 rounded to the nearest, ties to
+even. Codes are kept where the kernels' lanes take them:
+  K  token t, value d = 32 w + 8 g + j: 32-bit word (t, g, w); j even in nibble j / 2, odd in 4 + j / 2
+  V  token t = 4 g + 2 p + e, value d = 64 a + 4 r + n: 16-bit half e of word (g, r, p, a), nibble n
+followed by the (s, z) pairs, [group a][token].
+
+Shapes are the package's own, 8 heads x 64 (the default model) and 32 heads x 128 (its large
+workloads), and the same query heads over fewer KV heads; contexts up to 32768 tokens, 16-token blocks,
+shuffled block tables. Q, K and V are N(0, 1), as behind a LayerNorm.
+"""
+import math
+import random
+import sys
+from pathlib import Path
+
+import torch
+
+own = False
+
+BLOCK, GROUP = 16, 64
+DTYPES = {"fp32": torch.float32, "bf16": torch.bfloat16}
+DEV = "cuda"
+HALF_MAX = 65504.0
+
+
+# ---------------------------------------------------------------------------------------------
+# The cases
+# ---------------------------------------------------------------------------------------------
+def listed():
+    return [
+        # A layer's append of a decode step of the default model, 8 requests: all latency.
+        dict(name="append_8x1_8x64_fp32", kind="append", batch=8, kv_heads=8, head_dim=64, rows=1, io="fp32"),
+        # Prompt chunks of a larger model entering the cache.
+        dict(name="append_4x512_32x128_bf16", kind="append", batch=4, kv_heads=32, head_dim=128, rows=512, io="bf16"),
+        # One chat request in the middle of its answer: the smallest attention call.
+        dict(name="decode_1x8x64_fp32", kind="decode", batch=1, heads=8, kv_heads=8, head_dim=64, lo=128, hi=128,
+             io="fp32", weights=False),
+        # A layer of the default model's decode step under continuous batching, totals kept for eviction.
+        dict(name="decode_8x8x64_fp32_weights", kind="decode", batch=8, heads=8, kv_heads=8, head_dim=64, lo=128,
+             hi=1024, io="fp32", weights=True),
+        # A bf16 model serving a handful of requests whose contexts differ widely.
+        dict(name="decode_16x32x128_bf16", kind="decode", batch=16, heads=32, kv_heads=32, head_dim=128, lo=512,
+             hi=32768, io="bf16", weights=False),
+        # A full batch of long contexts over shared KV heads, totals kept.
+        dict(name="decode_64x32over8x128_bf16_weights", kind="decode", batch=64, heads=32, kv_heads=8, head_dim=128,
+             lo=512, hi=16384, io="bf16", weights=True),
+        # Chunked prefill of the default model: 4 prompts, chunks of up to 256 tokens.
+        dict(name="prefill_4x8x64_fp32", kind="prefill", batch=4, heads=8, kv_heads=8, head_dim=64, chunk=256,
+             ragged=True, lo=0, hi=768, io="fp32", weights=False),
+        # Short odd-sized questions over shared KV heads, totals kept from the first token on.
+        dict(name="prefill_3x61_24over3x64_fp32_weights", kind="prefill", batch=3, heads=24, kv_heads=3, head_dim=64,
+             chunk=61, ragged=True, lo=0, hi=101, io="fp32", weights=True),
+        # Long prompts of a larger bf16 model, 512-token chunks.
+        dict(name="prefill_4x32x128_bf16", kind="prefill", batch=4, heads=32, kv_heads=32, head_dim=128, chunk=512,
+             ragged=False, lo=1024, hi=4096, io="bf16", weights=False),
+        # The last chunk of one long document over shared KV heads, totals kept.
+        dict(name="prefill_1x200_32over8x128_bf16_weights", kind="prefill", batch=1, heads=32, kv_heads=8,
+             head_dim=128, chunk=200, ragged=False, lo=16384, hi=16384, io="bf16", weights=True),
+        # The default model's requests cut back to half of its position table.
+        dict(name="evict_8x8x64_to_512", kind="evict", batch=8, kv_heads=8, head_dim=64, lo=600, hi=1000, keep=512,
+             window=64),
+        # Long contexts of a larger model cut back to a fixed budget.
+        dict(name="evict_16x32x128_to_2048", kind="evict", batch=16, kv_heads=32, head_dim=128, lo=2500, hi=16384,
+             keep=2048, window=256),
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    kind = rng.choice(["append", "decode", "decode", "prefill", "prefill", "evict"])
+    heads, kv_heads, head_dim = rng.choice([(8, 8, 64), (32, 32, 128), (32, 8, 128), (24, 3, 64), (8, 2, 64), (16, 1, 128)])
+    io = rng.choice(["fp32", "bf16"])
+    while True:
+        batch = _log_int(rng, 1, 64)
+        if kind == "append":
+            c = dict(kind=kind, batch=batch, kv_heads=kv_heads, head_dim=head_dim, rows=_log_int(rng, 1, 512), io=io)
+        elif kind == "evict":
+            keep = _log_int(rng, 16, 4096)
+            hi = keep + _log_int(rng, 1, 12288)
+            c = dict(kind=kind, batch=batch, kv_heads=kv_heads, head_dim=head_dim, lo=rng.choice([hi, keep + 1, max(1, keep // 2)]),
+                     hi=hi, keep=keep, window=rng.choice([0, 1, keep // 8, keep // 2, keep]))
+        elif kind == "decode":
+            hi = _log_int(rng, 16, 32768)
+            c = dict(kind=kind, batch=batch, heads=heads, kv_heads=kv_heads, head_dim=head_dim,
+                     lo=max(1, hi // rng.choice([1, 4, 64])), hi=hi, io=io, weights=rng.random() < 0.5)
+        else:
+            hi = _log_int(rng, 1, 16384)
+            c = dict(kind=kind, batch=batch, heads=heads, kv_heads=kv_heads, head_dim=head_dim, chunk=_log_int(rng, 2, 512),
+                     ragged=rng.random() < 0.5, lo=rng.choice([0, hi // 4, hi]), hi=hi, io=io, weights=rng.random() < 0.5)
+        # no more than the largest listed calls, padded to the longest request as the plain form has them
+        w = work(c)
+        longest = c.get("hi", 0) + c.get("chunk", 0)
+        if (w["bytes"] <= 5.5e8 and w["flops"] <= 9e10 and batch * kv_heads * longest * head_dim <= 2.2e9
+                and batch * heads * c.get("chunk", 1) * longest <= 3.2e8):
+            return c
+
+
+# ---------------------------------------------------------------------------------------------
+# Lengths and block tables (host, from the case and a seed; work() uses the seed 0 ones)
+# ---------------------------------------------------------------------------------------------
+def _lengths(case, seed):
+    """(tokens cached once the new ones are in, new tokens) of every request."""
+    rng = random.Random(seed * 7919 + 17)
+    n = case["batch"]
+    if case["kind"] == "append":
+        first = [rng.randrange(0, 1000) for _ in range(n)]
+        return [f + case["rows"] for f in first], [case["rows"]] * n
+    lo, hi = case["lo"], case["hi"]
+    if case["kind"] == "prefill":
+        ctx = [int(round(lo + (hi - lo) * (i + rng.random()) / n)) for i in range(n)]
+        rng.shuffle(ctx)
+        new = [case["chunk"]] * n
+        if case["ragged"]:  # one request keeps the full chunk, so the batch keeps its width
+            new = [case["chunk"]] + [max(1, int(case["chunk"] * rng.uniform(0.3, 1.0))) for _ in range(n - 1)]
+        return [c + t for c, t in zip(ctx, new)], new
+    total = [int(round(lo * (hi / lo) ** ((i + rng.random()) / n))) for i in range(n)]
+    rng.shuffle(total)
+    return total, [1] * n
+
+
+def _pool_blocks(case):
+    """Blocks of the pool: enough for the longest requests of any seed, and some that are free."""
+    n, most = case["batch"], case.get("chunk", 0)
+    if case["kind"] == "append":
+        each = [1000 + case["rows"]] * n
+    elif case["kind"] == "prefill":
+        each = [case["lo"] + math.ceil((case["hi"] - case["lo"]) * (i + 1) / n) + most for i in range(n)]
+    else:
+        each = [math.ceil(case["lo"] * (case["hi"] / case["lo"]) ** ((i + 1) / n)) + 1 for i in range(n)]
+    total = sum(-(-x // BLOCK) for x in each) + (n * -(-case["keep"] // BLOCK) if case["kind"] == "evict" else 0)
+    return total + max(4, total // 16)
+
+
+def _tables(lens, rng, total, spare=()):
+    """Shuffled block tables for requests of these lengths in a pool of `total` blocks, and `spare`
+    more tables of these block counts behind them."""
+    need = [-(-n // BLOCK) for n in lens]
+    ids = list(range(total))
+    rng.shuffle(ids)
+    rows, at = [], 0
+    for n in need + list(spare):
+        rows.append(ids[at:at + n])
+        at += n
+
+    def table(part):
+        width = max(len(r) for r in part)
+        return torch.tensor([r + [-1] * (width - len(r)) for r in part], dtype=torch.int32, device=DEV)
+
+    return table(rows[:len(lens)]), (table(rows[len(lens):]) if spare else None)
+
+
+def page_bytes(head_dim):
+    return BLOCK * (head_dim // 2 + 4 * (head_dim // GROUP))
+
+
+def work(case):
+    hd, hk = case["head_dim"], case["kv_heads"]
+    row = 2 * (hd // 2 + 4 * (hd // GROUP))  # K and V of one token and KV head
+    lens, new = _lengths(case, 0)
+    if case["kind"] == "append":
+        rows = sum(new) * hk
+        e = DTYPES[case["io"]].itemsize
+        # rows in, codes out; codes in, values out
+        return {"bytes": rows * (2 * hd * e + row + row + 2 * hd * e) + 2 * 4 * sum(new), "flops": 0}
+    if case["kind"] == "evict":
+        kept = sum(min(n, case["keep"]) for n in lens)
+        # every total once, the kept rows and totals moved, their places written
+        return {"bytes": hk * (4 * sum(lens) + kept * (2 * row + 4 + 4)) + 4 * sum(-(-n // BLOCK) for n in lens), "flops": 0}
+    h, e = case["heads"], DTYPES[case["io"]].itemsize
+    pairs = sum(sum(n - t + 1 + i for i in range(t)) for n, t in zip(lens, new))
+    b = hk * sum(lens) * row + h * sum(new) * 2 * hd * e + 4 * sum(-(-n // BLOCK) for n in lens)
+    if case["weights"]:
+        b += hk * sum(lens) * 8
+    return {"bytes": b, "flops": 4 * h * hd * pairs}
+
+
+# ---------------------------------------------------------------------------------------------
+# Inputs
+# ---------------------------------------------------------------------------------------------
+def _quantise(x):
+    """Rows [..., head_dim] -> codes (int64, same shape), s and z (half, [..., groups]). The codes are
+    found in 64 bits: a value next to a border goes to its own side."""
+    g = x.float().clamp(-HALF_MAX, HALF_MAX).unflatten(-1, (-1, GROUP))
+    hi, lo = g.amax(-1), g.amin(-1)
+    s = ((hi - lo) * (1.0 / 15.0)).half()
+    z = ((hi + lo) * 0.5).half()
+    step = s.double()[..., None]
+    c = torch.where(step > 0, (g.double() - z.double()[..., None]) / torch.where(step > 0, step, 1.0) + 7.5, 0.0)
+    return c.round().clamp(0, 15).long().flatten(-2), s, z
+
+
+def _row_k(c, s, z):
+    """Codes [..., head_dim], s and z -> a token's bytes of a K page: its codes (g, w, byte), then its pairs."""
+    w = c.unflatten(-1, (-1, 4, 4, 2))  # [.., w, g, j // 2, j % 2]
+    n = w.transpose(-4, -3).transpose(-2, -1).flatten(-2).unflatten(-1, (4, 2))  # [.., g, w, byte, nibble of it]
+    return torch.cat([(n[..., 0] | (n[..., 1] << 4)).flatten(-3).to(torch.uint8), _pairs(s, z)], -1)
+
+
+def _row_v(c, s, z):
+    """The same of a V page: its codes (r, a, byte), then its pairs."""
+    n = c.unflatten(-1, (-1, 16, 2, 2)).transpose(-4, -3)  # [.., r, a, byte, nibble of it]
+    return torch.cat([(n[..., 0] | (n[..., 1] << 4)).flatten(-3).to(torch.uint8), _pairs(s, z)], -1)
+
+
+def _pairs(s, z):
+    return torch.stack([s, z], -1).flatten(-2).view(torch.uint8)
+
+
+def _place_k(t, hd):
+    """Tokens [...] -> the places of their bytes in a K page, in _row_k's order."""
+    t = t[..., None]
+    return torch.cat([t * (hd // 2) + torch.arange(hd // 2, device=t.device), _place_pairs(t, hd)], -1)
+
+
+def _place_v(t, hd):
+    t, groups = t[..., None], hd // GROUP
+    at = torch.arange(hd // 2, device=t.device)
+    r, a, e = at // (2 * groups), at // 2 % groups, at % 2
+    return torch.cat([(((t // 4 * 16 + r) * 2 + t // 2 % 2) * groups + a) * 4 + t % 2 * 2 + e, _place_pairs(t, hd)], -1)
+
+
+def _place_pairs(t, hd):
+    at = torch.arange(4 * (hd // GROUP), device=t.device)
+    return BLOCK * hd // 2 + at // 4 * (4 * BLOCK) + 4 * t + at % 4
+
+
+def _filled(blocks, heads, head_dim, gen, row, place):
+    """A pool whose every slot holds the codes of an N(0, 1) row."""
+    at = place(torch.arange(BLOCK, device=DEV), head_dim).flatten()
+    out = torch.empty(blocks, heads, page_bytes(head_dim), dtype=torch.uint8, device=DEV)
+    step = max(1, (1 << 25) // (heads * BLOCK * head_dim))
+    for first in range(0, blocks, step):
+        n = min(step, blocks - first)
+        x = torch.randn(n, heads, BLOCK, head_dim, generator=gen, device=DEV)
+        out[first:first + n, :, at] = row(*_quantise(x)).flatten(-2)
+    return out
+
+
+def prepare(case, seed):
+    rng = random.Random(seed * 104729 + 5)
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(seed)
+    hd, hk, n = case["head_dim"], case["kv_heads"], case["batch"]
+    lens, new = _lengths(case, seed)
+    spare = [-(-min(x, case["keep"]) // BLOCK) for x in lens] if case["kind"] == "evict" else ()
+    blocks = _pool_blocks(case)
+    table, fresh = _tables(lens, rng, blocks, spare)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    st = dict(case=case, page_table=table, seq_lens=i32(lens), cur_lens=i32(new))
+    if case["kind"] == "append":
+        dt = DTYPES[case["io"]]
+        for name in ("k", "v"):  # [B, T, H, Hd] activations seen as [B, H, T, Hd], as the projections leave them
+            st[name] = torch.randn(n, case["rows"], hk, hd, generator=gen, device=DEV).to(dt).transpose(1, 2)
+        pos = st["seq_lens"].long()[:, None] - case["rows"] + torch.arange(case["rows"], device=DEV)
+        st["slots"] = (table.long().gather(1, pos // BLOCK) * BLOCK + pos % BLOCK).to(torch.int32).flatten()
+        st["k_pool"] = torch.zeros(blocks, hk, page_bytes(hd), dtype=torch.uint8, device=DEV)
+        st["v_pool"] = torch.zeros_like(st["k_pool"])
+        return st
+    st["k_pool"] = _filled(blocks, hk, hd, gen, _row_k, _place_k)
+    st["v_pool"] = _filled(blocks, hk, hd, gen, _row_v, _place_v)
+    if case["kind"] == "evict":
+        # totals as attention leaves them: a few heavy keys, a long tail, some never looked at
+        w = torch.exp(2.0 * torch.randn(blocks, hk, BLOCK, generator=gen, device=DEV))
+        st["weights"] = torch.where(torch.rand(w.shape, generator=gen, device=DEV) < 0.1, 0.0, w)
+        st["fresh"] = fresh
+        return st
+    t = case["chunk"] if case["kind"] == "prefill" else 1
+    st["q"] = torch.randn(n, t, case["heads"], hd, generator=gen, device=DEV).to(DTYPES[case["io"]]).transpose(1, 2)
+    st["weights"] = torch.rand(blocks, hk, BLOCK, generator=gen, device=DEV) if case["weights"] else None
+    return st
+
+
+# ---------------------------------------------------------------------------------------------
+# One pass
+# ---------------------------------------------------------------------------------------------
+def run(st):
+    case = st["case"]
+    if own:
+        return _run_own(case["kind"], st)
+    return {"append": _append, "decode": _attend, "prefill": _attend, "evict": _evict}[case["kind"]](st)
+
+
+def _run_own(kind, st):
+    path = str(Path(__file__).resolve().parents[1] / "efficient-inference-system_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    from src.kernels import hip_q4_attention as q4
+
+    case = st["case"]
+    if kind == "append":
+        q4.kv_append_q4_hip(st["k"], st["v"], st["k_pool"], st["v_pool"], st["slots"])
+        return q4.kv_read_q4_hip(st["k_pool"], st["v_pool"], st["slots"], batch=case["batch"], dtype=DTYPES[case["io"]])
+    if kind == "evict":
+        kept, lens = q4.evict_q4_hip(st["k_pool"], st["v_pool"], st["weights"], st["page_table"], st["seq_lens"],
+                                     st["fresh"], keep=case["keep"], window=case["window"])
+        return kept, lens, st["k_pool"], st["v_pool"], st["weights"]
+    attend = q4.paged_attention_decode_q4_hip if kind == "decode" else q4.paged_attention_prefill_q4_hip
+    out = attend(st["q"], st["k_pool"], st["v_pool"], st["page_table"], st["seq_lens"], st["cur_lens"],
+                 weights=st["weights"])
+    return out, st["weights"]
+
+
+def _codes_k(pages, hd):
+    """K pages [..., page bytes] -> codes as float32 [..., 16, head_dim]."""
+    b = pages[..., :BLOCK * hd // 2].unflatten(-1, (BLOCK, 4, hd // 32, 4))
+    n = torch.stack([b & 15, b >> 4], -1).flatten(-2)  # [.., t, g, w, nibble]
+    n = n.unflatten(-1, (2, 4)).transpose(-2, -1).flatten(-2)  # [.., t, g, w, j]
+    return n.transpose(-3, -2).flatten(-3).float()
+
+
+def _codes_v(pages, hd):
+    b = pages[..., :BLOCK * hd // 2].unflatten(-1, (4, 16, 2, hd // GROUP, 2, 2))  # [.., g, r, p, a, e, byte]
+    n = torch.stack([b & 15, b >> 4], -1).flatten(-2)  # [.., g, r, p, a, e, n]
+    k = n.dim()
+    lead = tuple(range(k - 6))
+    n = n.permute(*lead, k - 6, k - 4, k - 2, k - 3, k - 5, k - 1)  # [.., g, p, e, a, r, n]
+    return n.flatten(-6, -4).flatten(-3).float()
+
+
+def _values(pages, hd, codes):
+    """Pages [..., page bytes] -> the float32 values that they stand for, [..., 16, head_dim]."""
+    c = codes(pages, hd).unflatten(-1, (hd // GROUP, GROUP))
+    m = pages[..., BLOCK * hd // 2:].contiguous().view(torch.float16).float()
+    m = m.unflatten(-1, (hd // GROUP, BLOCK, 2)).transpose(-3, -2)  # [.., token, group, 2]
+    return (m[..., 1:] + m[..., :1] * (c - 7.5)).flatten(-2)
+
+
+def _append(st):
+    k_pool, v_pool = st["k_pool"], st["v_pool"]
+    k, v = _rows_in_and_out(st, st["k"], k_pool, _row_k, _place_k, _codes_k), _rows_in_and_out(
+        st, st["v"], v_pool, _row_v, _place_v, _codes_v)
+    return k, v
+
+
+def _rows_in_and_out(st, new, pool, row, place, codes):
+    blk, off, hd = st["slots"].long() // BLOCK, st["slots"].long() % BLOCK, st["case"]["head_dim"]
+    head = torch.arange(pool.shape[1], device=DEV)[None, :, None]
+    pool[blk[:, None, None], head, place(off, hd)[:, None]] = row(*_quantise(new.transpose(1, 2).flatten(0, 1)))
+    back = _values(pool[blk], hd, codes)[torch.arange(len(blk), device=DEV), :, off]  # [B * T, H, Hd]
+    return back.unflatten(0, (new.shape[0], -1)).transpose(1, 2).to(new.dtype)
+
+
+def _attend(st):
+    q, table = st["q"], st["page_table"].long()
+    n, h, t, hd = q.shape
+    hk = st["k_pool"].shape[1]
+    pages = table.clamp(min=0)
+    k = _values(st["k_pool"][pages], hd, _codes_k).transpose(1, 2).flatten(2, 3)  # [B, Hkv, keys, Hd]
+    rows = q.float().unflatten(1, (hk, h // hk)).flatten(2, 3)  # [B, Hkv, group * T, Hd]
+    scores = torch.matmul(rows, k.transpose(2, 3)) * (1.0 / math.sqrt(hd))
+    del k
+    lens, cur = st["seq_lens"].long()[:, None], st["cur_lens"].long()[:, None]
+    row = torch.arange(t, device=DEV)[None]
+    seen = torch.minimum(lens, lens - cur + 1 + row).clamp(min=0)  # [B, T]
+    seen = seen[:, None].expand(n, h // hk, t).flatten(1)[:, None, :, None]
+    scores.masked_fill_(torch.arange(scores.shape[3], device=DEV) >= seen, -math.inf)
+    top = scores.amax(-1, keepdim=True)
+    p = torch.exp(scores - torch.where(top > -math.inf, top, 0.0))
+    p = p / p.sum(-1, keepdim=True).clamp(min=1e-30)
+    v = _values(st["v_pool"][pages], hd, _codes_v).transpose(1, 2).flatten(2, 3)
+    out = torch.matmul(p, v).unflatten(2, (h // hk, t)).flatten(1, 2)  # [B, H, T, Hd]
+    del v
+    if st["weights"] is not None:
+        real = (row < cur)[:, None].expand(n, h // hk, t).flatten(1)[:, None, :, None]
+        total = torch.where(real, p, 0.0).double().sum(2).float()  # [B, Hkv, keys]
+        total = total.unflatten(2, (-1, BLOCK)).transpose(1, 2)  # [B, pages, Hkv, 16]
+        total = torch.where(table[:, :, None, None] >= 0, total, 0.0)
+        st["weights"].index_add_(0, pages.flatten(), total.flatten(0, 1))
+    return out.to(q.dtype), st["weights"]
+
+
+def _evict(st):
+    case, table, lens = st["case"], st["page_table"].long(), st["seq_lens"].long()
+    keep, window = case["keep"], case["window"]
+    w = st["weights"][table.clamp(min=0)].transpose(1, 2).flatten(2)  # [B, Hkv, keys]
+    keys = w.shape[2]
+    at = torch.arange(keys, device=DEV)
+    end = lens[:, None, None]
+    # the newest above every total, what is not there below all; equal totals in the keys' order
+    rank = torch.where(at >= end - window, math.inf, w)
+    rank = torch.where(at < end, rank, -1.0)
+    order = torch.sort(rank, dim=-1, descending=True, stable=True).indices[..., :keep]
+    count = lens.clamp(max=keep)
+    room = torch.arange(order.shape[2], device=DEV)
+    order = torch.where(room < count[:, None, None], order, keys).sort(-1).values
+    kept = torch.full((*w.shape[:2], keep), -1, dtype=torch.int32, device=DEV)
+    kept[..., :order.shape[2]] = torch.where(order < keys, order, -1)
+    # the kept rows into their new slots, page by page: tokens' bits of K and V lie in known bytes
+    fresh = st["fresh"].long()
+    width = fresh.shape[1] * BLOCK
+    src = torch.full((*w.shape[:2], width), -1, dtype=torch.long, device=DEV)
+    src[..., :min(width, keep)] = kept[..., :width]
+    there = src >= 0
+    src = src.clamp(min=0)
+    batch = torch.arange(len(lens), device=DEV)[:, None, None]
+    head = torch.arange(w.shape[1], device=DEV)[None, :, None]
+    page, off = table.clamp(min=0)[batch, src // BLOCK], src % BLOCK  # [B, Hkv, width]
+    page_to, off_to = fresh.clamp(min=0)[batch, torch.arange(width, device=DEV) // BLOCK], torch.arange(width, device=DEV) % BLOCK
+    off_to = off_to.expand_as(page)
+    page_to = page_to.expand_as(page)
+    head = head.expand_as(page)
+    i, hd = there.flatten().nonzero()[:, 0], case["head_dim"]
+    page, off, page_to, off_to, head = (x.flatten()[i] for x in (page, off, page_to, off_to, head))
+    for pool, place in ((st["k_pool"], _place_k), (st["v_pool"], _place_v)):
+        pool[page_to[:, None], head[:, None], place(off_to, hd)] = pool[page[:, None], head[:, None], place(off, hd)]
+    st["weights"][page_to, head, off_to] = st["weights"][page, head, off]
+    return kept, count.to(torch.int32), st["k_pool"], st["v_pool"], st["weights"]
+
+
+# ---------------------------------------------------------------------------------------------
+# The definition in 64 bits, one request at a time
+# ---------------------------------------------------------------------------------------------
+def _row_values(pool, blk, head_dim, is_k):
+    """Blocks [n] of a pool -> float64 [n * 16, heads, head_dim], each value's bits looked up by its place."""
+    t = torch.arange(BLOCK, device=DEV)[:, None]
+    d = torch.arange(head_dim, device=DEV)[None]
+    if is_k:
+        j = d % 8
+        word = (t * 4 + d // 8 % 4) * (head_dim // 32) + d // 32
+        nibble = torch.where(j % 2 == 0, j // 2, 4 + j // 2)
+    else:
+        word = ((t // 4 * 16 + d % GROUP // 4) * 2 + t % 4 // 2) * (head_dim // GROUP) + d // GROUP
+        nibble = t % 2 * 4 + d % 4
+    byte = (word * 4 + nibble // 2).flatten()
+    raw = pool[blk][:, :, byte].view(len(blk), -1, BLOCK, head_dim)
+    code = torch.div(raw, torch.where(nibble % 2 == 1, 16, 1).to(torch.uint8), rounding_mode="floor") % 16
+    pair = (BLOCK * head_dim // 2 // 4 + d // GROUP * BLOCK + t).flatten()
+    words = pool[blk].view(torch.float16).double()
+    s = words[:, :, 2 * pair].view(code.shape)
+    z = words[:, :, 2 * pair + 1].view(code.shape)
+    return (z + s * (code.double() - 7.5)).transpose(1, 2).flatten(0, 1)
+
+
+def exact(case, seed):
+    st = prepare(case, seed)
+    hd = case["head_dim"]
+    if case["kind"] == "append":
+        out = []
+        for name in ("k", "v"):
+            x = st[name].double().clamp(-HALF_MAX, HALF_MAX).unflatten(-1, (-1, GROUP))
+            hi, lo = x.max(-1, keepdim=True).values.float(), x.min(-1, keepdim=True).values.float()
+            s = ((hi - lo) * (1.0 / 15.0)).half().double()
+            z = ((hi + lo) * 0.5).half().double()
+            code = torch.clamp(torch.round((x - z) / torch.where(s > 0, s, 1.0) + 7.5), 0, 15)
+            out.append((z + s * (code - 7.5)).flatten(-2))
+        return tuple(out)
+    if case["kind"] == "evict":
+        return None  # whole numbers and moved bits: nothing is rounded
+    lens, cur = st["seq_lens"].tolist(), st["cur_lens"].tolist()
+    out = torch.zeros(st["q"].shape, dtype=torch.float64, device=DEV)
+    totals = st["weights"].double() if st["weights"] is not None else None
+    group = case["heads"] // case["kv_heads"]
+    for b, (n, c) in enumerate(zip(lens, cur)):
+        blk = st["page_table"][b, :-(-n // BLOCK)].long()
+        k = _row_values(st["k_pool"], blk, hd, True)[:n]
+        v = _row_values(st["v_pool"], blk, hd, False)[:n]
+        added = torch.zeros(len(blk) * BLOCK, case["kv_heads"], dtype=torch.float64, device=DEV)
+        for h in range(case["kv_heads"]):
+            for i in range(h * group, h * group + group):
+                a = st["q"][b, i].double() @ k[:, h].T / math.sqrt(hd)
+                row = torch.arange(a.shape[0], device=DEV)[:, None]
+                a = torch.where(torch.arange(n, device=DEV)[None] < (n - c + 1 + row).clamp(max=n), a, -math.inf)
+                p = torch.softmax(a, -1).nan_to_num(0.0)
+                out[b, i] = p @ v[:, h]
+                added[:n, h] += p[:c].sum(0)
+        if totals is not None:
+            totals[blk] += added.view(len(blk), BLOCK, -1).transpose(1, 2)
+    return out, totals
