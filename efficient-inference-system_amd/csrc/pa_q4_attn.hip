@@ -1,0 +1,817 @@
+// Paged attention over 4-bit KV pages on gfx950: decode steps and causal prefill chunks, with grouped
+// query heads and, on request, the attention weights added to each slot's running total.
+//
+// A request's query rows over one KV head are numbered m = i * group + j (query position i, head j of
+// the `group` heads that share the KV head) and are columns of 16-column tiles. Per step of 32 keys
+// (two pages), wavefront and tile, with v_mfma_f32_16x16x32_f16 (fp32 accumulation):
+//   S^T = K Q^T   per page and group of 64 values: A = the codes (exact), B = the q rows, held as fp16 in
+//                 registers for the whole walk. s and z enter outside: S = sum_groups s (acc - 7.5 qs) +
+//                 z qs, qs = the sum of the group's q as rounded, -7.5 qs the accumulator's start.
+//   softmax       lane (g, c) holds column c's scores of keys 4 g + i of both pages.
+//   O^T += V^T P^T  A = the codes, B = w = p s of the value's group, in the lanes that hold p. The rest of
+//                 the value, sum_keys p z - 7.5 w, is one fp32 sum per column and group.
+// The codes never leave the matrix cores' operands and no cross-lane move feeds them (see pa_q4.h).
+//
+// Precision. bf16 q is exact in fp16 once scaled by a power of two per row (below 2^-23 of the row's
+// largest element bits are lost); w is rounded to fp16 (2^-12), the 7.5 w beside it is the rounded
+// one, so the error is that of a code within +-7.5. For fp32 q (PARTS = 2) q and w are each the sum
+// of two fp16 values, 2^-23 or better: the columns of a tile are 8 rows twice, column c the high parts
+// of row c, column c + 8 the low ones, both parts' products summed with one DPP rotation. The second
+// product costs no matrix instruction up to 8 rows per tile.
+//
+// Range. Weights are kept as p = 2^(S - M), M per column, with M chosen so that p * max(s) is near 2^4 when M
+// is set, and set again (accumulators rescaled) when a key's p * max(s, 2^-14) passes 2^15: p s stays
+// inside fp16, above its subnormals for keys within 2^-18 of the heaviest. M cancels in O / l.
+//
+// Kernels:
+//   q4_attn_kernel<WIDE = false>  up to one tile of rows: the workgroup's wavefronts split the keys and
+//                 merge in LDS (decode, short chunks).
+//   q4_attn_kernel<WIDE = true>   each wavefront has NC tiles of its own and walks all keys.
+//   Either splits the keys over several workgroups when the grid is small, as records (M, l, O) that
+//   q4_finish_kernel merges; it also adds the weights of decode steps up, from the scores that the first
+//   kernel left in the workspace. q4_weights_kernel does so for chunks: it forms the scores again.
+#include "pa_attention.h"
+#include "pa_q4.h"
+
+namespace pa {
+
+struct Q4Args {
+  const void* q;
+  int64_t q_sb, q_sh, q_st;
+  void* out;
+  int64_t o_sb, o_sh, o_st;
+  const uint8_t* k_pool;
+  const uint8_t* v_pool;
+  float* weights;  // null: no totals
+  int64_t num_blocks;
+  const int32_t* page_table;
+  int64_t pt_stride;
+  int32_t max_pages;
+  const int32_t* seq_lens;
+  const int32_t* cur_lens;
+  int32_t B, H, Hk, group, T;
+  float scale_log2;
+  int32_t tiles;        // row tiles (workgroups' worth of rows) per (request, KV head)
+  int32_t splits;       // key ranges per tile, >= 1
+  int32_t split_pages;  // pages per key range, even
+  float* rec;           // splits > 1: (M, l, O[HD]) per (split, row)
+  float* lse;           // totals: log2 of each row's denominator
+  float* scores;        // decode totals: log2-domain scores [B, H, score_stride]
+  int64_t score_stride;
+};
+
+constexpr float kQ4Start = 4.f;         // log2 of p * max(s) when M is set
+constexpr float kQ4Limit = 32768.f;     // p * max(s, 2^-14) beyond which M is set again
+constexpr float kQ4Floor = 6.103515625e-5f;  // 2^-14
+// Codes as the matrix cores take them. As fp16 subnormals (c 2^-24) they cost one AND, but the cores align
+// a product by its operands' exponents without normalising them, so that a sum keeps 7 to 10 bits fewer
+// than fp32: 2^-17 of the largest term, enough beside a bf16 result. For fp32 q (PARTS = 2) they are
+// multiplied by 2^15 (v_pk_mul_f16, one more instruction per pair), which makes them normal and the sums
+// fp32's. The error of 1024 keys' output falls from 3e-5 to what the table below says.
+template <int PARTS> constexpr float kQ4Unit = PARTS == 2 ? 512.f : 16777216.f;  // 1 / the value of code 1
+template <int PARTS> constexpr int kQ4UnitLog2 = PARTS == 2 ? 9 : 24;
+template <int PARTS>
+__device__ __forceinline__ uint32_t q4_pair(uint32_t masked) {
+  if constexpr (PARTS == 1) return masked;
+  return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, masked) * f16x2{(_Float16)32768.f, (_Float16)32768.f});
+}
+
+// One step's page data of a lane.
+template <int HD>
+struct Q4Raw {
+  static constexpr int G = HD / kQ4Group, W = HD / 32;
+  uint32_t k[2][W], v[2][2 * G];
+  u32x4 km[2][G], vm[2][G];
+};
+
+template <int HD>
+__device__ __forceinline__ void q4_load_page(const uint8_t* kp, const uint8_t* vp, int lane, Q4Raw<HD>& r, int h) {
+  constexpr int G = HD / kQ4Group, W = HD / 32;
+  const int g = lane >> 4, c = lane & 15;
+  const uint32_t* kc = reinterpret_cast<const uint32_t*>(kp) + (c * 4 + g) * W;
+  const uint32_t* vc = reinterpret_cast<const uint32_t*>(vp) + lane * 2 * G;
+  if constexpr (HD == 128) {
+    const u32x4 a = *reinterpret_cast<const u32x4*>(kc), b = *reinterpret_cast<const u32x4*>(vc);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      r.k[h][i] = a[i];
+      r.v[h][i] = b[i];
+    }
+  } else {
+    const u32x2 a = *reinterpret_cast<const u32x2*>(kc), b = *reinterpret_cast<const u32x2*>(vc);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      r.k[h][i] = a[i];
+      r.v[h][i] = b[i];
+    }
+  }
+#pragma unroll
+  for (int a = 0; a < G; ++a) {
+    const int off = q4_codes_bytes(HD) + (a * kQ4Tokens + 4 * g) * 4;
+    r.km[h][a] = *reinterpret_cast<const u32x4*>(kp + off);
+    r.vm[h][a] = *reinterpret_cast<const u32x4*>(vp + off);
+  }
+}
+
+// A wavefront's columns: operands, sums and running state of NC tiles.
+template <int HD, int PARTS, int NC>
+struct Q4Wave {
+  static constexpr int G = HD / kQ4Group, W = HD / 32;
+  f16x8 q[NC][W];
+  float qs[NC][G];  // sum of the group's q operands (units of code 1)
+  float sc[NC];     // log2-domain score of such a unit
+  int n[NC];        // keys the column sees (a column without a row: 0x7fffffff)
+  f32x4 o[NC][G][4];
+  float y[NC][G], M[NC], l[NC];
+};
+
+template <typename IO>
+__device__ __forceinline__ void q4_load_q(const IO* p, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8 * (int)sizeof(IO) / 16; ++i) {
+    float f[Vec16<IO>::EPL];
+    u32x4 w;
+    __builtin_memcpy(&w, reinterpret_cast<const char*>(p) + 16 * i, 16);
+    Vec16<IO>::unpack(w, f);
+#pragma unroll
+    for (int j = 0; j < Vec16<IO>::EPL; ++j) x[i * Vec16<IO>::EPL + j] = f[j];
+  }
+}
+
+// The row of column c of a tile, and whether the column holds its low parts.
+template <int PARTS>
+__device__ __forceinline__ int q4_row(int tile, int c) { return PARTS == 2 ? tile * 8 + (c & 7) : tile * 16 + c; }
+
+// Column tile `tile` of (request b, KV head hk): q as operands, scaled by a power of two per row.
+template <typename IO, int HD, int PARTS, int NC>
+__device__ __forceinline__ void q4_setup(const Q4Args& a, int b, int hk, int tile, int L, int C, int keys, int lane,
+                                         Q4Wave<HD, PARTS, NC>& w, int nc) {
+  constexpr int G = HD / kQ4Group, W = HD / 32;
+  const int g = lane >> 4, c = lane & 15;
+  const int row = q4_row<PARTS>(tile, c);
+  const bool there = row < a.T * a.group;
+  const int i = row / a.group, j = row - i * a.group;
+  const IO* src = static_cast<const IO*>(a.q) + (int64_t)b * a.q_sb + (int64_t)(hk * a.group + j) * a.q_sh + (int64_t)i * a.q_st;
+  float x[W][8];
+  float top = 0.f;
+#pragma unroll
+  for (int s = 0; s < W; ++s) {
+    if (there) {
+      q4_load_q<IO>(src + 32 * s + 8 * g, x[s]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[s][e] = 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[s][e]));
+  }
+  top = max_xor32(max_xor16(top));
+  // top * 2^up in [2^13, 2^14); rows of zeros, of infinities and of the last binades stay as they are
+  int up = top > 0.f && top < INFINITY ? 14 - (__builtin_amdgcn_frexp_expf(top)) : 0;
+  up = up > 120 ? 120 : up;
+  up = up < -120 ? -120 : up;
+  float sum[G];
+#pragma unroll
+  for (int k = 0; k < G; ++k) sum[k] = 0.f;
+#pragma unroll
+  for (int s = 0; s < W; ++s) {
+    f16x8 v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float f = ldexpf(x[s][e], up - ((e & 2) ? 4 : 0));  // codes of the odd masks read 16 times as large
+      _Float16 h = (_Float16)f;
+      if (PARTS == 2 && c >= 8) h = (_Float16)(f - (float)h);
+      v[e] = h;
+      sum[s / 2] += (e & 2) ? 16.f * (float)h : (float)h;
+    }
+    w.q[nc][s] = v;
+  }
+#pragma unroll
+  for (int k = 0; k < G; ++k) w.qs[nc][k] = sum_xor32(sum_xor16(sum[k])) * (1.f / kQ4Unit<PARTS>);
+  w.sc[nc] = fminf(ldexpf(a.scale_log2, kQ4UnitLog2<PARTS> - up), 1e38f);
+  int n = valid_keys(L, C, i);
+  n = n < keys ? n : keys;
+  w.n[nc] = there ? n : 0x7fffffff;
+  w.M[nc] = kNegBig;
+  w.l[nc] = 0.f;
+#pragma unroll
+  for (int k = 0; k < G; ++k) {
+    w.y[nc][k] = 0.f;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) w.o[nc][k][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+}
+
+// Scores (units of code 1) of one page: lane (g, c) gets keys 4 g + i of its column.
+template <int HD, int PARTS, int NC>
+__device__ __forceinline__ f32x4 q4_scores(const f16x8 (&kf)[HD / 32], const u32x4 (&km)[HD / kQ4Group],
+                                           const Q4Wave<HD, PARTS, NC>& w, int nc) {
+  constexpr int G = HD / kQ4Group;
+  f32x4 S = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < G; ++k) {
+    const float q0 = w.qs[nc][k], start = -7.5f * q0;
+    f32x4 acc = {start, start, start, start};
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[2 * k], w.q[nc][2 * k], acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[2 * k + 1], w.q[nc][2 * k + 1], acc, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      S[i] = fmaf(q4_scale(km[k][i]), acc[i], k == 0 ? q4_centre(km[k][i]) * q0 : fmaf(q4_centre(km[k][i]), q0, S[i]));
+  }
+  if constexpr (PARTS == 2) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) S[i] += dpp<0x128>(S[i]);
+  }
+  return S;
+}
+
+template <int HD, int PARTS>
+__device__ __forceinline__ void q4_k_operands(const uint32_t (&k)[HD / 32], f16x8 (&kf)[HD / 32]) {
+#pragma unroll
+  for (int s = 0; s < HD / 32; ++s) {
+    const uint32_t x = k[s], y = x >> 8;
+    kf[s] = q4_operand(q4_pair<PARTS>(x & kQ4Even), q4_pair<PARTS>(x & kQ4Odd), q4_pair<PARTS>(y & kQ4Even),
+                       q4_pair<PARTS>(y & kQ4Odd));
+  }
+}
+
+// One step: 32 keys from key `key0` on. MASK: some column does not see all of them, or a page is
+// missing (live: bit h set where page h is there). scores: where to leave the log2-domain scores of
+// this lane's column, or null.
+template <int HD, int PARTS, int NC, bool MASK>
+__device__ __forceinline__ void q4_step(const Q4Raw<HD>& r, Q4Wave<HD, PARTS, NC>& w, int key0, int live, int lane,
+                                        float* scores) {
+  constexpr int G = HD / kQ4Group, W = HD / 32;
+  const int g = lane >> 4;
+  const bool low = PARTS == 2 && (lane & 15) >= 8;
+  f16x8 kf[2][W];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) q4_k_operands<HD, PARTS>(r.k[h], kf[h]);
+  // max(s) over the groups of V, and z - 7.5 s where w is whole (PARTS = 2)
+  float vs[2][4];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float m = kQ4Floor;
+#pragma unroll
+      for (int k = 0; k < G; ++k) m = fmaxf(m, q4_scale(r.vm[h][k][i]));
+      vs[h][i] = m;
+    }
+#pragma unroll
+  for (int nc = 0; nc < NC; ++nc) {
+    f32x4 S[2];
+    bool see[2][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      S[h] = q4_scores<HD, PARTS, NC>(kf[h], r.km[h], w, nc);
+      if constexpr (MASK) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          see[h][i] = (live >> h & 1) && key0 + 16 * h + 4 * g + i < w.n[nc];
+          S[h][i] = see[h][i] ? S[h][i] : -INFINITY;
+        }
+      }
+    }
+    if (scores != nullptr) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) *reinterpret_cast<f32x4*>(scores + 16 * h) = S[h] * w.sc[nc];
+    }
+    float p[2][4], far = 0.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[h][i] = fast_exp2(fmaf(S[h][i], w.sc[nc], -w.M[nc]));
+        far = fmaxf(far, p[h][i] * (MASK && !see[h][i] ? 0.f : vs[h][i]));
+      }
+    if (__builtin_expect(__any(far > kQ4Limit), 0)) {
+      float m = kNegBig;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float u = fmaf(S[h][i], w.sc[nc], __builtin_amdgcn_logf(vs[h][i])) - kQ4Start;
+          m = fmaxf(m, MASK && !see[h][i] ? kNegBig : u);
+        }
+      m = max_xor32(max_xor16(m));
+      const float M = fmaxf(w.M[nc], m), f = fast_exp2(w.M[nc] - M);
+      w.M[nc] = M;
+      w.l[nc] *= f;
+#pragma unroll
+      for (int k = 0; k < G; ++k) {
+        w.y[nc][k] *= f;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) w.o[nc][k][t] *= f;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[h][i] = fast_exp2(fmaf(S[h][i], w.sc[nc], -M));
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w.l[nc] += p[h][i];
+#pragma unroll
+    for (int k = 0; k < G; ++k) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t m = r.vm[e >> 2][k][e & 3];
+        const bool on = !MASK || see[e >> 2][e & 3];
+        x[e] = on ? p[e >> 2][e & 3] * q4_scale(m) : 0.f;
+        w.y[nc][k] = fmaf(p[e >> 2][e & 3], on ? q4_centre(m) : 0.f, w.y[nc][k]);
+      }
+      f16x8 b;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        _Float16 hi = (_Float16)x[e];
+        if constexpr (PARTS == 2) {
+          w.y[nc][k] = fmaf(-7.5f, x[e], w.y[nc][k]);
+          const _Float16 lo = (_Float16)(x[e] - (float)hi);
+          b[e] = low ? lo : hi;
+        } else {
+          w.y[nc][k] = fmaf(-7.5f, (float)hi, w.y[nc][k]);
+          b[e] = hi;
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        uint32_t o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {  // page e / 2, token pair e % 2
+          const uint32_t x0 = r.v[e >> 1][(e & 1) * G + k];
+          o[e] = q4_pair<PARTS>((t & 2 ? x0 >> 8 : x0) & (t & 1 ? kQ4Odd : kQ4Even));
+        }
+        w.o[nc][k][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q4_operand(o[0], o[1], o[2], o[3]), b, w.o[nc][k][t], 0, 0, 0);
+      }
+    }
+  }
+}
+
+// The walk over pages [p0, p1) (p0 even): page ids 64 at a time in a register, the next step's pages loaded
+// before this one's products. all: keys below it are seen by every column.
+template <int HD, int PARTS, int NC>
+__device__ __forceinline__ void q4_walk(const Q4Args& a, int b, int hk, int p0, int p1, int all, int lane,
+                                        Q4Wave<HD, PARTS, NC>& w, float* scores) {
+  constexpr int PB = q4_page_bytes(HD);
+  if (p0 >= p1) return;
+  const int32_t* table = a.page_table + (int64_t)b * a.pt_stride;
+  const int64_t step = (int64_t)a.Hk * PB;
+  const uint8_t* kb = a.k_pool + (int64_t)hk * PB;
+  const uint8_t* vb = a.v_pool + (int64_t)hk * PB;
+  auto ids_at = [&](int p) { return p + lane < p1 ? table[p + lane] : -1; };
+  int ids = ids_at(p0), base = p0;
+  Q4Raw<HD> cur, next;
+  auto fetch = [&](int p, Q4Raw<HD>& r) {  // pages p and p + 1; returns which are there
+    if (p - base >= 64) {
+      base += 64;
+      ids = ids_at(base);
+    }
+    int live = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int id = q4_block(__builtin_amdgcn_readlane(ids, p - base + h), a.num_blocks);
+      live |= (id >= 0) << h;
+      const int64_t off = (int64_t)(id >= 0 ? id : 0) * step;
+      q4_load_page<HD>(kb + off, vb + off, lane, r, h);
+    }
+    return live;
+  };
+  int live = fetch(p0, cur);
+  for (int p = p0; p < p1; p += 2) {
+    int live_next = 0;
+    if (p + 2 < p1) live_next = fetch(p + 2, next);
+    const int key0 = p * kQ4Tokens;
+    float* at = scores == nullptr ? nullptr : scores + key0;
+    if (live == 3 && key0 + 32 <= all)
+      q4_step<HD, PARTS, NC, false>(cur, w, key0, live, lane, at);
+    else
+      q4_step<HD, PARTS, NC, true>(cur, w, key0, live, lane, at);
+    cur = next;
+    live = live_next;
+  }
+}
+
+// A tile's walk is done: the lanes' sums joined. Leaves in lane (g, c) the 16 values d = 64 k + 16 g ..
+// + 15 of column c's unnormalised row per group, and l.
+template <int HD, int PARTS, int NC>
+__device__ __forceinline__ void q4_join(Q4Wave<HD, PARTS, NC>& w, int nc, float (&o)[HD / kQ4Group][16], float& l) {
+  constexpr int G = HD / kQ4Group;
+  l = sum_xor32(sum_xor16(w.l[nc]));
+#pragma unroll
+  for (int k = 0; k < G; ++k) {
+    const float y = sum_xor32(sum_xor16(w.y[nc][k]));
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float v = w.o[nc][k][t][i];
+        if constexpr (PARTS == 2) v += dpp<0x128>(v);
+        o[k][4 * i + t] = fmaf(v, (t & 1) ? kQ4Unit<PARTS> / 16.f : kQ4Unit<PARTS>, y);
+      }
+  }
+}
+
+template <typename IO>
+__device__ __forceinline__ void q4_store16(IO* p, const float (&o)[16], float f) {
+  if constexpr (sizeof(IO) == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f32x4 v = {o[4 * i] * f, o[4 * i + 1] * f, o[4 * i + 2] * f, o[4 * i + 3] * f};
+      __builtin_memcpy(p + 4 * i, &v, 16);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      u32x4 v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = pack_bf16x2(o[8 * i + 2 * j] * f, o[8 * i + 2 * j + 1] * f);
+      __builtin_memcpy(p + 8 * i, &v, 16);
+    }
+  }
+}
+
+// Record of a row's part: M, l, O[HD].
+template <int HD>
+__device__ __forceinline__ float* q4_record(const Q4Args& a, int b, int hk, int row, int split) {
+  const int64_t rows = (int64_t)a.T * a.group;
+  return a.rec + ((((int64_t)b * a.Hk + hk) * rows + row) * a.splits + split) * (HD + 2);
+}
+__device__ __forceinline__ float* q4_lse(const Q4Args& a, int b, int hk, int row) {
+  return a.lse + ((int64_t)b * a.Hk + hk) * a.T * a.group + row;
+}
+
+// Workgroup -> (request, KV head, tile, split): KV heads innermost, so that workgroups of one moment
+// read neighbouring slabs of the same blocks; later (longer) tiles first.
+struct Q4Unit { int b, hk, tile, split; };
+__device__ __forceinline__ Q4Unit q4_unit(const Q4Args& a) {
+  int x = blockIdx.x;
+  Q4Unit u;
+  u.hk = x % a.Hk;
+  x /= a.Hk;
+  u.split = x % a.splits;
+  x /= a.splits;
+  u.b = x % a.B;
+  u.tile = a.tiles - 1 - x / a.B;
+  return u;
+}
+
+constexpr int kQ4Waves = 4;
+
+template <typename IO, int HD, int PARTS, int NC, bool WIDE>
+__global__ __launch_bounds__(64 * kQ4Waves) void q4_attn_kernel(const Q4Args a) {
+  constexpr int G = HD / kQ4Group;
+  constexpr int ROWS = PARTS == 2 ? 8 : 16;  // rows of a column tile
+  __shared__ float part[WIDE ? 1 : kQ4Waves * ROWS * (HD + 2)];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int g = lane >> 4, c = lane & 15;
+  const Q4Unit u = q4_unit(a);
+  const int L = a.seq_lens[u.b], C = a.cur_lens[u.b];
+  const int rows = a.T * a.group;
+  int keys = L < a.max_pages * kQ4Tokens ? L : a.max_pages * kQ4Tokens;
+  keys = keys > 0 ? keys : 0;
+  // the pages that the workgroup's rows see, and its share of them
+  const int first = WIDE ? u.tile * kQ4Waves * NC * ROWS : u.tile * ROWS;
+  const int my_first = WIDE ? first + wave * NC * ROWS : first;
+  const int end = my_first + NC * ROWS < rows ? my_first + NC * ROWS : rows;
+  int most = 0, all = 0;
+  if (my_first < rows) {
+    const int lo = my_first / a.group, hi = (end - 1) / a.group;
+    all = valid_keys(L, C, lo);
+    most = valid_keys(L, C, hi);
+    most = most < keys ? most : keys;
+    all = all < keys ? all : keys;
+  }
+  const int pages = (most + kQ4Tokens - 1) / kQ4Tokens;
+  int p0 = u.split * a.split_pages, p1 = a.splits > 1 ? p0 + a.split_pages : pages;
+  p1 = p1 < pages ? p1 : pages;
+  if (!WIDE) {  // the wavefronts' shares, whole steps
+    const int pairs = p1 > p0 ? (p1 - p0 + 1) / 2 : 0;
+    const int per = (pairs + kQ4Waves - 1) / kQ4Waves;
+    const int s0 = p0 + 2 * per * wave;
+    p1 = s0 + 2 * per < p1 ? s0 + 2 * per : p1;
+    p0 = s0;
+  }
+  Q4Wave<HD, PARTS, NC> w;
+  const int tile0 = my_first / ROWS;
+#pragma unroll
+  for (int nc = 0; nc < NC; ++nc) q4_setup<IO, HD, PARTS, NC>(a, u.b, u.hk, tile0 + nc, L, C, keys, lane, w, nc);
+  float* scores = nullptr;
+  if constexpr (!WIDE) {
+    const int row = q4_row<PARTS>(u.tile, c);
+    if (a.scores != nullptr && row < rows && c < ROWS)
+      scores = a.scores + ((int64_t)u.b * a.H + u.hk * a.group + row) * a.score_stride + 4 * g;
+  }
+  q4_walk<HD, PARTS, NC>(a, u.b, u.hk, p0, p1, all, lane, w, scores);
+
+  if constexpr (WIDE) {
+#pragma unroll
+    for (int nc = 0; nc < NC; ++nc) {
+      const int row = q4_row<PARTS>(tile0 + nc, c);
+      float o[G][16], l;
+      q4_join<HD, PARTS, NC>(w, nc, o, l);
+      if (row >= rows || c >= ROWS) continue;
+      if (a.splits > 1) {
+        float* rec = q4_record<HD>(a, u.b, u.hk, row, u.split);
+        if (g == 0) {
+          rec[0] = w.M[nc];
+          rec[1] = l;
+        }
+#pragma unroll
+        for (int k = 0; k < G; ++k)
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<f32x2*>(rec + 2 + 64 * k + 16 * g + 2 * i) = f32x2{o[k][2 * i], o[k][2 * i + 1]};
+      } else {
+        const int i = row / a.group, j = row - i * a.group;
+        IO* out = static_cast<IO*>(a.out) + (int64_t)u.b * a.o_sb + (int64_t)(u.hk * a.group + j) * a.o_sh + (int64_t)i * a.o_st;
+        const float f = l > 0.f || l != l ? 1.f / l : 0.f;
+#pragma unroll
+        for (int k = 0; k < G; ++k) q4_store16<IO>(out + 64 * k + 16 * g, o[k], f);
+        if (a.lse != nullptr && g == 0) *q4_lse(a, u.b, u.hk, row) = l > 0.f ? w.M[nc] + __builtin_amdgcn_logf(l) : INFINITY;
+      }
+    }
+  } else {
+    float o[G][16], l;
+    q4_join<HD, PARTS, NC>(w, 0, o, l);
+    float* mine = part + (wave * ROWS + (c & (ROWS - 1))) * (HD + 2);
+    if (c < ROWS) {
+      if (g == 0) {
+        mine[0] = w.M[0];
+        mine[1] = l;
+      }
+#pragma unroll
+      for (int k = 0; k < G; ++k)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mine[2 + 64 * k + 16 * g + i] = o[k][i];
+    }
+    __syncthreads();
+    const int n = rows - first < ROWS ? rows - first : ROWS;
+    for (int x = threadIdx.x; x < n * HD; x += 64 * kQ4Waves) {
+      const int r = x / HD, d = x - r * HD, row = first + r;
+      float M = kNegBig;
+#pragma unroll
+      for (int v = 0; v < kQ4Waves; ++v) M = fmaxf(M, part[(v * ROWS + r) * (HD + 2)]);
+      float l2 = 0.f, s = 0.f;
+#pragma unroll
+      for (int v = 0; v < kQ4Waves; ++v) {
+        const float* rec = part + (v * ROWS + r) * (HD + 2);
+        const float f = fast_exp2(rec[0] - M);
+        l2 = fmaf(f, rec[1], l2);
+        s = fmaf(f, rec[2 + d], s);
+      }
+      if (a.splits > 1) {
+        float* rec = q4_record<HD>(a, u.b, u.hk, row, u.split);
+        if (d == 0) {
+          rec[0] = M;
+          rec[1] = l2;
+        }
+        rec[2 + d] = s;
+      } else {
+        const int i = row / a.group, j = row - i * a.group;
+        IO* out = static_cast<IO*>(a.out) + (int64_t)u.b * a.o_sb + (int64_t)(u.hk * a.group + j) * a.o_sh + (int64_t)i * a.o_st;
+        Elem<IO>::store(out + d, l2 > 0.f || l2 != l2 ? s / l2 : 0.f);
+        if (a.lse != nullptr && d == 0) *q4_lse(a, u.b, u.hk, row) = l2 > 0.f ? M + __builtin_amdgcn_logf(l2) : INFINITY;
+      }
+    }
+  }
+}
+
+// Records of a row's splits -> its output and log2 denominator. One wavefront per row.
+template <typename IO, int HD>
+__global__ __launch_bounds__(256) void q4_merge_kernel(const Q4Args a, int64_t total) {
+  const int64_t x = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (x >= total) return;
+  const int lane = threadIdx.x & 63;
+  const int rows = a.T * a.group;
+  const int row = (int)(x % rows);
+  const int hk = (int)(x / rows % a.Hk), b = (int)(x / rows / a.Hk);
+  const float* rec = q4_record<HD>(a, b, hk, row, 0);
+  float M = kNegBig;
+  for (int s = 0; s < a.splits; ++s) M = fmaxf(M, rec[(int64_t)s * (HD + 2)]);
+  constexpr int E = HD / 64;
+  float l = 0.f, o[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.f;
+  for (int s = 0; s < a.splits; ++s) {
+    const float* p = rec + (int64_t)s * (HD + 2);
+    const float f = fast_exp2(p[0] - M);
+    l = fmaf(f, p[1], l);
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = fmaf(f, p[2 + lane + 64 * e], o[e]);
+  }
+  const int i = row / a.group, j = row - i * a.group;
+  IO* out = static_cast<IO*>(a.out) + (int64_t)b * a.o_sb + (int64_t)(hk * a.group + j) * a.o_sh + (int64_t)i * a.o_st;
+#pragma unroll
+  for (int e = 0; e < E; ++e) Elem<IO>::store(out + lane + 64 * e, l > 0.f || l != l ? o[e] / l : 0.f);
+  if (a.lse != nullptr && lane == 0) *q4_lse(a, b, hk, row) = l > 0.f ? M + __builtin_amdgcn_logf(l) : INFINITY;
+}
+
+// Decode totals: each key's weight, from the scores left in the workspace. A block that two rows of
+// the page table share is added to by both, hence the atomic; otherwise each slot gets one addition.
+__global__ __launch_bounds__(256) void q4_decode_weights_kernel(const Q4Args a) {
+  const int b = blockIdx.z, hk = blockIdx.y;
+  const int t = blockIdx.x * 256 + threadIdx.x;
+  const int L = a.seq_lens[b], C = a.cur_lens[b];
+  int n = valid_keys(L, C, 0);
+  n = n < a.max_pages * kQ4Tokens ? n : a.max_pages * kQ4Tokens;
+  if (t >= n || C < 1) return;
+  const int id = q4_block(a.page_table[(int64_t)b * a.pt_stride + t / kQ4Tokens], a.num_blocks);
+  if (id < 0) return;
+  float sum = 0.f;
+  for (int j = 0; j < a.group; ++j)
+    sum += fast_exp2(a.scores[((int64_t)b * a.H + hk * a.group + j) * a.score_stride + t] - *q4_lse(a, b, hk, j));
+  atomicAdd(a.weights + ((int64_t)id * a.Hk + hk) * kQ4Tokens + (t & (kQ4Tokens - 1)), sum);
+}
+
+// Totals of a chunk: the scores formed again, page pair by page pair, the rows' weights summed. One
+// wavefront per (request, KV head, two pages); K operands stay in registers over all rows.
+template <typename IO, int HD, int PARTS>
+__global__ __launch_bounds__(256) void q4_chunk_weights_kernel(const Q4Args a) {
+  constexpr int W = HD / 32, PB = q4_page_bytes(HD);
+  constexpr int ROWS = PARTS == 2 ? 8 : 16;
+  const int b = blockIdx.z, hk = blockIdx.y;
+  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  const int p0 = 2 * ((int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6));
+  const int L = a.seq_lens[b], C = a.cur_lens[b];
+  int keys = L < a.max_pages * kQ4Tokens ? L : a.max_pages * kQ4Tokens;
+  if (p0 * kQ4Tokens >= keys || C < 1) return;
+  const int real = (C < a.T ? C : a.T) * a.group;  // rows behind it are padding
+  const int rows = a.T * a.group;
+  // rows that see the first of these keys: p0 * 16 < L - C + 1 + i
+  int i0 = p0 * kQ4Tokens - (L - C);
+  i0 = i0 > 0 ? i0 : 0;
+  const int32_t* table = a.page_table + (int64_t)b * a.pt_stride;
+  int id[2];
+  Q4Raw<HD> r;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    id[h] = p0 + h < a.max_pages ? q4_block(__builtin_amdgcn_readfirstlane(table[p0 + h]), a.num_blocks) : -1;
+    const int64_t off = ((int64_t)(id[h] >= 0 ? id[h] : 0) * a.Hk + hk) * PB;
+    q4_load_page<HD>(a.k_pool + off, a.v_pool + off, lane, r, h);
+  }
+  f16x8 kf[2][W];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) q4_k_operands<HD, PARTS>(r.k[h], kf[h]);
+  float sum[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  for (int tile = i0 * a.group / ROWS; tile * ROWS < real; ++tile) {
+    Q4Wave<HD, PARTS, 1> w;
+    q4_setup<IO, HD, PARTS, 1>(a, b, hk, tile, L, C, keys, lane, w, 0);
+    const int row = q4_row<PARTS>(tile, c);
+    const float lse = row < real && c < ROWS ? *q4_lse(a, b, hk, row < rows ? row : rows - 1) : INFINITY;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const f32x4 S = q4_scores<HD, PARTS, 1>(kf[h], r.km[h], w, 0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float p = fast_exp2(fmaf(S[i], w.sc[0], -lse));
+        sum[h][i] += row < real && c < ROWS && (p0 + h) * kQ4Tokens + 4 * g + i < w.n[0] ? p : 0.f;
+      }
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float s = group_sum<16>(sum[h][i]);
+      if (c == i && id[h] >= 0 && (p0 + h) * kQ4Tokens + 4 * g + i < keys)
+        atomicAdd(a.weights + ((int64_t)id[h] * a.Hk + hk) * kQ4Tokens + 4 * g + i, s);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------------------------
+struct Q4Plan {
+  int parts, nc, rows_per_tile;
+  bool wide;
+  int tiles, splits, split_pages;
+  int64_t rows;
+  size_t rec, lse, scores, score_stride, bytes;
+};
+
+// Which kernel, how many row tiles and key ranges, and the workspace.
+static Q4Plan q4_plan(int io_dtype, int32_t batch, int32_t heads, int32_t kv_heads, int32_t query_len, int32_t head_dim,
+                      int32_t max_pages, bool weights) {
+  Q4Plan p{};
+  p.parts = io_dtype == PA_DTYPE_F32 ? 2 : 1;
+  const int rpt = p.parts == 2 ? 8 : 16;
+  p.rows = (int64_t)query_len * (heads / kv_heads);
+  p.wide = p.rows > 2 * rpt;
+  p.nc = p.wide ? 2 : 1;
+  p.rows_per_tile = p.wide ? kQ4Waves * p.nc * rpt : rpt;
+  p.tiles = (int)((p.rows + p.rows_per_tile - 1) / p.rows_per_tile);
+  const int64_t units = (int64_t)batch * kv_heads * p.tiles;
+  const int64_t target = (p.wide ? 2 : 6) * (int64_t)pa_host::device_cu_count();
+  const int least = p.wide ? 16 : 8;  // pages per range
+  int64_t want = units > 0 ? (target + units - 1) / units : 1;
+  int pages = (int)((max_pages + want - 1) / want);
+  if (!p.wide && pages > 64) pages = 64;  // requests of very different lengths: ranges end together
+  pages = pages < least ? least : pages;
+  pages += pages & 1;
+  p.split_pages = pages;
+  p.splits = max_pages > pages ? (max_pages + pages - 1) / pages : 1;
+  p.rec = p.splits > 1 ? (size_t)batch * kv_heads * p.rows * p.splits * (head_dim + 2) : 0;
+  p.lse = weights ? (size_t)batch * kv_heads * p.rows : 0;
+  p.score_stride = (size_t)(max_pages + (max_pages & 1)) * kQ4Tokens;
+  p.scores = weights && query_len == 1 && !p.wide ? (size_t)batch * heads * p.score_stride : 0;
+  auto up = [](size_t n) { return (n + 63) / 64 * 64; };
+  p.rec = up(p.rec);
+  p.lse = up(p.lse);
+  p.bytes = (p.rec + p.lse + p.scores) * sizeof(float);
+  return p;
+}
+
+template <typename IO, int HD, int PARTS>
+static void launch_q4(const Q4Args& a, const Q4Plan& p, hipStream_t stream) {
+  const dim3 grid((unsigned)((int64_t)a.B * a.Hk * p.tiles * p.splits));
+  if (p.wide)
+    q4_attn_kernel<IO, HD, PARTS, 2, true><<<grid, 64 * kQ4Waves, 0, stream>>>(a);
+  else
+    q4_attn_kernel<IO, HD, PARTS, 1, false><<<grid, 64 * kQ4Waves, 0, stream>>>(a);
+  if (p.splits > 1) {
+    const int64_t total = (int64_t)a.B * a.Hk * a.T * a.group;
+    q4_merge_kernel<IO, HD><<<(unsigned)((total + 3) / 4), 256, 0, stream>>>(a, total);
+  }
+  if (a.weights != nullptr) {
+    if (a.scores != nullptr) {
+      const dim3 wg((unsigned)((a.max_pages * kQ4Tokens + 255) / 256), a.Hk, a.B);
+      q4_decode_weights_kernel<<<wg, 256, 0, stream>>>(a);
+    } else {
+      const dim3 wg((unsigned)((a.max_pages + 7) / 8), a.Hk, a.B);
+      q4_chunk_weights_kernel<IO, HD, PARTS><<<wg, 256, 0, stream>>>(a);
+    }
+  }
+}
+
+}  // namespace pa
+
+using namespace pa;
+
+extern "C" size_t pa_q4_attention_workspace_size(int io_dtype, int32_t batch, int32_t num_heads, int32_t kv_heads,
+                                                 int32_t query_len, int32_t head_dim, int32_t max_pages, int32_t weights) {
+  if (batch <= 0 || num_heads <= 0 || kv_heads <= 0 || num_heads % kv_heads || query_len <= 0 || max_pages <= 0 ||
+      (head_dim != 64 && head_dim != 128))
+    return 0;
+  return q4_plan(io_dtype, batch, num_heads, kv_heads, query_len, head_dim, max_pages, weights != 0).bytes;
+}
+
+extern "C" int pa_q4_attention(const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t,
+                               void* out, int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_t, int io_dtype,
+                               const void* k_pool, const void* v_pool, int64_t num_blocks,
+                               const int32_t* page_table, int64_t pt_stride, int32_t max_pages,
+                               const int32_t* seq_lens, const int32_t* cur_lens, float* weights,
+                               int32_t batch, int32_t num_heads, int32_t kv_heads, int32_t query_len, int32_t head_dim,
+                               float scale, void* workspace, size_t workspace_bytes, void* stream_) {
+  pa_host::clear_error();
+  PA_CHECK_ARG(batch >= 0 && num_heads > 0 && kv_heads > 0 && query_len >= 0 && max_pages >= 0,
+               "pa_q4_attention: bad sizes: batch=%d heads=%d kv_heads=%d query_len=%d max_pages=%d", batch, num_heads,
+               kv_heads, query_len, max_pages);
+  PA_CHECK_ARG(num_heads % kv_heads == 0, "pa_q4_attention: %d query heads are no multiple of %d KV heads", num_heads, kv_heads);
+  PA_CHECK_ARG(io_dtype == PA_DTYPE_F32 || io_dtype == PA_DTYPE_BF16, "pa_q4_attention: bad io dtype %d", io_dtype);
+  PA_CHECK_ARG(scale > 0.f && scale < INFINITY, "pa_q4_attention: scale must be positive and finite");
+  if (head_dim != 64 && head_dim != 128)
+    PA_FAIL(PA_ERR_UNSUPPORTED, "pa_q4_attention: no 4-bit pages for head_dim %d (64 and 128)", head_dim);
+  if (batch == 0 || query_len == 0) return PA_OK;
+  PA_CHECK_ARG(q && out && seq_lens && cur_lens, "pa_q4_attention: null q/out/seq_lens/cur_lens");
+  if (max_pages > 0) {
+    PA_CHECK_ARG(page_table != nullptr && pt_stride >= max_pages, "pa_q4_attention: page table missing or stride < max_pages");
+    PA_CHECK_ARG(k_pool && v_pool && num_blocks > 0, "pa_q4_attention: KV pool missing or empty");
+    PA_CHECK_ARG(((reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(v_pool)) & 15) == 0,
+                 "pa_q4_attention: the pools must be 16-byte aligned");
+  }
+  PA_CHECK_ARG(max_pages <= (1 << 26) && (int64_t)query_len * (num_heads / kv_heads) <= (1 << 26) && kv_heads <= 65535 &&
+                   batch <= 65535, "pa_q4_attention: sizes beyond the kernels' 32-bit indices");
+  const Q4Plan p = q4_plan(io_dtype, batch, num_heads, kv_heads, query_len, head_dim, max_pages, weights != nullptr && max_pages > 0);
+  PA_CHECK_ARG((int64_t)batch * kv_heads * p.tiles * p.splits <= 0x7fffffffLL, "pa_q4_attention: grid too large");
+  if (p.bytes && (workspace == nullptr || workspace_bytes < p.bytes))
+    PA_FAIL(PA_ERR_WORKSPACE, "pa_q4_attention: workspace too small: need %zu bytes, have %zu", p.bytes, workspace_bytes);
+  PA_CHECK_ARG((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "pa_q4_attention: the workspace must be 16-byte aligned");
+
+  Q4Args a{};
+  a.q = q; a.q_sb = q_stride_b; a.q_sh = q_stride_h; a.q_st = q_stride_t;
+  a.out = out; a.o_sb = out_stride_b; a.o_sh = out_stride_h; a.o_st = out_stride_t;
+  a.k_pool = static_cast<const uint8_t*>(k_pool); a.v_pool = static_cast<const uint8_t*>(v_pool);
+  a.weights = max_pages > 0 ? weights : nullptr;
+  a.num_blocks = num_blocks;
+  a.page_table = page_table; a.pt_stride = pt_stride; a.max_pages = max_pages;
+  a.seq_lens = seq_lens; a.cur_lens = cur_lens;
+  a.B = batch; a.H = num_heads; a.Hk = kv_heads; a.group = num_heads / kv_heads; a.T = query_len;
+  a.scale_log2 = scale * kLog2e;
+  a.tiles = p.tiles; a.splits = p.splits; a.split_pages = p.split_pages;
+  float* ws = static_cast<float*>(workspace);
+  a.rec = p.splits > 1 ? ws : nullptr;
+  a.lse = p.lse ? ws + p.rec : nullptr;
+  a.scores = p.scores ? ws + p.rec + p.lse : nullptr;
+  a.score_stride = (int64_t)p.score_stride;
+  hipStream_t stream = static_cast<hipStream_t>(stream_);
+  if (io_dtype == PA_DTYPE_F32) {
+    if (head_dim == 64) launch_q4<float, 64, 2>(a, p, stream); else launch_q4<float, 128, 2>(a, p, stream);
+  } else {
+    if (head_dim == 64) launch_q4<uint16_t, 64, 1>(a, p, stream); else launch_q4<uint16_t, 128, 1>(a, p, stream);
+  }
+  PA_CHECK_LAUNCH("pa_q4_attention");
+  return PA_OK;
+}

@@ -1,0 +1,280 @@
+// The 4-bit paged KV cache: rows quantised into their slots, slots read back as values (gfx950).
+#include "pa_q4.h"
+
+namespace pa {
+
+struct Q4RowArgs {
+  const void* k_new;  // append: rows in; read: rows out
+  const void* v_new;
+  int64_t sb, sh, st;
+  uint8_t* k_pool;
+  uint8_t* v_pool;
+  float* weights;  // append: the slots' running totals, cleared; may be null
+  int64_t num_blocks;
+  const int32_t* slots;
+  int32_t B, H, T;
+};
+
+// Eight lanes share a group of 64 values, lane i of them values 8 i .. 8 i + 7: the eight of one K
+// word, and two n-quadruples of V. K and V are the two halves of the grid's y axis.
+template <int HD>
+__device__ __forceinline__ void q4_row_place(int h, int H, int64_t blk, int tok, int e, uint32_t& kw, uint32_t& vw,
+                                             uint32_t& meta, int64_t& page) {
+  constexpr int G = HD / kQ4Group, W = HD / 32;
+  page = (blk * H + h) * q4_page_bytes(HD);
+  const int w = e >> 2, g = e & 3;               // values 8 e = 32 w + 8 g of the row
+  kw = (uint32_t)((tok * 4 + g) * W + w) * 4u;   // byte of the K word
+  const int a = e >> 3, r = (e & 7) * 2;         // V: group a, quadruples r and r + 1
+  vw = (uint32_t)((((tok >> 2) * 16 + r) * 2 + ((tok >> 1) & 1)) * G + a) * 4u + (uint32_t)(tok & 1) * 2u;
+  meta = (uint32_t)q4_codes_bytes(HD) + (uint32_t)(a * kQ4Tokens + tok) * 4u;
+}
+
+template <typename T>
+__device__ __forceinline__ void q4_load8(const T* p, bool vec, float (&x)[8]) {
+  if (vec) {
+    constexpr int V = 8 * (int)sizeof(T) / 16;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const u32x4 w = reinterpret_cast<const u32x4*>(p)[i];
+      float f[Vec16<T>::EPL];
+      Vec16<T>::unpack(w, f);
+#pragma unroll
+      for (int j = 0; j < Vec16<T>::EPL; ++j) x[i * Vec16<T>::EPL + j] = f[j];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = Elem<T>::load(p + j);
+  }
+}
+
+// The code of x: (x - z) / s + 7.5 to the nearest, ties to even, in 0..15. Where the quotient is below 16
+// its fp32 value is within 2e-6 of the real one (8 x 3 roundings of 2^-24, and one of the sum), so it
+// decides unless it lies within 4e-6 of a border between two codes; there (about one value in 10^5) the
+// fp64 one does. Larger quotients are clamped whatever their error.
+__device__ __forceinline__ int q4_code(float x, float z, float s, float rs) {
+  const float y = (x - z) * rs + 7.5f;
+  const float n = rintf(y);
+  if (__builtin_expect(!(fabsf(fabsf(y - n) - 0.5f) > 4e-6f), 0)) {
+    const double d = ((double)x - (double)z) / (double)s + 7.5;
+    return (int)fmin(fmax(rint(d), 0.0), 15.0);
+  }
+  return (int)fminf(fmaxf(n, 0.f), 15.f);
+}
+
+// Scale and centre of a group. The products round to fp32 before they round to halves: left to itself the
+// compiler forms product and conversion as one v_fma_mixlo_f16, which rounds once, and a scale next to a
+// border differs.
+__device__ __forceinline__ void q4_pair_of(float hi, float lo, _Float16& s, _Float16& z) {
+  float sf = (hi - lo) * (float)(1.0 / 15.0), zf = (hi + lo) * 0.5f;
+  asm("" : "+v"(sf), "+v"(zf));
+  s = (_Float16)sf;
+  z = (_Float16)zf;
+}
+
+// Quantising append: per (row, head, group) s = half((hi - lo) / 15), z = half((hi + lo) / 2) of the values
+// clamped to half's range, then the codes. Bound by HBM for long chunks (a row is read once, written
+// as 4.5 bits a value) and by latency for decode steps.
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void q4_append_kernel(const Q4RowArgs a, uint32_t total, int vec) {
+  constexpr int LPR = HD / 8;  // lanes per row
+  const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
+  if (idx >= total) return;  // (whole rows: 8 or 16 lanes each)
+  const bool is_v = blockIdx.y != 0;
+  const uint32_t rh = idx / LPR;
+  const int e = (int)(idx % LPR);
+  const uint32_t row = rh / (uint32_t)a.H;  // b * T + j
+  const int h = (int)(rh - row * (uint32_t)a.H);
+  const uint32_t b = row / (uint32_t)a.T, j = row - b * (uint32_t)a.T;
+  const int32_t slot = a.slots[row];
+  float x[8];
+  const T* src = static_cast<const T*>(is_v ? a.v_new : a.k_new) + (int64_t)b * a.sb + (int64_t)h * a.sh +
+                 (int64_t)j * a.st + 8 * e;
+  q4_load8(src, vec, x);
+  if (slot < 0) return;
+  const int64_t blk = (uint32_t)slot / kQ4Tokens;
+  if (blk >= a.num_blocks) return;
+  const int tok = slot & (kQ4Tokens - 1);
+
+  bool nan = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    nan |= x[i] != x[i];
+    x[i] = fminf(fmaxf(x[i], -65504.f), 65504.f);
+  }
+  float hi = x[0], lo = x[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) {
+    hi = fmaxf(hi, x[i]);
+    lo = fminf(lo, x[i]);
+  }
+  hi = group_max<8>(nan ? INFINITY : hi);  // a group with a NaN: (NaN, NaN)
+  lo = -group_max<8>(-lo);
+  _Float16 sh, zh;
+  q4_pair_of(hi, lo, sh, zh);
+  const bool bad = hi == INFINITY;
+  const float s = (float)sh, z = (float)zh, rs = 1.f / s;
+  uint32_t c[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c[i] = bad || !(s > 0.f) ? 0u : (uint32_t)q4_code(x[i], z, s, rs);
+
+  uint32_t kw, vw, meta;
+  int64_t page;
+  q4_row_place<HD>(h, a.H, blk, tok, e, kw, vw, meta, page);
+  uint8_t* p = (is_v ? a.v_pool : a.k_pool) + page;
+  if (!is_v) {
+    *reinterpret_cast<uint32_t*>(p + kw) = c[0] | c[2] << 4 | c[4] << 8 | c[6] << 12 | c[1] << 16 | c[3] << 20 |
+                                           c[5] << 24 | c[7] << 28;
+  } else {
+    constexpr int G = HD / kQ4Group;
+    *reinterpret_cast<uint16_t*>(p + vw) = (uint16_t)(c[0] | c[1] << 4 | c[2] << 8 | c[3] << 12);
+    *reinterpret_cast<uint16_t*>(p + vw + 8 * G) = (uint16_t)(c[4] | c[5] << 4 | c[6] << 8 | c[7] << 12);
+  }
+  if ((e & 7) == 0) {
+    const uint32_t su = bad ? 0x7e00u : (uint32_t)__builtin_bit_cast(uint16_t, sh);
+    uint32_t zu = bad ? 0x7e00u : (uint32_t)__builtin_bit_cast(uint16_t, zh);
+    zu = zu == 0x8000u ? 0u : zu;  // a centre of zero is +0, whatever zeros the row holds
+    *reinterpret_cast<uint32_t*>(p + meta) = su | zu << 16;
+  }
+  if (!is_v && e == 0 && a.weights != nullptr) a.weights[(blk * a.H + h) * kQ4Tokens + tok] = 0.f;
+}
+
+// The values that slots stand for, z + s (c - 7.5) rounded once to T; rows without a slot are zeros.
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void q4_read_kernel(const Q4RowArgs a, uint32_t total) {
+  constexpr int LPR = HD / 8;
+  const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
+  if (idx >= total) return;
+  const bool is_v = blockIdx.y != 0;
+  const uint32_t rh = idx / LPR;
+  const int e = (int)(idx % LPR);
+  const uint32_t row = rh / (uint32_t)a.H;
+  const int h = (int)(rh - row * (uint32_t)a.H);
+  const uint32_t b = row / (uint32_t)a.T, j = row - b * (uint32_t)a.T;
+  const int32_t slot = a.slots[row];
+  const int64_t blk = (uint32_t)slot / kQ4Tokens;
+  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (slot >= 0 && blk < a.num_blocks) {
+    uint32_t kw, vw, meta;
+    int64_t page;
+    q4_row_place<HD>(h, a.H, blk, slot & (kQ4Tokens - 1), e, kw, vw, meta, page);
+    const uint8_t* p = (is_v ? a.v_pool : a.k_pool) + page;
+    uint32_t c;  // nibble i: value i
+    if (!is_v) {
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(p + kw);
+      c = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) c |= (w >> (4 * ((i >> 1) + 4 * (i & 1))) & 15u) << (4 * i);
+    } else {
+      constexpr int G = HD / kQ4Group;
+      c = (uint32_t)*reinterpret_cast<const uint16_t*>(p + vw) |
+          (uint32_t)*reinterpret_cast<const uint16_t*>(p + vw + 8 * G) << 16;
+    }
+    const uint32_t m = *reinterpret_cast<const uint32_t*>(p + meta);
+    const float s = q4_scale(m), z = q4_centre(m);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = fmaf(s, (float)(c >> (4 * i) & 15u) - 7.5f, z);
+  }
+  T* out = static_cast<T*>(const_cast<void*>(is_v ? a.v_new : a.k_new)) + (int64_t)b * a.sb + (int64_t)h * a.sh +
+           (int64_t)j * a.st + 8 * e;
+  if constexpr (sizeof(T) == 4) {
+    reinterpret_cast<f32x4*>(out)[0] = f32x4{x[0], x[1], x[2], x[3]};
+    reinterpret_cast<f32x4*>(out)[1] = f32x4{x[4], x[5], x[6], x[7]};
+  } else {
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+    *reinterpret_cast<u32x4*>(out) = w;
+  }
+}
+
+template <int HD>
+static void launch_append(const Q4RowArgs& a, int dtype, int vec, hipStream_t stream) {
+  const uint32_t total = (uint32_t)((int64_t)a.B * a.T * a.H * (HD / 8));
+  const dim3 grid((total + 255) / 256, 2);
+  if (dtype == PA_DTYPE_F32)
+    q4_append_kernel<float, HD><<<grid, 256, 0, stream>>>(a, total, vec);
+  else
+    q4_append_kernel<uint16_t, HD><<<grid, 256, 0, stream>>>(a, total, vec);
+}
+
+template <int HD>
+static void launch_read(const Q4RowArgs& a, int dtype, hipStream_t stream) {
+  const uint32_t total = (uint32_t)((int64_t)a.B * a.T * a.H * (HD / 8));
+  const dim3 grid((total + 255) / 256, 2);
+  if (dtype == PA_DTYPE_F32)
+    q4_read_kernel<float, HD><<<grid, 256, 0, stream>>>(a, total);
+  else
+    q4_read_kernel<uint16_t, HD><<<grid, 256, 0, stream>>>(a, total);
+}
+
+static int check_rows(const char* what, const void* k, const void* v, int dtype, const void* k_pool, const void* v_pool,
+                      int64_t num_blocks, const int32_t* slots, int32_t batch, int32_t heads, int32_t rows,
+                      int32_t head_dim, bool& empty) {
+  PA_CHECK_ARG(batch >= 0 && rows >= 0 && heads > 0 && num_blocks >= 0, "%s: bad sizes: batch=%d rows=%d heads=%d", what,
+               batch, rows, heads);
+  PA_CHECK_ARG(dtype == PA_DTYPE_F32 || dtype == PA_DTYPE_BF16, "%s: bad dtype %d", what, dtype);
+  if (head_dim != 64 && head_dim != 128) PA_FAIL(PA_ERR_UNSUPPORTED, "%s: no 4-bit pages for head_dim %d (64 and 128)", what, head_dim);
+  empty = batch == 0 || rows == 0;
+  if (empty) return PA_OK;
+  PA_CHECK_ARG(k && v && slots, "%s: null rows or slots", what);
+  PA_CHECK_ARG(num_blocks == 0 || (k_pool && v_pool), "%s: null pool", what);
+  PA_CHECK_ARG(((reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(v_pool)) & 15) == 0,
+               "%s: the pools must be 16-byte aligned", what);
+  PA_CHECK_ARG((int64_t)batch * rows * heads * (head_dim / 8) <= 0x7fffff00LL, "%s: too many rows in one call", what);
+  return PA_OK;
+}
+
+}  // namespace pa
+
+using namespace pa;
+
+extern "C" size_t pa_q4_page_bytes(int32_t head_dim) {
+  return head_dim == 64 || head_dim == 128 ? (size_t)q4_page_bytes(head_dim) : 0;
+}
+
+extern "C" int pa_q4_append(const void* k_new, const void* v_new, int64_t new_stride_b, int64_t new_stride_h,
+                            int64_t new_stride_t, int new_dtype, void* k_pool, void* v_pool, int64_t num_blocks,
+                            float* weights, const int32_t* slot_mapping, int32_t batch, int32_t kv_heads,
+                            int32_t query_len, int32_t head_dim, void* stream) {
+  pa_host::clear_error();
+  bool empty = false;
+  if (const int st = check_rows("pa_q4_append", k_new, v_new, new_dtype, k_pool, v_pool, num_blocks, slot_mapping, batch,
+                                kv_heads, query_len, head_dim, empty))
+    return st;
+  if (empty || num_blocks == 0) return PA_OK;
+  Q4RowArgs a{k_new, v_new, new_stride_b, new_stride_h, new_stride_t, static_cast<uint8_t*>(k_pool),
+              static_cast<uint8_t*>(v_pool), weights, num_blocks, slot_mapping, batch, kv_heads, query_len};
+  const int64_t per = new_dtype == PA_DTYPE_F32 ? 4 : 8;  // elements of 16 bytes
+  const int vec = ((reinterpret_cast<uintptr_t>(k_new) | reinterpret_cast<uintptr_t>(v_new)) & 15) == 0 &&
+                  new_stride_b % per == 0 && new_stride_h % per == 0 && new_stride_t % per == 0;
+  if (head_dim == 64)
+    launch_append<64>(a, new_dtype, vec, static_cast<hipStream_t>(stream));
+  else
+    launch_append<128>(a, new_dtype, vec, static_cast<hipStream_t>(stream));
+  PA_CHECK_LAUNCH("pa_q4_append");
+  return PA_OK;
+}
+
+extern "C" int pa_q4_read(const void* k_pool, const void* v_pool, int64_t num_blocks, const int32_t* slot_mapping,
+                          void* k_out, void* v_out, int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_t,
+                          int out_dtype, int32_t batch, int32_t kv_heads, int32_t query_len, int32_t head_dim,
+                          void* stream) {
+  pa_host::clear_error();
+  bool empty = false;
+  if (const int st = check_rows("pa_q4_read", k_out, v_out, out_dtype, k_pool, v_pool, num_blocks, slot_mapping, batch,
+                                kv_heads, query_len, head_dim, empty))
+    return st;
+  if (empty) return PA_OK;
+  const int64_t per = out_dtype == PA_DTYPE_F32 ? 4 : 8;
+  PA_CHECK_ARG(((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15) == 0 &&
+                   out_stride_b % per == 0 && out_stride_h % per == 0 && out_stride_t % per == 0,
+               "pa_q4_read: the outputs must start, and their rows follow each other, at multiples of 16 bytes");
+  Q4RowArgs a{k_out, v_out, out_stride_b, out_stride_h, out_stride_t, static_cast<uint8_t*>(const_cast<void*>(k_pool)),
+              static_cast<uint8_t*>(const_cast<void*>(v_pool)), nullptr, num_blocks, slot_mapping, batch, kv_heads, query_len};
+  if (head_dim == 64)
+    launch_read<64>(a, out_dtype, static_cast<hipStream_t>(stream));
+  else
+    launch_read<128>(a, out_dtype, static_cast<hipStream_t>(stream));
+  PA_CHECK_LAUNCH("pa_q4_read");
+  return PA_OK;
+}

@@ -1,4 +1,4 @@
-"""Loader and ctypes signatures for libpaged_hip.so (declared in include/paged_hip.h).
+"""Loader and ctypes signatures for libpaged_hip.so (declared in include/paged_hip.h and paged_hip_q4.h).
 
 The library is built in-tree by `efficient-inference-system_amd/build_lib.py`. There is no
 fallback: if the library is missing or fails to load, every "hip_paged" call raises.
@@ -146,6 +146,42 @@ SIGNATURES: dict[str, tuple] = {
     ),
 }
 
+# name -> (restype, argtypes) of the 4-bit cache; mirrors include/paged_hip_q4.h one to one.
+SIGNATURES_Q4: dict[str, tuple] = {
+    "pa_q4_page_bytes": (_size_t, [_i32]),
+    "pa_q4_append": (
+        _int,
+        [_c_void_p, _c_void_p, _i64, _i64, _i64, _int,  # k new, v new, strides b, h, t, dtype
+         _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p,  # k pool, v pool, num_blocks, weights, slots
+         _i32, _i32, _i32, _i32, _c_void_p],  # batch, kv heads, query_len, head_dim, stream
+    ),
+    "pa_q4_read": (
+        _int,
+        [_c_void_p, _c_void_p, _i64, _c_void_p,  # k pool, v pool, num_blocks, slots
+         _c_void_p, _c_void_p, _i64, _i64, _i64, _int,  # k out, v out, strides b, h, t, dtype
+         _i32, _i32, _i32, _i32, _c_void_p],  # batch, kv heads, query_len, head_dim, stream
+    ),
+    "pa_q4_attention": (
+        _int,
+        [_c_void_p, _i64, _i64, _i64,  # q, strides b, h, t
+         _c_void_p, _i64, _i64, _i64, _int,  # out, strides b, h, t, io dtype
+         _c_void_p, _c_void_p, _i64,  # k pool, v pool, num_blocks
+         _c_void_p, _i64, _i32,  # page table, stride, max_pages
+         _c_void_p, _c_void_p, _c_void_p,  # seq_lens, cur_lens, weights
+         _i32, _i32, _i32, _i32, _i32,  # batch, heads, kv heads, query_len, head_dim
+         _f32, _c_void_p, _size_t, _c_void_p],  # scale, workspace, bytes, stream
+    ),
+    "pa_q4_attention_workspace_size": (_size_t, [_int, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "pa_q4_evict": (
+        _int,
+        [_c_void_p, _c_void_p, _c_void_p, _i64,  # k pool, v pool, weights, num_blocks
+         _c_void_p, _i64, _i32, _c_void_p,  # page table, stride, max_pages, seq_lens
+         _c_void_p, _i64, _i32,  # new page table, stride, max_pages
+         _i32, _i32, _c_void_p, _c_void_p,  # keep, window, kept, new seq_lens
+         _i32, _i32, _i32, _c_void_p],  # batch, kv heads, head_dim, stream
+    ),
+}
+
 # What the wrappers use beside the public entry points; mirrors csrc/pa_internal.h.
 INTERNAL: dict[str, tuple] = {
     "paged_internal_capture_id": (ctypes.c_uint64, [_c_void_p]),
@@ -173,7 +209,7 @@ def load() -> ctypes.CDLL:
                     "`python efficient-inference-system_amd/build_lib.py` (hipcc, gfx950)"
                 )
             lib = ctypes.CDLL(str(LIB_PATH))
-            for name, (restype, argtypes) in (SIGNATURES | INTERNAL).items():
+            for name, (restype, argtypes) in (SIGNATURES | SIGNATURES_Q4 | INTERNAL).items():
                 fn = getattr(lib, name)
                 fn.restype = restype
                 fn.argtypes = argtypes

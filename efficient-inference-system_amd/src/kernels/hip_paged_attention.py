@@ -100,8 +100,9 @@ def _workspace(device: torch.device, nbytes: int, kind: str) -> torch.Tensor:
 
 
 # PA_DECODE_COUNTER_BYTES and PA_PREFILL_COUNTER_BYTES in include/paged_hip.h.
-# (A balanced decode needs no initial state, but finds its tickets faster where it left them.)
-COUNTER_BYTES = {"decode": 256 << 10, "prefill": 64 << 10, "balanced": 0}
+# (A balanced decode needs no initial state, but finds its tickets faster where it left them; attention over
+# 4-bit pages keeps nothing between its calls.)
+COUNTER_BYTES = {"decode": 256 << 10, "prefill": 64 << 10, "balanced": 0, "q4": 0}
 
 
 def _capture_id(stream: int) -> int:
