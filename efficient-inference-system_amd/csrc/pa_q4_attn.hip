@@ -6,7 +6,8 @@
 // (two pages), wavefront and tile, with v_mfma_f32_16x16x32_f16 (fp32 accumulation):
 //   S^T = K Q^T   per page and group of 64 values: A = the codes (exact), B = the q rows, held as fp16 in
 //                 registers for the whole walk. s and z enter outside: S = sum_groups s (acc - 7.5 qs) +
-//                 z qs, qs = the sum of the group's q as rounded, -7.5 qs the accumulator's start.
+//                 z qs, qs = the sum of the group's q as rounded, -7.5 qs the accumulator's start (0 where
+//                 the codes are centred, below).
 //   softmax       lane (g, c) holds column c's scores of keys 4 g + i of both pages.
 //   O^T += V^T P^T  A = the codes, B = w = p s of the value's group, in the lanes that hold p. The rest of
 //                 the value, sum_keys p z - 7.5 w, is one fp32 sum per column and group.
@@ -65,15 +66,17 @@ constexpr float kQ4Limit = 32768.f;     // p * max(s, 2^-14) beyond which M is s
 constexpr float kQ4Floor = 6.103515625e-5f;  // 2^-14
 // Codes as the matrix cores take them. As fp16 subnormals (c 2^-24) they cost one AND, but the cores align
 // a product by its operands' exponents without normalising them, so that a sum keeps 7 to 10 bits fewer
-// than fp32: 2^-17 of the largest term, enough beside a bf16 result. For fp32 q (PARTS = 2) they are
-// multiplied by 2^15 (v_pk_mul_f16, one more instruction per pair), which makes them normal and the sums
-// fp32's. The error of 1024 keys' output falls from 3e-5 to what the table below says.
+// than fp32, and sums of uncentred codes cancel against 7.5 times their weights: 2^-17 of the largest term,
+// enough beside a bf16 result. For fp32 q (PARTS = 2) one v_pk_fma_f16 per pair makes them (c - 7.5) 2^-9,
+// normal and centred: 5e-7 for 1024 keys' output where the subnormals left 5e-5.
 template <int PARTS> constexpr float kQ4Unit = PARTS == 2 ? 512.f : 16777216.f;  // 1 / the value of code 1
 template <int PARTS> constexpr int kQ4UnitLog2 = PARTS == 2 ? 9 : 24;
-template <int PARTS>
-__device__ __forceinline__ uint32_t q4_pair(uint32_t masked) {
+template <int PARTS, bool ODD>
+__device__ __forceinline__ uint32_t q4_pair(uint32_t word) {
+  const uint32_t masked = word & (ODD ? kQ4Odd : kQ4Even);
   if constexpr (PARTS == 1) return masked;
-  return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, masked) * f16x2{(_Float16)32768.f, (_Float16)32768.f});
+  constexpr _Float16 up = (_Float16)32768.f, mid = (_Float16)((ODD ? -16.f : -1.f) * 7.5f / 512.f);
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(f16x2, masked), f16x2{up, up}, f16x2{mid, mid}));
 }
 
 // One step's page data of a lane.
@@ -210,7 +213,7 @@ __device__ __forceinline__ f32x4 q4_scores(const f16x8 (&kf)[HD / 32], const u32
   f32x4 S = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int k = 0; k < G; ++k) {
-    const float q0 = w.qs[nc][k], start = -7.5f * q0;
+    const float q0 = w.qs[nc][k], start = PARTS == 2 ? 0.f : -7.5f * q0;  // (PARTS = 2: the codes are centred)
     f32x4 acc = {start, start, start, start};
     acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[2 * k], w.q[nc][2 * k], acc, 0, 0, 0);
     acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[2 * k + 1], w.q[nc][2 * k + 1], acc, 0, 0, 0);
@@ -230,8 +233,8 @@ __device__ __forceinline__ void q4_k_operands(const uint32_t (&k)[HD / 32], f16x
 #pragma unroll
   for (int s = 0; s < HD / 32; ++s) {
     const uint32_t x = k[s], y = x >> 8;
-    kf[s] = q4_operand(q4_pair<PARTS>(x & kQ4Even), q4_pair<PARTS>(x & kQ4Odd), q4_pair<PARTS>(y & kQ4Even),
-                       q4_pair<PARTS>(y & kQ4Odd));
+    kf[s] = q4_operand(q4_pair<PARTS, false>(x), q4_pair<PARTS, true>(x), q4_pair<PARTS, false>(y),
+                       q4_pair<PARTS, true>(y));
   }
 }
 
@@ -247,7 +250,7 @@ __device__ __forceinline__ void q4_step(const Q4Raw<HD>& r, Q4Wave<HD, PARTS, NC
   f16x8 kf[2][W];
 #pragma unroll
   for (int h = 0; h < 2; ++h) q4_k_operands<HD, PARTS>(r.k[h], kf[h]);
-  // max(s) over the groups of V, and z - 7.5 s where w is whole (PARTS = 2)
+  // max(s) over the groups of V
   float vs[2][4];
 #pragma unroll
   for (int h = 0; h < 2; ++h)
@@ -328,7 +331,6 @@ __device__ __forceinline__ void q4_step(const Q4Raw<HD>& r, Q4Wave<HD, PARTS, NC
       for (int e = 0; e < 8; ++e) {
         _Float16 hi = (_Float16)x[e];
         if constexpr (PARTS == 2) {
-          w.y[nc][k] = fmaf(-7.5f, x[e], w.y[nc][k]);
           const _Float16 lo = (_Float16)(x[e] - (float)hi);
           b[e] = low ? lo : hi;
         } else {
@@ -342,7 +344,8 @@ __device__ __forceinline__ void q4_step(const Q4Raw<HD>& r, Q4Wave<HD, PARTS, NC
 #pragma unroll
         for (int e = 0; e < 4; ++e) {  // page e / 2, token pair e % 2
           const uint32_t x0 = r.v[e >> 1][(e & 1) * G + k];
-          o[e] = q4_pair<PARTS>((t & 2 ? x0 >> 8 : x0) & (t & 1 ? kQ4Odd : kQ4Even));
+          const uint32_t x1 = t & 2 ? x0 >> 8 : x0;
+          o[e] = t & 1 ? q4_pair<PARTS, true>(x1) : q4_pair<PARTS, false>(x1);
         }
         w.o[nc][k][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q4_operand(o[0], o[1], o[2], o[3]), b, w.o[nc][k][t], 0, 0, 0);
       }
