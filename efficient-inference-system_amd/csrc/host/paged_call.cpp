@@ -20,6 +20,7 @@
 #include <cmath>
 
 #include "paged_hip.h"
+#include "paged_hip_q4.h"
 #include "pa_internal.h"
 
 namespace {
@@ -32,6 +33,13 @@ struct Lib {
   decltype(&pa_kv_append) append = nullptr;
   decltype(&pa_linear_rows) linear = nullptr;
   decltype(&pa_qkv_append) qkv = nullptr;
+  decltype(&pa_q4_page_bytes) q4_page = nullptr;
+  decltype(&pa_q4_append) q4_append = nullptr;
+  decltype(&pa_q4_read) q4_read = nullptr;
+  decltype(&pa_q4_attention) q4_attention = nullptr;
+  decltype(&pa_q4_attention_workspace_size) q4_ws = nullptr;
+  decltype(&pa_q4_evict) q4_evict = nullptr;
+  decltype(&paged_internal_device) device = nullptr;
 };
 Lib L;
 bool ready = false;
@@ -40,7 +48,7 @@ PyObject* raw_stream = nullptr;  // torch._C._cuda_getCurrentRawStream
 PyObject* fail = nullptr;        // _lib.check(status, what)
 PyObject* side_workspace = nullptr;  // _call_workspace(device, bytes, kind): off the default stream
 PyObject* splits = nullptr;      // default_split_blocks(batch, heads, max_pages, device, ordered)
-PyObject *kind_decode, *kind_prefill, *kind_balanced, *str_device;
+PyObject *kind_decode, *kind_prefill, *kind_balanced, *kind_q4, *str_device;
 
 using Tensor = at::Tensor;
 
@@ -342,6 +350,148 @@ PyObject* qkv_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// The 4-bit cache. All operands of a call on one device, the current one (a launch on another device's
+// stream is the wrapper's, which makes it current first).
+struct Q4 {
+  const Tensor *k, *v, *w;
+  int64_t nblk, heads, Hd;
+  bool parse(PyObject* k_o, PyObject* v_o, PyObject* w_o) {
+    k = plain(k_o); v = plain(v_o);
+    if (!on_gpu(k) || !on_gpu(v) || !optional(w_o, w)) return false;
+    if (k->dim() != 3 || k->scalar_type() != at::kByte || v->scalar_type() != at::kByte || k->sizes() != v->sizes() ||
+        !k->is_contiguous() || !v->is_contiguous() || k->get_device() != L.device() || !here(v))
+      return false;
+    nblk = k->size(0); heads = k->size(1);
+    Hd = k->size(2) == (int64_t)L.q4_page(64) ? 64 : k->size(2) == (int64_t)L.q4_page(128) ? 128 : 0;
+    if (Hd == 0 || !fits32(heads) || heads == 0) return false;
+    return w == nullptr || (here(w) && w->scalar_type() == at::kFloat && w->is_contiguous() && w->dim() == 3 &&
+                            w->size(0) == nblk && w->size(1) == heads && w->size(2) == 16);
+  }
+  bool here(const Tensor* t) const { return on_gpu(t) && t->get_device() == k->get_device(); }
+  bool ints(const Tensor* t, int64_t entries) const {
+    return t != nullptr && here(t) && t->scalar_type() == at::kInt && t->is_contiguous() && t->numel() >= entries && fits32(t->numel());
+  }
+  bool table(const Tensor* t, int64_t rows) const { return ints(t, 0) && t->dim() == 2 && t->size(0) >= rows && t->size(1) > 0; }
+  float* totals() const { return w ? w->data_ptr<float>() : nullptr; }
+};
+
+// q4_append(k_new, v_new, k_pool, v_pool, slot_mapping, weights): True, or None
+PyObject* q4_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!usable(n, 6)) Py_RETURN_NONE;
+  return guarded([&]() -> PyObject* {
+    Q4 c;
+    const Tensor *kn = plain(a[0]), *vn = plain(a[1]), *sm = plain(a[4]);
+    if (!c.parse(a[2], a[3], a[5]) || kn == nullptr || vn == nullptr || !c.here(kn) || !c.here(vn) || kn->dim() != 4 ||
+        kn->sizes() != vn->sizes() || kn->scalar_type() != vn->scalar_type() || kn->strides() != vn->strides() ||
+        kn->stride(3) != 1 || dtype_of(*kn) < 0)
+      return nullptr;
+    const int64_t B = kn->size(0), H = kn->size(1), T = kn->size(2);
+    if (H != c.heads || kn->size(3) != c.Hd || !fits32(B) || !fits32(T) || !c.ints(sm, 0) || sm->numel() != B * T) return nullptr;
+    void* stream;
+    if (!stream_of(*c.k, stream)) return nullptr;
+    const int st = unlocked([&] {
+      return L.q4_append(kn->data_ptr(), vn->data_ptr(), kn->stride(0), kn->stride(1), kn->stride(2), dtype_of(*kn),
+                         c.k->data_ptr(), c.v->data_ptr(), c.nblk, c.totals(), sm->data_ptr<int>(), B, H, T, c.Hd, stream);
+    });
+    return finish(st, "pa_q4_append", Py_True, *kn);
+  });
+}
+
+// q4_read(k_pool, v_pool, slot_mapping, batch, dtype code): (k, v), or None
+PyObject* q4_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!usable(n, 5)) Py_RETURN_NONE;
+  return guarded([&]() -> PyObject* {
+    Q4 c;
+    const Tensor* sm = plain(a[2]);
+    if (!c.parse(a[0], a[1], Py_None) || !c.ints(sm, 0) || !PyLong_Check(a[3]) || !PyLong_Check(a[4])) return nullptr;
+    const int64_t B = PyLong_AsLongLong(a[3]);
+    const int dt = (int)PyLong_AsLong(a[4]);
+    if (PyErr_Occurred()) {
+      PyErr_Clear();
+      return nullptr;
+    }
+    if (B < 1 || sm->numel() % B || !fits32(B)) return nullptr;
+    const int64_t T = sm->numel() / B, H = c.heads;
+    void* stream;
+    if (!stream_of(*c.k, stream)) return nullptr;
+    const auto opt = c.k->options().dtype(dt == PA_DTYPE_F32 ? at::kFloat : at::kBFloat16);
+    const Tensor k = at::empty({B, T, H, c.Hd}, opt).transpose(1, 2), v = at::empty({B, T, H, c.Hd}, opt).transpose(1, 2);
+    const int st = unlocked([&] {
+      return L.q4_read(c.k->data_ptr(), c.v->data_ptr(), c.nblk, sm->data_ptr<int>(), k.data_ptr(), v.data_ptr(),
+                       T * H * c.Hd, c.Hd, H * c.Hd, dt, B, H, T, c.Hd, stream);
+    });
+    PyObject *ko = finish(st, "pa_q4_read", nullptr, k), *vo = ko ? THPVariable_Wrap(v) : nullptr;
+    PyObject* both = vo ? PyTuple_Pack(2, ko, vo) : nullptr;
+    Py_XDECREF(ko);
+    Py_XDECREF(vo);
+    return both;
+  });
+}
+
+// q4_attention(q, k_pool, v_pool, page_table, seq_lens, current_lengths, weights, out)
+PyObject* q4_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!usable(n, 8)) Py_RETURN_NONE;
+  return guarded([&]() -> PyObject* {
+    Q4 c;
+    const Tensor *q = plain(a[0]), *pt = plain(a[3]), *sl = plain(a[4]), *cl = plain(a[5]), *out;
+    if (!c.parse(a[1], a[2], a[6]) || q == nullptr || !c.here(q) || !optional(a[7], out) || q->dim() != 4 || dtype_of(*q) < 0 ||
+        q->stride(3) != 1)
+      return nullptr;
+    const int64_t B = q->size(0), H = q->size(1), T = q->size(2);
+    if (q->size(3) != c.Hd || H == 0 || H % c.heads || B == 0 || !fits32(B) || !fits32(H) || !fits32(T) || !c.table(pt, B) ||
+        !c.ints(sl, B) || !c.ints(cl, B))
+      return nullptr;
+    if (out != nullptr && (!c.here(out) || out->sizes() != q->sizes() || out->scalar_type() != q->scalar_type() || out->stride(3) != 1))
+      return nullptr;
+    const int dt = dtype_of(*q);
+    const int64_t pages = pt->size(1);
+    const size_t need = L.q4_ws(dt, B, H, c.heads, T, c.Hd, pages, c.w != nullptr);
+    void* stream;
+    if (!stream_of(*q, stream)) return nullptr;
+    Ref held;
+    void* ws = need ? workspace(a[0], *q, stream, kind_q4, need, held) : nullptr;
+    if (need && ws == nullptr) return nullptr;
+    const Tensor made = out ? Tensor() : at::empty_like(*q);
+    const Tensor& o = out ? *out : made;
+    const int st = unlocked([&] {
+      return L.q4_attention(q->data_ptr(), q->stride(0), q->stride(1), q->stride(2), o.data_ptr(), o.stride(0), o.stride(1),
+                            o.stride(2), dt, c.k->data_ptr(), c.v->data_ptr(), c.nblk, pt->data_ptr<int>(), pages, pages,
+                            sl->data_ptr<int>(), cl->data_ptr<int>(), c.totals(), B, H, c.heads, T, c.Hd,
+                            (float)(1.0 / std::sqrt((double)c.Hd)), ws, need, stream);
+    });
+    return finish(st, "pa_q4_attention", a[7], o);
+  });
+}
+
+// q4_evict(k_pool, v_pool, weights, page_table, seq_lens, new_page_table, keep, window): (kept, lengths), or None
+PyObject* q4_evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!usable(n, 8)) Py_RETURN_NONE;
+  return guarded([&]() -> PyObject* {
+    Q4 c;
+    const Tensor *pt = plain(a[3]), *sl = plain(a[4]), *np = plain(a[5]);
+    if (!c.parse(a[0], a[1], a[2]) || c.w == nullptr || !c.ints(sl, 1) || !PyLong_Check(a[6]) || !PyLong_Check(a[7])) return nullptr;
+    const int64_t B = sl->numel(), keep = PyLong_AsLongLong(a[6]), window = PyLong_AsLongLong(a[7]);
+    if (PyErr_Occurred()) {
+      PyErr_Clear();
+      return nullptr;
+    }
+    if (!c.table(pt, B) || !c.table(np, B) || keep < 1 || window < 0 || window > keep || !fits32(keep)) return nullptr;
+    void* stream;
+    if (!stream_of(*c.k, stream)) return nullptr;
+    const Tensor kept = at::empty({B, c.heads, keep}, sl->options()), lens = at::empty({B}, sl->options());
+    const int st = unlocked([&] {
+      return L.q4_evict(c.k->data_ptr(), c.v->data_ptr(), c.totals(), c.nblk, pt->data_ptr<int>(), pt->size(1), pt->size(1),
+                        sl->data_ptr<int>(), np->data_ptr<int>(), np->size(1), np->size(1), keep, window,
+                        kept.data_ptr<int>(), lens.data_ptr<int>(), B, c.heads, c.Hd, stream);
+    });
+    PyObject *ko = finish(st, "pa_q4_evict", nullptr, kept), *lo = ko ? THPVariable_Wrap(lens) : nullptr;
+    PyObject* both = lo ? PyTuple_Pack(2, ko, lo) : nullptr;
+    Py_XDECREF(ko);
+    Py_XDECREF(lo);
+    return both;
+  });
+}
+
 // bind({name: address}, workspaces, raw stream lookup, check, default_split_blocks, _call_workspace): the
 // functions serve calls from here on.
 PyObject* bind(PyObject*, PyObject* args) {
@@ -359,7 +509,10 @@ PyObject* bind(PyObject*, PyObject* args) {
   if (!get("pa_decode", L.decode) || !get("pa_decode_workspace_size", L.decode_ws) ||
       !get("pa_prefill", L.prefill) ||
       !get("paged_internal_prefill_workspace", L.prefill_ws) || !get("pa_kv_append", L.append) ||
-      !get("pa_linear_rows", L.linear) || !get("pa_qkv_append", L.qkv))
+      !get("pa_linear_rows", L.linear) || !get("pa_qkv_append", L.qkv) || !get("pa_q4_page_bytes", L.q4_page) ||
+      !get("pa_q4_append", L.q4_append) || !get("pa_q4_read", L.q4_read) || !get("pa_q4_attention", L.q4_attention) ||
+      !get("pa_q4_attention_workspace_size", L.q4_ws) || !get("pa_q4_evict", L.q4_evict) ||
+      !get("paged_internal_device", L.device))
     return nullptr;
   Py_INCREF(ws); Py_INCREF(rs); Py_INCREF(ck); Py_INCREF(sp); Py_INCREF(sw);
   Py_XSETREF(workspaces, ws);
@@ -382,6 +535,10 @@ PyMethodDef methods[] = {
     {"kv_append", fast(kv_append), METH_FASTCALL, "KV append of a plain call, or None."},
     {"linear_rows", fast(linear_rows), METH_FASTCALL, "Linear layer over a step's rows of a plain call, or None."},
     {"qkv_append", fast(qkv_append), METH_FASTCALL, "q/k/v projections and append of a plain call, or None."},
+    {"q4_append", fast(q4_append), METH_FASTCALL, "Append to a 4-bit cache of a plain call, or None."},
+    {"q4_read", fast(q4_read), METH_FASTCALL, "Rows of a 4-bit cache of a plain call, or None."},
+    {"q4_attention", fast(q4_attention), METH_FASTCALL, "Attention over a 4-bit cache of a plain call, or None."},
+    {"q4_evict", fast(q4_evict), METH_FASTCALL, "Eviction from a 4-bit cache of a plain call, or None."},
     {nullptr, nullptr, 0, nullptr},
 };
 
@@ -394,6 +551,7 @@ PyMODINIT_FUNC PyInit__paged_call(void) {
   kind_decode = PyUnicode_InternFromString("decode");
   kind_prefill = PyUnicode_InternFromString("prefill");
   kind_balanced = PyUnicode_InternFromString("balanced");
+  kind_q4 = PyUnicode_InternFromString("q4");
   str_device = PyUnicode_InternFromString("device");
-  return kind_decode && kind_prefill && kind_balanced && str_device ? PyModule_Create(&module) : nullptr;
+  return kind_decode && kind_prefill && kind_balanced && kind_q4 && str_device ? PyModule_Create(&module) : nullptr;
 }

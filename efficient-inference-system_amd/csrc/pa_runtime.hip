@@ -44,6 +44,11 @@ extern "C" unsigned long long paged_internal_capture_id(void* stream) {
   return status == hipStreamCaptureStatusNone ? 0 : id;
 }
 
+extern "C" int paged_internal_device(void) {
+  int dev = -1;
+  return hipGetDevice(&dev) == hipSuccess ? dev : -1;
+}
+
 extern "C" int pa_version(void) { return 100; }  // 0.1.0
 
 extern "C" const char* pa_last_error_message(void) { return pa_host::g_last_error; }

@@ -185,6 +185,7 @@ SIGNATURES_Q4: dict[str, tuple] = {
 # What the wrappers use beside the public entry points; mirrors csrc/pa_internal.h.
 INTERNAL: dict[str, tuple] = {
     "paged_internal_capture_id": (ctypes.c_uint64, [_c_void_p]),
+    "paged_internal_device": (_int, []),
     "paged_internal_prefill_workspace": (_size_t, [_int, _i32, _i32, _i32, _i32, _i32, _i32]),
 }
 
@@ -220,7 +221,7 @@ def load() -> ctypes.CDLL:
 def entry_addresses() -> dict[str, int]:
     """Entry point -> address in the loaded library."""
     lib = load()
-    return {name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in SIGNATURES | INTERNAL}
+    return {name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in SIGNATURES | SIGNATURES_Q4 | INTERNAL}
 
 
 def check(status: int, what: str) -> None:

@@ -23,7 +23,7 @@ import math
 import torch
 
 from src.kernels import _lib
-from src.kernels.hip_paged_attention import _call_workspace, _check_out, _require_i32, _stream_ptr
+from src.kernels.hip_paged_attention import _call_workspace, _check_out, _require_i32, _stream_ptr, native_call
 
 BLOCK = 16
 GROUP = 64
@@ -88,6 +88,9 @@ def kv_append_q4_hip(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Ten
                      slot_mapping: torch.Tensor, *, weights: torch.Tensor | None = None) -> None:
     """Quantise k_new/v_new [B, kv_heads, T, head_dim] (float32 or bfloat16) into their slots (slot_mapping int32
     [B * T]; -1 = skip). weights: the written slots' totals are cleared."""
+    native = native_call()
+    if native is not None and native.q4_append(k_new, v_new, k_pool, v_pool, slot_mapping, weights) is not None:
+        return
     name = "kv_append_q4_hip"
     head_dim = _check_q4_pools(name, k_pool, v_pool, weights)
     _check_device(name, k_pool.device, k_new=k_new, v_new=v_new, slot_mapping=slot_mapping)
@@ -116,13 +119,18 @@ def kv_read_q4_hip(k_pool: torch.Tensor, v_pool: torch.Tensor, slot_mapping: tor
     """The values that slots stand for: (k, v), each [batch, kv_heads, T, head_dim], for slot_mapping int32
     [batch * T]; zeros where a slot is negative or outside the pool. The tensors are views of [batch, T,
     kv_heads, head_dim] memory, the layout that the model's projections leave."""
+    code = _lib.dtype_code(dtype)
+    native = native_call()
+    if native is not None:
+        done = native.q4_read(k_pool, v_pool, slot_mapping, batch, code)
+        if done is not None:
+            return done
     name = "kv_read_q4_hip"
     head_dim = _check_q4_pools(name, k_pool, v_pool, None)
     _check_device(name, k_pool.device, slot_mapping=slot_mapping)
     _require_i32("slot_mapping", slot_mapping)
     if batch < 1 or slot_mapping.numel() % batch:
         raise ValueError(f"{name}: {slot_mapping.numel()} slots are no whole rows of {batch} requests")
-    code = _lib.dtype_code(dtype)
     H, T = k_pool.shape[1], slot_mapping.numel() // batch
     k = torch.empty((batch, T, H, head_dim), dtype=dtype, device=k_pool.device).transpose(1, 2)
     v = torch.empty((batch, T, H, head_dim), dtype=dtype, device=k_pool.device).transpose(1, 2)
@@ -173,6 +181,11 @@ def paged_attention_prefill_q4_hip(
 
 
 def _attention(name, q, k_pool, v_pool, page_table, seq_lens, current_lengths, weights, out):
+    native = native_call()
+    if native is not None:
+        done = native.q4_attention(q, k_pool, v_pool, page_table, seq_lens, current_lengths, weights, out)
+        if done is not None:
+            return done
     head_dim = _check_q4_pools(name, k_pool, v_pool, weights)
     _check_device(name, k_pool.device, q=q, page_table=page_table, seq_lens=seq_lens, current_lengths=current_lengths)
     if q.dim() != 4:
@@ -222,6 +235,11 @@ def evict_q4_hip(
     order, into the pages of new_page_table (int32 [B, pages], none of them an old page of the batch).
     Returns (kept int32 [B, kv_heads, keep], the kept keys' old indices, -1 behind the last; new lengths int32
     [B]). Old pages stay as they are, for the caller to release."""
+    native = native_call()
+    if native is not None:
+        done = native.q4_evict(k_pool, v_pool, weights, page_table, seq_lens, new_page_table, keep, window)
+        if done is not None:
+            return done
     name = "evict_q4_hip"
     head_dim = _check_q4_pools(name, k_pool, v_pool, weights)
     if weights is None:
