@@ -31,6 +31,8 @@
 //   Either splits the keys over several workgroups when the grid is small, as records (M, l, O) that
 //   q4_finish_kernel merges; it also adds the weights of decode steps up, from the scores that the first
 //   kernel left in the workspace. q4_weights_kernel does so for chunks: it forms the scores again.
+#include <utility>
+
 #include "pa_attention.h"
 #include "pa_q4.h"
 
@@ -145,16 +147,12 @@ __device__ __forceinline__ void q4_load_q(const IO* p, float (&x)[8]) {
 template <int PARTS>
 __device__ __forceinline__ int q4_row(int tile, int c) { return PARTS == 2 ? tile * 8 + (c & 7) : tile * 16 + c; }
 
-// Column tile `tile` of (request b, KV head hk): q as operands, scaled by a power of two per row.
-template <typename IO, int HD, int PARTS, int NC>
-__device__ __forceinline__ void q4_setup(const Q4Args& a, int b, int hk, int tile, int L, int C, int keys, int lane,
-                                         Q4Wave<HD, PARTS, NC>& w, int nc) {
+// q's row at `src` as operands of lane group g: scaled by a power of two so that its largest element is in
+// [2^13, 2^14), the factor taken out of sc; odd-mask slots hold a sixteenth. low: the second fp16 part.
+template <typename IO, int HD, int PARTS>
+__device__ __forceinline__ void q4_row_operands(const IO* src, bool there, bool low, int g, float scale_log2, f16x8 (&q)[HD / 32],
+                                                float (&qs)[HD / kQ4Group], float& sc) {
   constexpr int G = HD / kQ4Group, W = HD / 32;
-  const int g = lane >> 4, c = lane & 15;
-  const int row = q4_row<PARTS>(tile, c);
-  const bool there = row < a.T * a.group;
-  const int i = row / a.group, j = row - i * a.group;
-  const IO* src = static_cast<const IO*>(a.q) + (int64_t)b * a.q_sb + (int64_t)(hk * a.group + j) * a.q_sh + (int64_t)i * a.q_st;
   float x[W][8];
   float top = 0.f;
 #pragma unroll
@@ -169,7 +167,7 @@ __device__ __forceinline__ void q4_setup(const Q4Args& a, int b, int hk, int til
     for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[s][e]));
   }
   top = max_xor32(max_xor16(top));
-  // top * 2^up in [2^13, 2^14); rows of zeros, of infinities and of the last binades stay as they are
+  // rows of zeros and of infinities stay as they are
   int up = top > 0.f && top < INFINITY ? 14 - (__builtin_amdgcn_frexp_expf(top)) : 0;
   up = up > 120 ? 120 : up;
   up = up < -120 ? -120 : up;
@@ -181,17 +179,30 @@ __device__ __forceinline__ void q4_setup(const Q4Args& a, int b, int hk, int til
     f16x8 v;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float f = ldexpf(x[s][e], up - ((e & 2) ? 4 : 0));  // codes of the odd masks read 16 times as large
+      const float f = ldexpf(x[s][e], up - ((e & 2) ? 4 : 0));
       _Float16 h = (_Float16)f;
-      if (PARTS == 2 && c >= 8) h = (_Float16)(f - (float)h);
+      if (PARTS == 2 && low) h = (_Float16)(f - (float)h);
       v[e] = h;
       sum[s / 2] += (e & 2) ? 16.f * (float)h : (float)h;
     }
-    w.q[nc][s] = v;
+    q[s] = v;
   }
 #pragma unroll
-  for (int k = 0; k < G; ++k) w.qs[nc][k] = sum_xor32(sum_xor16(sum[k])) * (1.f / kQ4Unit<PARTS>);
-  w.sc[nc] = fminf(ldexpf(a.scale_log2, kQ4UnitLog2<PARTS> - up), 1e38f);
+  for (int k = 0; k < G; ++k) qs[k] = sum_xor32(sum_xor16(sum[k])) * (1.f / kQ4Unit<PARTS>);
+  sc = fminf(ldexpf(scale_log2, kQ4UnitLog2<PARTS> - up), 1e38f);
+}
+
+// Column tile `tile` of (request b, KV head hk).
+template <typename IO, int HD, int PARTS, int NC>
+__device__ __forceinline__ void q4_setup(const Q4Args& a, int b, int hk, int tile, int L, int C, int keys, int lane,
+                                         Q4Wave<HD, PARTS, NC>& w, int nc) {
+  constexpr int G = HD / kQ4Group;
+  const int g = lane >> 4, c = lane & 15;
+  const int row = q4_row<PARTS>(tile, c);
+  const bool there = row < a.T * a.group;
+  const int i = row / a.group, j = row - i * a.group;
+  const IO* src = static_cast<const IO*>(a.q) + (int64_t)b * a.q_sb + (int64_t)(hk * a.group + j) * a.q_sh + (int64_t)i * a.q_st;
+  q4_row_operands<IO, HD, PARTS>(src, there, c >= 16 / PARTS, g, a.scale_log2, w.q[nc], w.qs[nc], w.sc[nc]);
   int n = valid_keys(L, C, i);
   n = n < keys ? n : keys;
   w.n[nc] = there ? n : 0x7fffffff;
@@ -239,11 +250,9 @@ __device__ __forceinline__ void q4_k_operands(const uint32_t (&k)[HD / 32], f16x
 }
 
 // One step: 32 keys from key `key0` on. MASK: some column does not see all of them, or a page is
-// missing (live: bit h set where page h is there). scores: where to leave the log2-domain scores of
-// this lane's column, or null.
+// missing (live: bit h set where page h is there).
 template <int HD, int PARTS, int NC, bool MASK>
-__device__ __forceinline__ void q4_step(const Q4Raw<HD>& r, Q4Wave<HD, PARTS, NC>& w, int key0, int live, int lane,
-                                        float* scores) {
+__device__ __forceinline__ void q4_step(const Q4Raw<HD>& r, Q4Wave<HD, PARTS, NC>& w, int key0, int live, int lane) {
   constexpr int G = HD / kQ4Group, W = HD / 32;
   const int g = lane >> 4;
   const bool low = PARTS == 2 && (lane & 15) >= 8;
@@ -275,10 +284,6 @@ __device__ __forceinline__ void q4_step(const Q4Raw<HD>& r, Q4Wave<HD, PARTS, NC
           S[h][i] = see[h][i] ? S[h][i] : -INFINITY;
         }
       }
-    }
-    if (scores != nullptr) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) *reinterpret_cast<f32x4*>(scores + 16 * h) = S[h] * w.sc[nc];
     }
     float p[2][4], far = 0.f;
 #pragma unroll
@@ -357,7 +362,7 @@ __device__ __forceinline__ void q4_step(const Q4Raw<HD>& r, Q4Wave<HD, PARTS, NC
 // before this one's products. all: keys below it are seen by every column.
 template <int HD, int PARTS, int NC>
 __device__ __forceinline__ void q4_walk(const Q4Args& a, int b, int hk, int p0, int p1, int all, int lane,
-                                        Q4Wave<HD, PARTS, NC>& w, float* scores) {
+                                        Q4Wave<HD, PARTS, NC>& w) {
   constexpr int PB = q4_page_bytes(HD);
   if (p0 >= p1) return;
   const int32_t* table = a.page_table + (int64_t)b * a.pt_stride;
@@ -387,11 +392,10 @@ __device__ __forceinline__ void q4_walk(const Q4Args& a, int b, int hk, int p0, 
     int live_next = 0;
     if (p + 2 < p1) live_next = fetch(p + 2, next);
     const int key0 = p * kQ4Tokens;
-    float* at = scores == nullptr ? nullptr : scores + key0;
     if (live == 3 && key0 + 32 <= all)
-      q4_step<HD, PARTS, NC, false>(cur, w, key0, live, lane, at);
+      q4_step<HD, PARTS, NC, false>(cur, w, key0, live, lane);
     else
-      q4_step<HD, PARTS, NC, true>(cur, w, key0, live, lane, at);
+      q4_step<HD, PARTS, NC, true>(cur, w, key0, live, lane);
     cur = next;
     live = live_next;
   }
@@ -463,11 +467,11 @@ __device__ __forceinline__ Q4Unit q4_unit(const Q4Args& a) {
 
 constexpr int kQ4Waves = 4;
 
-template <typename IO, int HD, int PARTS, int NC, bool WIDE>
-__global__ __launch_bounds__(64 * kQ4Waves) void q4_attn_kernel(const Q4Args a) {
+// Each wavefront has NC column tiles of its own and walks all of the workgroup's keys.
+template <typename IO, int HD, int PARTS, int NC>
+__global__ __launch_bounds__(64 * kQ4Waves) void q4_wide_kernel(const Q4Args a) {
   constexpr int G = HD / kQ4Group;
-  constexpr int ROWS = PARTS == 2 ? 8 : 16;  // rows of a column tile
-  __shared__ float part[WIDE ? 1 : kQ4Waves * ROWS * (HD + 2)];
+  constexpr int ROWS = 16 / PARTS;  // rows of a column tile
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int g = lane >> 4, c = lane & 15;
   const Q4Unit u = q4_unit(a);
@@ -475,109 +479,424 @@ __global__ __launch_bounds__(64 * kQ4Waves) void q4_attn_kernel(const Q4Args a) 
   const int rows = a.T * a.group;
   int keys = L < a.max_pages * kQ4Tokens ? L : a.max_pages * kQ4Tokens;
   keys = keys > 0 ? keys : 0;
-  // the pages that the workgroup's rows see, and its share of them
-  const int first = WIDE ? u.tile * kQ4Waves * NC * ROWS : u.tile * ROWS;
-  const int my_first = WIDE ? first + wave * NC * ROWS : first;
-  const int end = my_first + NC * ROWS < rows ? my_first + NC * ROWS : rows;
+  // the pages that the wavefront's rows see, and the workgroup's share of them
+  const int first = (u.tile * kQ4Waves + wave) * NC * ROWS;
+  const int end = first + NC * ROWS < rows ? first + NC * ROWS : rows;
   int most = 0, all = 0;
-  if (my_first < rows) {
-    const int lo = my_first / a.group, hi = (end - 1) / a.group;
-    all = valid_keys(L, C, lo);
-    most = valid_keys(L, C, hi);
+  if (first < rows) {
+    all = valid_keys(L, C, first / a.group);
+    most = valid_keys(L, C, (end - 1) / a.group);
     most = most < keys ? most : keys;
     all = all < keys ? all : keys;
   }
   const int pages = (most + kQ4Tokens - 1) / kQ4Tokens;
-  int p0 = u.split * a.split_pages, p1 = a.splits > 1 ? p0 + a.split_pages : pages;
+  const int p0 = u.split * a.split_pages;
+  int p1 = a.splits > 1 ? p0 + a.split_pages : pages;
   p1 = p1 < pages ? p1 : pages;
-  if (!WIDE) {  // the wavefronts' shares, whole steps
-    const int pairs = p1 > p0 ? (p1 - p0 + 1) / 2 : 0;
-    const int per = (pairs + kQ4Waves - 1) / kQ4Waves;
-    const int s0 = p0 + 2 * per * wave;
-    p1 = s0 + 2 * per < p1 ? s0 + 2 * per : p1;
-    p0 = s0;
-  }
   Q4Wave<HD, PARTS, NC> w;
-  const int tile0 = my_first / ROWS;
+  const int tile0 = first / ROWS;
 #pragma unroll
   for (int nc = 0; nc < NC; ++nc) q4_setup<IO, HD, PARTS, NC>(a, u.b, u.hk, tile0 + nc, L, C, keys, lane, w, nc);
-  float* scores = nullptr;
-  if constexpr (!WIDE) {
-    const int row = q4_row<PARTS>(u.tile, c);
-    if (a.scores != nullptr && row < rows && c < ROWS)
-      scores = a.scores + ((int64_t)u.b * a.H + u.hk * a.group + row) * a.score_stride + 4 * g;
-  }
-  q4_walk<HD, PARTS, NC>(a, u.b, u.hk, p0, p1, all, lane, w, scores);
-
-  if constexpr (WIDE) {
+  q4_walk<HD, PARTS, NC>(a, u.b, u.hk, p0, p1, all, lane, w);
 #pragma unroll
-    for (int nc = 0; nc < NC; ++nc) {
-      const int row = q4_row<PARTS>(tile0 + nc, c);
-      float o[G][16], l;
-      q4_join<HD, PARTS, NC>(w, nc, o, l);
-      if (row >= rows || c >= ROWS) continue;
-      if (a.splits > 1) {
-        float* rec = q4_record<HD>(a, u.b, u.hk, row, u.split);
-        if (g == 0) {
-          rec[0] = w.M[nc];
-          rec[1] = l;
-        }
-#pragma unroll
-        for (int k = 0; k < G; ++k)
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            *reinterpret_cast<f32x2*>(rec + 2 + 64 * k + 16 * g + 2 * i) = f32x2{o[k][2 * i], o[k][2 * i + 1]};
-      } else {
-        const int i = row / a.group, j = row - i * a.group;
-        IO* out = static_cast<IO*>(a.out) + (int64_t)u.b * a.o_sb + (int64_t)(u.hk * a.group + j) * a.o_sh + (int64_t)i * a.o_st;
-        const float f = l > 0.f || l != l ? 1.f / l : 0.f;
-#pragma unroll
-        for (int k = 0; k < G; ++k) q4_store16<IO>(out + 64 * k + 16 * g, o[k], f);
-        if (a.lse != nullptr && g == 0) *q4_lse(a, u.b, u.hk, row) = l > 0.f ? w.M[nc] + __builtin_amdgcn_logf(l) : INFINITY;
-      }
-    }
-  } else {
+  for (int nc = 0; nc < NC; ++nc) {
+    const int row = q4_row<PARTS>(tile0 + nc, c);
     float o[G][16], l;
-    q4_join<HD, PARTS, NC>(w, 0, o, l);
-    float* mine = part + (wave * ROWS + (c & (ROWS - 1))) * (HD + 2);
-    if (c < ROWS) {
+    q4_join<HD, PARTS, NC>(w, nc, o, l);
+    if (row >= rows || c >= ROWS) continue;
+    if (a.splits > 1) {
+      float* rec = q4_record<HD>(a, u.b, u.hk, row, u.split);
       if (g == 0) {
-        mine[0] = w.M[0];
-        mine[1] = l;
+        rec[0] = w.M[nc];
+        rec[1] = l;
       }
 #pragma unroll
       for (int k = 0; k < G; ++k)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) mine[2 + 64 * k + 16 * g + i] = o[k][i];
+        for (int i = 0; i < 8; ++i)
+          *reinterpret_cast<f32x2*>(rec + 2 + 64 * k + 16 * g + 2 * i) = f32x2{o[k][2 * i], o[k][2 * i + 1]};
+    } else {
+      const int i = row / a.group, j = row - i * a.group;
+      IO* out = static_cast<IO*>(a.out) + (int64_t)u.b * a.o_sb + (int64_t)(u.hk * a.group + j) * a.o_sh + (int64_t)i * a.o_st;
+      const float f = l > 0.f || l != l ? 1.f / l : 0.f;
+#pragma unroll
+      for (int k = 0; k < G; ++k) q4_store16<IO>(out + 64 * k + 16 * g, o[k], f);
+      if (a.lse != nullptr && g == 0) *q4_lse(a, u.b, u.hk, row) = l > 0.f ? w.M[nc] + __builtin_amdgcn_logf(l) : INFINITY;
     }
-    __syncthreads();
-    const int n = rows - first < ROWS ? rows - first : ROWS;
-    for (int x = threadIdx.x; x < n * HD; x += 64 * kQ4Waves) {
-      const int r = x / HD, d = x - r * HD, row = first + r;
-      float M = kNegBig;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Up to one tile of rows (decode, short chunks). A column tile has 16 / PARTS columns, and a decode step over
+// unshared heads would fill one of them, its softmax repeated in all. So GP columns hold rows (GP the
+// rows rounded up to 1, 4 or the whole tile), q is repeated in the others, and a batch of pages goes
+// through together: page t's scores are kept by the lanes of columns GP t' .. (t' = t % PG, PG = columns / GP), where
+// softmax, scales and running sums then cost one page's work for PG pages. For the second product page t's
+// weights turn back to the first GP columns by a DPP rotation of the row; the other columns' sums are
+// never read. VALU work per key falls from about 7 to 3 instructions per lane at one row (head_dim 128).
+//
+// A batch's loads are all issued before its products, and K's registers are filled again while the second
+// product runs: 16 KB and more in flight per wavefront.
+// ---------------------------------------------------------------------------------------------
+template <int N>
+__device__ __forceinline__ uint32_t row_from(uint32_t x) {  // lane c of a 16-lane row: lane (c + N) % 16
+  if constexpr (N % 16 == 0) return x;
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x120 + (16 - N % 16), 0xF, 0xF, false);  // row_ror
+}
+template <int GP, int N = 8>
+__device__ __forceinline__ float row_max(float x) {  // over the lanes c + k GP of a row
+  if constexpr (N < GP) return x;
+  else return row_max<GP, N / 2>(fmaxf(x, dpp<0x120 + N>(x)));
+}
+template <int GP, int N = 8>
+__device__ __forceinline__ float row_sum(float x) {
+  if constexpr (N < GP) return x;
+  else return row_sum<GP, N / 2>(x + dpp<0x120 + N>(x));
+}
+
+template <int HD, int PARTS, int GP>
+struct Q4Batch {
+  static constexpr int G = HD / kQ4Group, W = HD / 32;
+  static constexpr int COLS = 16 / PARTS, PG = COLS / GP;
+  static constexpr int PAGES = PG < 4 ? 4 : PG, NB = PAGES / PG;
+  uint32_t k[PAGES][W], v[PAGES][2 * G];
+  u32x4 km[NB][G], vm[NB][G];
+  int live[NB];  // this lane's pages: 1 where the page is there
+};
+
+template <int N>
+__device__ __forceinline__ void q4_load_words(const uint8_t* p, uint32_t (&w)[N]) {
+  if constexpr (N == 4) {
+    const u32x4 x = *reinterpret_cast<const u32x4*>(p);
 #pragma unroll
-      for (int v = 0; v < kQ4Waves; ++v) M = fmaxf(M, part[(v * ROWS + r) * (HD + 2)]);
-      float l2 = 0.f, s = 0.f;
+    for (int i = 0; i < 4; ++i) w[i] = x[i];
+  } else {
+    const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+    w[0] = x[0];
+    w[1] = x[1];
+  }
+}
+
+// O^T += V^T P^T over a batch, two pages per matrix instruction.
+template <int HD, int PARTS, int GP, int... PAIRS>
+__device__ __forceinline__ void q4_narrow_values(const Q4Batch<HD, PARTS, GP>& r,
+                                                 const uint32_t (&w)[Q4Batch<HD, PARTS, GP>::NB][HD / kQ4Group][2],
+                                                 f32x4 (&o)[HD / kQ4Group][4], int cnt, std::integer_sequence<int, PAIRS...>) {
+  constexpr int G = HD / kQ4Group, PG = Q4Batch<HD, PARTS, GP>::PG;
+  auto pair = [&](auto index) {
+    constexpr int T0 = 2 * decltype(index)::value, T1 = T0 + 1;
+    if (T0 >= cnt) return;
 #pragma unroll
-      for (int v = 0; v < kQ4Waves; ++v) {
-        const float* rec = part + (v * ROWS + r) * (HD + 2);
-        const float f = fast_exp2(rec[0] - M);
-        l2 = fmaf(f, rec[1], l2);
-        s = fmaf(f, rec[2 + d], s);
-      }
-      if (a.splits > 1) {
-        float* rec = q4_record<HD>(a, u.b, u.hk, row, u.split);
-        if (d == 0) {
-          rec[0] = M;
-          rec[1] = l2;
+    for (int k = 0; k < G; ++k) {
+      const f16x8 b = q4_operand(row_from<(T0 % PG) * GP>(w[T0 / PG][k][0]), row_from<(T0 % PG) * GP>(w[T0 / PG][k][1]),
+                                 row_from<(T1 % PG) * GP>(w[T1 / PG][k][0]), row_from<(T1 % PG) * GP>(w[T1 / PG][k][1]));
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        uint32_t x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t x0 = r.v[e >> 1 ? T1 : T0][(e & 1) * G + k], x1 = t & 2 ? x0 >> 8 : x0;
+          x[e] = t & 1 ? q4_pair<PARTS, true>(x1) : q4_pair<PARTS, false>(x1);
         }
-        rec[2 + d] = s;
-      } else {
-        const int i = row / a.group, j = row - i * a.group;
-        IO* out = static_cast<IO*>(a.out) + (int64_t)u.b * a.o_sb + (int64_t)(u.hk * a.group + j) * a.o_sh + (int64_t)i * a.o_st;
-        Elem<IO>::store(out + d, l2 > 0.f || l2 != l2 ? s / l2 : 0.f);
-        if (a.lse != nullptr && d == 0) *q4_lse(a, u.b, u.hk, row) = l2 > 0.f ? M + __builtin_amdgcn_logf(l2) : INFINITY;
+        o[k][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q4_operand(x[0], x[1], x[2], x[3]), b, o[k][t], 0, 0, 0);
       }
+    }
+  };
+  (pair(std::integral_constant<int, PAIRS>()), ...);
+}
+
+template <typename IO, int HD, int PARTS, int GP>
+__global__ __launch_bounds__(64 * kQ4Waves, 2) void q4_narrow_kernel(const Q4Args a) {
+  using Batch = Q4Batch<HD, PARTS, GP>;
+  constexpr int G = Batch::G, W = Batch::W, COLS = Batch::COLS, PG = Batch::PG, PAGES = Batch::PAGES, NB = Batch::NB;
+  constexpr int PB = q4_page_bytes(HD), CB = q4_codes_bytes(HD);
+  __shared__ float part[kQ4Waves * GP * (HD + 2)];
+  __shared__ float lse_of[GP];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int g = lane >> 4, c = lane & 15, col = c & (COLS - 1);
+  const int row_in = col % GP, page_in = col / GP;  // this lane's row of the tile and page of the batch
+  const bool low = PARTS == 2 && c >= COLS;
+  const Q4Unit u = q4_unit(a);
+  const int L = a.seq_lens[u.b], C = a.cur_lens[u.b];
+  const int rows = a.T * a.group, first = u.tile * COLS;
+  const int here = rows - first < GP ? rows - first : GP;  // rows of this tile (tiles of one row set have GP = COLS)
+  int keys = L < a.max_pages * kQ4Tokens ? L : a.max_pages * kQ4Tokens;
+  keys = keys > 0 ? keys : 0;
+  int most = valid_keys(L, C, (first + here - 1) / a.group);
+  most = most < keys ? most : keys;
+  const int pages = (most + kQ4Tokens - 1) / kQ4Tokens;
+  int p0 = u.split * a.split_pages, p1 = a.splits > 1 ? p0 + a.split_pages : pages;
+  p1 = p1 < pages ? p1 : pages;
+  {  // the wavefronts' shares, an even number of pages each
+    const int per = p1 > p0 ? ((p1 - p0 + 2 * kQ4Waves - 1) / (2 * kQ4Waves)) * 2 : 0;
+    p0 += per * wave;
+    p1 = p0 + per < p1 ? p0 + per : p1;
+  }
+
+  // q: the row of this lane's column, scaled by a power of two; see q4_setup for the factors
+  const int row = first + row_in;
+  const bool there = row_in < here;
+  const int qi = row / a.group, qj = row - qi * a.group;
+  f16x8 q[W];
+  float qs[G], sc;
+  {
+    const IO* src = static_cast<const IO*>(a.q) + (int64_t)u.b * a.q_sb + (int64_t)(u.hk * a.group + qj) * a.q_sh + (int64_t)qi * a.q_st;
+    q4_row_operands<IO, HD, PARTS>(src, there, low, g, a.scale_log2, q, qs, sc);
+  }
+  int n = valid_keys(L, C, qi);
+  n = n < keys ? n : keys;
+  n = there ? n : 0;
+
+  f32x4 start[G], o[G][4];
+  float y[G], l = 0.f, M = kNegBig;
+#pragma unroll
+  for (int k = 0; k < G; ++k) {
+    const float s0 = PARTS == 2 ? 0.f : -7.5f * qs[k];
+    start[k] = f32x4{s0, s0, s0, s0};
+    y[k] = 0.f;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) o[k][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  float* scores = nullptr;
+  if (a.scores != nullptr && there && !low)
+    scores = a.scores + ((int64_t)u.b * a.H + u.hk * a.group + row) * a.score_stride + 4 * g;
+
+  if (p0 < p1) {
+    const int32_t* table = a.page_table + (int64_t)u.b * a.pt_stride;
+    const int64_t step = (int64_t)a.Hk * PB;
+    const uint8_t* kb = a.k_pool + (int64_t)u.hk * PB;
+    const uint8_t* vb = a.v_pool + (int64_t)u.hk * PB;
+    const uint32_t k_lane = (uint32_t)(c * 4 + g) * (W * 4), v_lane = (uint32_t)lane * (8 * G);
+    int ids = 0, base = p0 - 64;
+    Batch r;
+    // page ids of a batch: 64 at a time in a register, a batch never crosses them (PAGES divides 64)
+    auto next_ids = [&](int p) {
+      if (p - base >= 64) {
+        base = p;
+        const int id = p + lane < p1 ? table[p + lane] : -1;
+        ids = q4_block(id, a.num_blocks);
+      }
+    };
+    auto id_at = [&](int p, int t) {
+      const int id = __builtin_amdgcn_readlane(ids, p - base + t);
+      return id >= 0 ? id : 0;
+    };
+    auto load_k = [&](int p) {
+#pragma unroll
+      for (int t = 0; t < PAGES; ++t)
+        if (p + t < p1) q4_load_words(kb + (int64_t)id_at(p, t) * step + k_lane, r.k[t]);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const int at = __shfl(ids, p - base + nb * PG + page_in);
+        const bool live = p + nb * PG + page_in < p1 && at >= 0;
+        r.live[nb] = live;
+#pragma unroll
+        for (int k = 0; k < G; ++k) {
+          const int64_t off = (int64_t)(live ? at : 0) * step + CB + (k * kQ4Tokens + 4 * g) * 4;
+          r.km[nb][k] = *reinterpret_cast<const u32x4*>(kb + off);
+          r.vm[nb][k] = *reinterpret_cast<const u32x4*>(vb + off);
+        }
+      }
+    };
+    auto load_v = [&](int p) {
+#pragma unroll
+      for (int t = 0; t < PAGES; ++t)
+        if (p + t < p1) q4_load_words(vb + (int64_t)id_at(p, t) * step + v_lane, r.v[t]);
+    };
+    // pages behind the last leave their registers as they were: any codes, weighted with zeros
+#pragma unroll
+    for (int t = 0; t < PAGES; ++t) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) r.k[t][i] = 0;
+#pragma unroll
+      for (int i = 0; i < 2 * G; ++i) r.v[t][i] = 0;
+    }
+    next_ids(p0);
+    load_k(p0);
+    load_v(p0);
+    for (int p = p0; p < p1; p += PAGES) {
+      const int cnt = p1 - p;
+      f32x4 acc[NB][G];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int k = 0; k < G; ++k) acc[nb][k] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int t = 0; t < PAGES; ++t) {
+        if (t >= cnt) continue;
+        f16x8 kf[W];
+        q4_k_operands<HD, PARTS>(r.k[t], kf);
+#pragma unroll
+        for (int k = 0; k < G; ++k) {
+          f32x4 x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[2 * k], q[2 * k], start[k], 0, 0, 0);
+          x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[2 * k + 1], q[2 * k + 1], x, 0, 0, 0);
+          if (t % PG == 0) {
+            acc[t / PG][k] = x;
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[t / PG][k][i] = page_in == t % PG ? x[i] : acc[t / PG][k][i];
+          }
+        }
+      }
+      f32x4 S[NB];
+      bool see[NB][4];
+      u32x4 vm[NB][G];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < G; ++k) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            x[i] = fmaf(q4_scale(r.km[nb][k][i]), acc[nb][k][i],
+                        k == 0 ? q4_centre(r.km[nb][k][i]) * qs[k] : fmaf(q4_centre(r.km[nb][k][i]), qs[k], x[i]));
+          vm[nb][k] = r.vm[nb][k];
+        }
+        const int key = (p + nb * PG + page_in) * kQ4Tokens + 4 * g;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (PARTS == 2) x[i] += dpp<0x128>(x[i]);
+          see[nb][i] = r.live[nb] && key + i < n;
+          S[nb][i] = see[nb][i] ? x[i] * sc : -INFINITY;
+        }
+        if (scores != nullptr && p + nb * PG + page_in < p1)
+          *reinterpret_cast<f32x4*>(scores + (p + nb * PG + page_in) * kQ4Tokens) = S[nb];
+      }
+      if (p + PAGES < p1) {
+        next_ids(p + PAGES);
+        load_k(p + PAGES);
+      }
+      float pr[NB][4], far = 0.f;
+      float vs[NB][4];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float m = kQ4Floor;
+#pragma unroll
+          for (int k = 0; k < G; ++k) m = fmaxf(m, q4_scale(vm[nb][k][i]));
+          vs[nb][i] = see[nb][i] ? m : 0.f;
+          pr[nb][i] = fast_exp2(S[nb][i] - M);
+          far = fmaxf(far, pr[nb][i] * vs[nb][i]);
+        }
+      if (__builtin_expect(__any(far > kQ4Limit), 0)) {
+        float m = kNegBig;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            m = fmaxf(m, see[nb][i] ? S[nb][i] + __builtin_amdgcn_logf(vs[nb][i]) - kQ4Start : kNegBig);
+        m = row_max<GP>(max_xor32(max_xor16(m)));
+        const float top = fmaxf(M, m), f = fast_exp2(M - top);
+        M = top;
+        l *= f;
+#pragma unroll
+        for (int k = 0; k < G; ++k) {
+          y[k] *= f;
+#pragma unroll
+          for (int t = 0; t < 4; ++t) o[k][t] *= f;
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) pr[nb][i] = fast_exp2(S[nb][i] - M);
+      }
+      uint32_t w[NB][G][2];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) l += pr[nb][i];
+#pragma unroll
+        for (int k = 0; k < G; ++k) {
+          _Float16 h[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t m = vm[nb][k][i];
+            const float x = see[nb][i] ? pr[nb][i] * q4_scale(m) : 0.f;
+            y[k] = fmaf(pr[nb][i], see[nb][i] ? q4_centre(m) : 0.f, y[k]);
+            h[i] = (_Float16)x;
+            if constexpr (PARTS == 2) {
+              const _Float16 rest = (_Float16)(x - (float)h[i]);
+              h[i] = low ? rest : h[i];
+            } else {
+              y[k] = fmaf(-7.5f, (float)h[i], y[k]);
+            }
+          }
+          w[nb][k][0] = __builtin_bit_cast(uint32_t, f16x2{h[0], h[1]});
+          w[nb][k][1] = __builtin_bit_cast(uint32_t, f16x2{h[2], h[3]});
+        }
+      }
+      q4_narrow_values<HD, PARTS, GP>(r, w, o, cnt, std::make_integer_sequence<int, PAGES / 2>());
+      if (p + PAGES < p1) load_v(p + PAGES);
+    }
+  }
+
+  // the lanes' sums joined, the wavefronts' parts merged
+  l = row_sum<GP>(sum_xor32(sum_xor16(l))) * (1.f / PARTS);
+#pragma unroll
+  for (int k = 0; k < G; ++k) y[k] = row_sum<GP>(sum_xor32(sum_xor16(y[k]))) * (1.f / PARTS);
+  {
+    float* mine = part + (wave * GP + row_in) * (HD + 2);
+    if (c < GP) {
+      if (g == 0) {
+        mine[0] = M;
+        mine[1] = l;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < G; ++k)
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float v = o[k][t][i];
+          if constexpr (PARTS == 2) v += dpp<0x128>(v);
+          v = fmaf(v, (t & 1) ? kQ4Unit<PARTS> / 16.f : kQ4Unit<PARTS>, y[k]);
+          if (c < GP) mine[2 + 64 * k + 16 * g + 4 * i + t] = v;
+        }
+  }
+  __syncthreads();
+  for (int x = threadIdx.x; x < here * HD; x += 64 * kQ4Waves) {
+    const int r = x / HD, d = x - r * HD, m = first + r;
+    float top = kNegBig;
+#pragma unroll
+    for (int v = 0; v < kQ4Waves; ++v) top = fmaxf(top, part[(v * GP + r) * (HD + 2)]);
+    float den = 0.f, s = 0.f;
+#pragma unroll
+    for (int v = 0; v < kQ4Waves; ++v) {
+      const float* rec = part + (v * GP + r) * (HD + 2);
+      const float f = fast_exp2(rec[0] - top);
+      den = fmaf(f, rec[1], den);
+      s = fmaf(f, rec[2 + d], s);
+    }
+    if (a.splits > 1) {
+      float* rec = q4_record<HD>(a, u.b, u.hk, m, u.split);
+      if (d == 0) {
+        rec[0] = top;
+        rec[1] = den;
+      }
+      rec[2 + d] = s;
+    } else {
+      const int i = m / a.group, j = m - i * a.group;
+      IO* out = static_cast<IO*>(a.out) + (int64_t)u.b * a.o_sb + (int64_t)(u.hk * a.group + j) * a.o_sh + (int64_t)i * a.o_st;
+      Elem<IO>::store(out + d, den > 0.f || den != den ? s / den : 0.f);
+      if (a.lse != nullptr && d == 0) {
+        const float e = den > 0.f ? top + __builtin_amdgcn_logf(den) : INFINITY;
+        lse_of[r] = e;
+        *q4_lse(a, u.b, u.hk, m) = e;
+      }
+    }
+  }
+  // one workgroup has seen all keys of all the head's rows: the totals without another launch
+  if (a.scores != nullptr && a.splits == 1 && a.tiles == 1 && C > 0) {
+    __syncthreads();
+    const float* mine = a.scores + ((int64_t)u.b * a.H + u.hk * a.group) * a.score_stride;
+    for (int t = threadIdx.x; t < most; t += 64 * kQ4Waves) {
+      const int id = q4_block(a.page_table[(int64_t)u.b * a.pt_stride + t / kQ4Tokens], a.num_blocks);
+      if (id < 0) continue;
+      float sum = 0.f;
+      for (int j = 0; j < here; ++j) sum += fast_exp2(mine[j * a.score_stride + t] - lse_of[j]);
+      atomicAdd(a.weights + ((int64_t)id * a.Hk + u.hk) * kQ4Tokens + (t & (kQ4Tokens - 1)), sum);
     }
   }
 }
@@ -707,13 +1026,13 @@ static Q4Plan q4_plan(int io_dtype, int32_t batch, int32_t heads, int32_t kv_hea
   p.rows_per_tile = p.wide ? kQ4Waves * p.nc * rpt : rpt;
   p.tiles = (int)((p.rows + p.rows_per_tile - 1) / p.rows_per_tile);
   const int64_t units = (int64_t)batch * kv_heads * p.tiles;
-  const int64_t target = (p.wide ? 2 : 6) * (int64_t)pa_host::device_cu_count();
-  const int least = p.wide ? 16 : 8;  // pages per range
-  int64_t want = units > 0 ? (target + units - 1) / units : 1;
+  const int64_t target = 2 * (int64_t)pa_host::device_cu_count();
+  const int64_t want = units > 0 ? (target + units - 1) / units : 1;
   int pages = (int)((max_pages + want - 1) / want);
-  if (!p.wide && pages > 64) pages = 64;  // requests of very different lengths: ranges end together
+  const int least = p.wide ? 16 : 64;
+  if (!p.wide && pages > 128) pages = 128;  // requests of very different lengths: ranges end together
   pages = pages < least ? least : pages;
-  pages += pages & 1;
+  pages = (pages + 7) / 8 * 8;
   p.split_pages = pages;
   p.splits = max_pages > pages ? (max_pages + pages - 1) / pages : 1;
   p.rec = p.splits > 1 ? (size_t)batch * kv_heads * p.rows * p.splits * (head_dim + 2) : 0;
@@ -731,15 +1050,20 @@ template <typename IO, int HD, int PARTS>
 static void launch_q4(const Q4Args& a, const Q4Plan& p, hipStream_t stream) {
   const dim3 grid((unsigned)((int64_t)a.B * a.Hk * p.tiles * p.splits));
   if (p.wide)
-    q4_attn_kernel<IO, HD, PARTS, 2, true><<<grid, 64 * kQ4Waves, 0, stream>>>(a);
+    q4_wide_kernel<IO, HD, PARTS, 2><<<grid, 64 * kQ4Waves, 0, stream>>>(a);
+  else if (p.rows == 1)
+    q4_narrow_kernel<IO, HD, PARTS, 1><<<grid, 64 * kQ4Waves, 0, stream>>>(a);
+  else if (p.rows <= 4)
+    q4_narrow_kernel<IO, HD, PARTS, 4><<<grid, 64 * kQ4Waves, 0, stream>>>(a);
   else
-    q4_attn_kernel<IO, HD, PARTS, 1, false><<<grid, 64 * kQ4Waves, 0, stream>>>(a);
+    q4_narrow_kernel<IO, HD, PARTS, 16 / PARTS><<<grid, 64 * kQ4Waves, 0, stream>>>(a);
   if (p.splits > 1) {
     const int64_t total = (int64_t)a.B * a.Hk * a.T * a.group;
     q4_merge_kernel<IO, HD><<<(unsigned)((total + 3) / 4), 256, 0, stream>>>(a, total);
   }
   if (a.weights != nullptr) {
     if (a.scores != nullptr) {
+      if (p.splits == 1 && p.tiles == 1) return;  // done in place
       const dim3 wg((unsigned)((a.max_pages * kQ4Tokens + 255) / 256), a.Hk, a.B);
       q4_decode_weights_kernel<<<wg, 256, 0, stream>>>(a);
     } else {
