@@ -31,6 +31,7 @@
 //   Either splits the keys over several workgroups when the grid is small, as records (M, l, O) that
 //   q4_finish_kernel merges; it also adds the weights of decode steps up, from the scores that the first
 //   kernel left in the workspace. q4_weights_kernel does so for chunks: it forms the scores again.
+#include <type_traits>
 #include <utility>
 
 #include "pa_attention.h"
@@ -493,6 +494,7 @@ __global__ __launch_bounds__(64 * kQ4Waves) void q4_wide_kernel(const Q4Args a) 
   const int p0 = u.split * a.split_pages;
   int p1 = a.splits > 1 ? p0 + a.split_pages : pages;
   p1 = p1 < pages ? p1 : pages;
+  if (a.splits > 1 && p0 >= p1) return;  // no record: the merge knows how far each row's pages reach
   Q4Wave<HD, PARTS, NC> w;
   const int tile0 = first / ROWS;
 #pragma unroll
@@ -557,7 +559,8 @@ __device__ __forceinline__ float row_sum(float x) {
 template <int HD, int PARTS, int GP>
 struct Q4Batch {
   static constexpr int G = HD / kQ4Group, W = HD / 32;
-  static constexpr int COLS = 16 / PARTS, PG = COLS / GP;
+  // pages that share a softmax: 8 at most, which 190 registers hold at head_dim 128 (16 spill)
+  static constexpr int COLS = 16 / PARTS, PG = COLS / GP < 8 ? COLS / GP : 8;
   static constexpr int PAGES = PG < 4 ? 4 : PG, NB = PAGES / PG;
   uint32_t k[PAGES][W], v[PAGES][2 * G];
   u32x4 km[NB][G], vm[NB][G];
@@ -578,14 +581,14 @@ __device__ __forceinline__ void q4_load_words(const uint8_t* p, uint32_t (&w)[N]
 }
 
 // O^T += V^T P^T over a batch, two pages per matrix instruction.
-template <int HD, int PARTS, int GP, int... PAIRS>
+template <int HD, int PARTS, int GP, bool LAST, int... PAIRS>
 __device__ __forceinline__ void q4_narrow_values(const Q4Batch<HD, PARTS, GP>& r,
                                                  const uint32_t (&w)[Q4Batch<HD, PARTS, GP>::NB][HD / kQ4Group][2],
                                                  f32x4 (&o)[HD / kQ4Group][4], int cnt, std::integer_sequence<int, PAIRS...>) {
   constexpr int G = HD / kQ4Group, PG = Q4Batch<HD, PARTS, GP>::PG;
   auto pair = [&](auto index) {
     constexpr int T0 = 2 * decltype(index)::value, T1 = T0 + 1;
-    if (T0 >= cnt) return;
+    if (LAST && T0 >= cnt) return;
 #pragma unroll
     for (int k = 0; k < G; ++k) {
       const f16x8 b = q4_operand(row_from<(T0 % PG) * GP>(w[T0 / PG][k][0]), row_from<(T0 % PG) * GP>(w[T0 / PG][k][1]),
@@ -614,7 +617,8 @@ __global__ __launch_bounds__(64 * kQ4Waves, 2) void q4_narrow_kernel(const Q4Arg
   __shared__ float lse_of[GP];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int g = lane >> 4, c = lane & 15, col = c & (COLS - 1);
-  const int row_in = col % GP, page_in = col / GP;  // this lane's row of the tile and page of the batch
+  const int row_in = col % GP, page_in = col / GP % PG;  // this lane's row of the tile and page of the batch
+  const bool spare = col / GP >= PG;                     // (columns beyond the batch's pages)
   const bool low = PARTS == 2 && c >= COLS;
   const Q4Unit u = q4_unit(a);
   const int L = a.seq_lens[u.b], C = a.cur_lens[u.b];
@@ -627,6 +631,7 @@ __global__ __launch_bounds__(64 * kQ4Waves, 2) void q4_narrow_kernel(const Q4Arg
   const int pages = (most + kQ4Tokens - 1) / kQ4Tokens;
   int p0 = u.split * a.split_pages, p1 = a.splits > 1 ? p0 + a.split_pages : pages;
   p1 = p1 < pages ? p1 : pages;
+  if (a.splits > 1 && p0 >= p1) return;  // no record: the merge knows how far the rows' pages reach
   {  // the wavefronts' shares, an even number of pages each
     const int per = p1 > p0 ? ((p1 - p0 + 2 * kQ4Waves - 1) / (2 * kQ4Waves)) * 2 : 0;
     p0 += per * wave;
@@ -658,7 +663,7 @@ __global__ __launch_bounds__(64 * kQ4Waves, 2) void q4_narrow_kernel(const Q4Arg
     for (int t = 0; t < 4; ++t) o[k][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   float* scores = nullptr;
-  if (a.scores != nullptr && there && !low)
+  if (a.scores != nullptr && there && !low && !spare)
     scores = a.scores + ((int64_t)u.b * a.H + u.hk * a.group + row) * a.score_stride + 4 * g;
 
   if (p0 < p1) {
@@ -677,18 +682,20 @@ __global__ __launch_bounds__(64 * kQ4Waves, 2) void q4_narrow_kernel(const Q4Arg
         ids = q4_block(id, a.num_blocks);
       }
     };
+    // (a last batch of fewer pages reads its last one again: loads under branches would make every wait for
+    // one a wait for all)
     auto id_at = [&](int p, int t) {
-      const int id = __builtin_amdgcn_readlane(ids, p - base + t);
+      const int at = p + t < p1 ? p + t : p1 - 1;
+      const int id = __builtin_amdgcn_readlane(ids, at - base);
       return id >= 0 ? id : 0;
     };
     auto load_k = [&](int p) {
 #pragma unroll
-      for (int t = 0; t < PAGES; ++t)
-        if (p + t < p1) q4_load_words(kb + (int64_t)id_at(p, t) * step + k_lane, r.k[t]);
+      for (int t = 0; t < PAGES; ++t) q4_load_words(kb + (int64_t)id_at(p, t) * step + k_lane, r.k[t]);
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         const int at = __shfl(ids, p - base + nb * PG + page_in);
-        const bool live = p + nb * PG + page_in < p1 && at >= 0;
+        const bool live = p + nb * PG + page_in < p1 && at >= 0 && !spare;
         r.live[nb] = live;
 #pragma unroll
         for (int k = 0; k < G; ++k) {
@@ -700,22 +707,11 @@ __global__ __launch_bounds__(64 * kQ4Waves, 2) void q4_narrow_kernel(const Q4Arg
     };
     auto load_v = [&](int p) {
 #pragma unroll
-      for (int t = 0; t < PAGES; ++t)
-        if (p + t < p1) q4_load_words(vb + (int64_t)id_at(p, t) * step + v_lane, r.v[t]);
+      for (int t = 0; t < PAGES; ++t) q4_load_words(vb + (int64_t)id_at(p, t) * step + v_lane, r.v[t]);
     };
-    // pages behind the last leave their registers as they were: any codes, weighted with zeros
-#pragma unroll
-    for (int t = 0; t < PAGES; ++t) {
-#pragma unroll
-      for (int i = 0; i < W; ++i) r.k[t][i] = 0;
-#pragma unroll
-      for (int i = 0; i < 2 * G; ++i) r.v[t][i] = 0;
-    }
-    next_ids(p0);
-    load_k(p0);
-    load_v(p0);
-    for (int p = p0; p < p1; p += PAGES) {
-      const int cnt = p1 - p;
+    auto batch = [&](int p, auto is_last) {
+      constexpr bool LAST = decltype(is_last)::value;
+      const int cnt = LAST ? p1 - p : PAGES;
       f32x4 acc[NB][G];
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
@@ -723,7 +719,7 @@ __global__ __launch_bounds__(64 * kQ4Waves, 2) void q4_narrow_kernel(const Q4Arg
         for (int k = 0; k < G; ++k) acc[nb][k] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int t = 0; t < PAGES; ++t) {
-        if (t >= cnt) continue;
+        if (LAST && t >= cnt) continue;
         f16x8 kf[W];
         q4_k_operands<HD, PARTS>(r.k[t], kf);
 #pragma unroll
@@ -762,7 +758,7 @@ __global__ __launch_bounds__(64 * kQ4Waves, 2) void q4_narrow_kernel(const Q4Arg
         if (scores != nullptr && p + nb * PG + page_in < p1)
           *reinterpret_cast<f32x4*>(scores + (p + nb * PG + page_in) * kQ4Tokens) = S[nb];
       }
-      if (p + PAGES < p1) {
+      if constexpr (!LAST) {
         next_ids(p + PAGES);
         load_k(p + PAGES);
       }
@@ -826,9 +822,15 @@ __global__ __launch_bounds__(64 * kQ4Waves, 2) void q4_narrow_kernel(const Q4Arg
           w[nb][k][1] = __builtin_bit_cast(uint32_t, f16x2{h[2], h[3]});
         }
       }
-      q4_narrow_values<HD, PARTS, GP>(r, w, o, cnt, std::make_integer_sequence<int, PAGES / 2>());
-      if (p + PAGES < p1) load_v(p + PAGES);
-    }
+      q4_narrow_values<HD, PARTS, GP, LAST>(r, w, o, cnt, std::make_integer_sequence<int, PAGES / 2>());
+      if constexpr (!LAST) load_v(p + PAGES);
+    };
+    next_ids(p0);
+    load_k(p0);
+    load_v(p0);
+    int p = p0;
+    for (; p + PAGES < p1; p += PAGES) batch(p, std::false_type());
+    batch(p, std::true_type());
   }
 
   // the lanes' sums joined, the wavefronts' parts merged
@@ -901,6 +903,13 @@ __global__ __launch_bounds__(64 * kQ4Waves, 2) void q4_narrow_kernel(const Q4Arg
   }
 }
 
+// Key ranges that hold keys of query position i.
+__device__ __forceinline__ int q4_splits_of(const Q4Args& a, int b, int i) {
+  int n = valid_keys(a.seq_lens[b], a.cur_lens[b], i);
+  n = n < a.max_pages * kQ4Tokens ? n : a.max_pages * kQ4Tokens;
+  return (n + a.split_pages * kQ4Tokens - 1) / (a.split_pages * kQ4Tokens);
+}
+
 // Records of a row's splits -> its output and log2 denominator. One wavefront per row.
 template <typename IO, int HD>
 __global__ __launch_bounds__(256) void q4_merge_kernel(const Q4Args a, int64_t total) {
@@ -911,20 +920,21 @@ __global__ __launch_bounds__(256) void q4_merge_kernel(const Q4Args a, int64_t t
   const int row = (int)(x % rows);
   const int hk = (int)(x / rows % a.Hk), b = (int)(x / rows / a.Hk);
   const float* rec = q4_record<HD>(a, b, hk, row, 0);
+  const int i = row / a.group, j = row - i * a.group;
+  const int splits = q4_splits_of(a, b, i);
   float M = kNegBig;
-  for (int s = 0; s < a.splits; ++s) M = fmaxf(M, rec[(int64_t)s * (HD + 2)]);
+  for (int s = 0; s < splits; ++s) M = fmaxf(M, rec[(int64_t)s * (HD + 2)]);
   constexpr int E = HD / 64;
   float l = 0.f, o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
-  for (int s = 0; s < a.splits; ++s) {
+  for (int s = 0; s < splits; ++s) {
     const float* p = rec + (int64_t)s * (HD + 2);
     const float f = fast_exp2(p[0] - M);
     l = fmaf(f, p[1], l);
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = fmaf(f, p[2 + lane + 64 * e], o[e]);
   }
-  const int i = row / a.group, j = row - i * a.group;
   IO* out = static_cast<IO*>(a.out) + (int64_t)b * a.o_sb + (int64_t)(hk * a.group + j) * a.o_sh + (int64_t)i * a.o_st;
 #pragma unroll
   for (int e = 0; e < E; ++e) Elem<IO>::store(out + lane + 64 * e, l > 0.f || l != l ? o[e] / l : 0.f);
