@@ -138,6 +138,11 @@ __device__ __forceinline__ void stage_load16(const void* base, uint32_t voff, co
   const uint32_t m0 = (uint32_t)(size_t)(const __attribute__((address_space(3))) void*)lds;
   asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "{m0}"(m0) : "memory");
 }
+// The same from an address of each lane's own.
+__device__ __forceinline__ void stage_load16_at(const void* src, const void* lds) {
+  const uint32_t m0 = (uint32_t)(size_t)(const __attribute__((address_space(3))) void*)lds;
+  asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(m0) : "memory");
+}
 // Wait until at most N vector memory loads of this wavefront are outstanding.
 template <int N>
 __device__ __forceinline__ void vm_wait() {

@@ -25,12 +25,13 @@
 // inside fp16, above its subnormals for keys within 2^-18 of the heaviest. M cancels in O / l.
 //
 // Kernels:
-//   q4_attn_kernel<WIDE = false>  up to one tile of rows: the workgroup's wavefronts split the keys and
-//                 merge in LDS (decode, short chunks).
-//   q4_attn_kernel<WIDE = true>   each wavefront has NC tiles of its own and walks all keys.
+//   q4_narrow_kernel  up to one tile of rows: the workgroup's wavefronts split the keys and merge in LDS
+//                     (decode, short chunks).
+//   q4_wide_kernel    each wavefront has a tile of its own, and the workgroup's walk all keys together,
+//                     staged through LDS.
 //   Either splits the keys over several workgroups when the grid is small, as records (M, l, O) that
-//   q4_finish_kernel merges; it also adds the weights of decode steps up, from the scores that the first
-//   kernel left in the workspace. q4_weights_kernel does so for chunks: it forms the scores again.
+//   q4_finish_kernel merges; it also adds the weights of decode steps up. q4_chunk_weights_kernel does so for
+//   chunks: it forms the scores again.
 #include <type_traits>
 #include <utility>
 
@@ -74,6 +75,7 @@ constexpr float kQ4Floor = 6.103515625e-5f;  // 2^-14
 // normal and centred: 5e-7 for 1024 keys' output where the subnormals left 5e-5.
 template <int PARTS> constexpr float kQ4Unit = PARTS == 2 ? 512.f : 16777216.f;  // 1 / the value of code 1
 template <int PARTS> constexpr int kQ4UnitLog2 = PARTS == 2 ? 9 : 24;
+typedef __fp16 h16x2 __attribute__((ext_vector_type(2)));  // v_dot2_f32_f16's operand
 template <int PARTS, bool ODD>
 __device__ __forceinline__ uint32_t q4_pair(uint32_t word) {
   const uint32_t masked = word & (ODD ? kQ4Odd : kQ4Even);
@@ -119,16 +121,16 @@ __device__ __forceinline__ void q4_load_page(const uint8_t* kp, const uint8_t* v
   }
 }
 
-// A wavefront's columns: operands, sums and running state of NC tiles.
-template <int HD, int PARTS, int NC>
+// A wavefront's column tile: operands, sums and running state.
+template <int HD, int PARTS>
 struct Q4Wave {
   static constexpr int G = HD / kQ4Group, W = HD / 32;
-  f16x8 q[NC][W];
-  float qs[NC][G];  // sum of the group's q operands (units of code 1)
-  float sc[NC];     // log2-domain score of such a unit
-  int n[NC];        // keys the column sees (a column without a row: 0x7fffffff)
-  f32x4 o[NC][G][4];
-  float y[NC][G], M[NC], l[NC];
+  f16x8 q[W];
+  float qs[G];  // sum of the group's q operands (units of code 1)
+  float sc;     // log2-domain score of such a unit
+  int n;        // keys the column sees (a column without a row: 0x7fffffff)
+  f32x4 o[G][4];
+  float y[G], M, l;
 };
 
 template <typename IO>
@@ -194,41 +196,41 @@ __device__ __forceinline__ void q4_row_operands(const IO* src, bool there, bool 
 }
 
 // Column tile `tile` of (request b, KV head hk).
-template <typename IO, int HD, int PARTS, int NC>
+template <typename IO, int HD, int PARTS>
 __device__ __forceinline__ void q4_setup(const Q4Args& a, int b, int hk, int tile, int L, int C, int keys, int lane,
-                                         Q4Wave<HD, PARTS, NC>& w, int nc) {
+                                         Q4Wave<HD, PARTS>& w) {
   constexpr int G = HD / kQ4Group;
   const int g = lane >> 4, c = lane & 15;
   const int row = q4_row<PARTS>(tile, c);
   const bool there = row < a.T * a.group;
   const int i = row / a.group, j = row - i * a.group;
   const IO* src = static_cast<const IO*>(a.q) + (int64_t)b * a.q_sb + (int64_t)(hk * a.group + j) * a.q_sh + (int64_t)i * a.q_st;
-  q4_row_operands<IO, HD, PARTS>(src, there, c >= 16 / PARTS, g, a.scale_log2, w.q[nc], w.qs[nc], w.sc[nc]);
+  q4_row_operands<IO, HD, PARTS>(src, there, c >= 16 / PARTS, g, a.scale_log2, w.q, w.qs, w.sc);
   int n = valid_keys(L, C, i);
   n = n < keys ? n : keys;
-  w.n[nc] = there ? n : 0x7fffffff;
-  w.M[nc] = kNegBig;
-  w.l[nc] = 0.f;
+  w.n = there ? n : 0x7fffffff;
+  w.M = kNegBig;
+  w.l = 0.f;
 #pragma unroll
   for (int k = 0; k < G; ++k) {
-    w.y[nc][k] = 0.f;
+    w.y[k] = 0.f;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) w.o[nc][k][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < 4; ++t) w.o[k][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 }
 
-// Scores (units of code 1) of one page: lane (g, c) gets keys 4 g + i of its column.
-template <int HD, int PARTS, int NC>
-__device__ __forceinline__ f32x4 q4_scores(const f16x8 (&kf)[HD / 32], const u32x4 (&km)[HD / kQ4Group],
-                                           const Q4Wave<HD, PARTS, NC>& w, int nc) {
+// Scores (units of code 1) of one page against q's operands: lane (g, c) gets keys 4 g + i of its column.
+template <int HD, int PARTS>
+__device__ __forceinline__ f32x4 q4_scores(const f16x8 (&kf)[HD / 32], const u32x4 (&km)[HD / kQ4Group], const f16x8 (&q)[HD / 32],
+                                           const float (&qs)[HD / kQ4Group]) {
   constexpr int G = HD / kQ4Group;
   f32x4 S = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int k = 0; k < G; ++k) {
-    const float q0 = w.qs[nc][k], start = PARTS == 2 ? 0.f : -7.5f * q0;  // (PARTS = 2: the codes are centred)
+    const float q0 = qs[k], start = PARTS == 2 ? 0.f : -7.5f * q0;  // (PARTS = 2: the codes are centred)
     f32x4 acc = {start, start, start, start};
-    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[2 * k], w.q[nc][2 * k], acc, 0, 0, 0);
-    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[2 * k + 1], w.q[nc][2 * k + 1], acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[2 * k], q[2 * k], acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[2 * k + 1], q[2 * k + 1], acc, 0, 0, 0);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       S[i] = fmaf(q4_scale(km[k][i]), acc[i], k == 0 ? q4_centre(km[k][i]) * q0 : fmaf(q4_centre(km[k][i]), q0, S[i]));
@@ -250,172 +252,183 @@ __device__ __forceinline__ void q4_k_operands(const uint32_t (&k)[HD / 32], f16x
   }
 }
 
-// One step: 32 keys from key `key0` on. MASK: some column does not see all of them, or a page is
-// missing (live: bit h set where page h is there).
-template <int HD, int PARTS, int NC, bool MASK>
-__device__ __forceinline__ void q4_step(const Q4Raw<HD>& r, Q4Wave<HD, PARTS, NC>& w, int key0, int live, int lane) {
-  constexpr int G = HD / kQ4Group, W = HD / 32;
+// A page in LDS: K codes, V codes, K pairs, V pairs, as the wide kernel stages them.
+template <int HD>
+struct Q4Staged {
+  static constexpr int G = HD / kQ4Group, W = HD / 32, CODES = q4_codes_bytes(HD), META = kQ4Tokens * 4 * G;
+  static constexpr int BYTES = 2 * (CODES + META);
+  // head_dim 128: K's 16-byte words come in lane order, so that lane L reads bytes 16 L .. (no bank twice)
+  __device__ static __forceinline__ void k_words(const uint8_t* p, int lane, uint32_t (&x)[W]) {
+    const int g = lane >> 4, c = lane & 15;
+    q4_lds_words(p + (HD == 128 ? lane * 16 : (c * 4 + g) * 8), x);
+  }
+  __device__ static __forceinline__ void v_words(const uint8_t* p, int lane, uint32_t (&x)[2 * G]) {
+    q4_lds_words(p + CODES + lane * 8 * G, x);
+  }
+  __device__ static __forceinline__ u32x4 k_pairs(const uint8_t* p, int g, int k) {
+    return *reinterpret_cast<const u32x4*>(p + 2 * CODES + (k * kQ4Tokens + 4 * g) * 4);
+  }
+  __device__ static __forceinline__ u32x4 v_pairs(const uint8_t* p, int g, int k) {
+    return *reinterpret_cast<const u32x4*>(p + 2 * CODES + META + (k * kQ4Tokens + 4 * g) * 4);
+  }
+  template <int N>
+  __device__ static __forceinline__ void q4_lds_words(const uint8_t* p, uint32_t (&x)[N]) {
+    if constexpr (N == 4) {
+      const u32x4 v = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = v[i];
+    } else {
+      const u32x2 v = *reinterpret_cast<const u32x2*>(p);
+      x[0] = v[0];
+      x[1] = v[1];
+    }
+  }
+};
+
+// One step: the two pages at pg (in LDS), 32 keys from key `key0` on. masked: the column may not see all of
+// them, or a page is missing (live: bit h set where page h is there). What a column does not see takes part
+// with score -inf and the pair (0, 0), so that nothing in its place reaches the sums.
+template <int HD, int PARTS>
+__device__ __forceinline__ void q4_step(const uint8_t* pg, Q4Wave<HD, PARTS>& w, int key0, bool masked, int live, int lane) {
+  using P = Q4Staged<HD>;
+  constexpr int G = P::G, W = P::W;
   const int g = lane >> 4;
   const bool low = PARTS == 2 && (lane & 15) >= 8;
-  f16x8 kf[2][W];
+  f32x4 S[2];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) q4_k_operands<HD, PARTS>(r.k[h], kf[h]);
-  // max(s) over the groups of V
-  float vs[2][4];
+  for (int h = 0; h < 2; ++h) {
+    uint32_t kw[W];
+    P::k_words(pg + h * P::BYTES, lane, kw);
+    f16x8 kf[W];
+    q4_k_operands<HD, PARTS>(kw, kf);
+    u32x4 km[G];
+#pragma unroll
+    for (int k = 0; k < G; ++k) km[k] = P::k_pairs(pg + h * P::BYTES, g, k);
+    S[h] = q4_scores<HD, PARTS>(kf, km, w.q, w.qs);
+  }
+  u32x4 vm[2][G];
 #pragma unroll
   for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float m = kQ4Floor;
-#pragma unroll
-      for (int k = 0; k < G; ++k) m = fmaxf(m, q4_scale(r.vm[h][k][i]));
-      vs[h][i] = m;
-    }
-#pragma unroll
-  for (int nc = 0; nc < NC; ++nc) {
-    f32x4 S[2];
-    bool see[2][4];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      S[h] = q4_scores<HD, PARTS, NC>(kf[h], r.km[h], w, nc);
-      if constexpr (MASK) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          see[h][i] = (live >> h & 1) && key0 + 16 * h + 4 * g + i < w.n[nc];
-          S[h][i] = see[h][i] ? S[h][i] : -INFINITY;
-        }
-      }
-    }
-    float p[2][4], far = 0.f;
+    for (int k = 0; k < G; ++k) vm[h][k] = P::v_pairs(pg + h * P::BYTES, g, k);
+  if (masked) {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        p[h][i] = fast_exp2(fmaf(S[h][i], w.sc[nc], -w.M[nc]));
-        far = fmaxf(far, p[h][i] * (MASK && !see[h][i] ? 0.f : vs[h][i]));
+        const bool see = (live >> h & 1) && key0 + 16 * h + 4 * g + i < w.n;
+        S[h][i] = see ? S[h][i] : -INFINITY;
+#pragma unroll
+        for (int k = 0; k < G; ++k) vm[h][k][i] = see ? vm[h][k][i] : 0u;
       }
-    if (__builtin_expect(__any(far > kQ4Limit), 0)) {
-      float m = kNegBig;
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float u = fmaf(S[h][i], w.sc[nc], __builtin_amdgcn_logf(vs[h][i])) - kQ4Start;
-          m = fmaxf(m, MASK && !see[h][i] ? kNegBig : u);
-        }
-      m = max_xor32(max_xor16(m));
-      const float M = fmaxf(w.M[nc], m), f = fast_exp2(w.M[nc] - M);
-      w.M[nc] = M;
-      w.l[nc] *= f;
-#pragma unroll
-      for (int k = 0; k < G; ++k) {
-        w.y[nc][k] *= f;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) w.o[nc][k][t] *= f;
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[h][i] = fast_exp2(fmaf(S[h][i], w.sc[nc], -M));
-    }
+  }
+  float p[2][4];
+  f16x8 pw[G];
+  // weights and, per group, w = p s as fp16 (PARTS = 2: this column's part of it); again with another M where
+  // one is too large (never more than once)
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    float big = 0.f;
+    f16x2 top = {(_Float16)0.f, (_Float16)0.f};
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w.l[nc] += p[h][i];
+      for (int i = 0; i < 4; ++i) {
+        p[h][i] = fast_exp2(fmaf(S[h][i], w.sc, -w.M));
+        big = fmaxf(big, p[h][i]);
+      }
 #pragma unroll
     for (int k = 0; k < G; ++k) {
-      float x[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t m = r.vm[e >> 2][k][e & 3];
-        const bool on = !MASK || see[e >> 2][e & 3];
-        x[e] = on ? p[e >> 2][e & 3] * q4_scale(m) : 0.f;
-        w.y[nc][k] = fmaf(p[e >> 2][e & 3], on ? q4_centre(m) : 0.f, w.y[nc][k]);
-      }
-      f16x8 b;
+      for (int e = 0; e < 8; e += 2) {
+        f16x2 hi, part;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        _Float16 hi = (_Float16)x[e];
-        if constexpr (PARTS == 2) {
-          const _Float16 lo = (_Float16)(x[e] - (float)hi);
-          b[e] = low ? lo : hi;
-        } else {
-          w.y[nc][k] = fmaf(-7.5f, (float)hi, w.y[nc][k]);
-          b[e] = hi;
+        for (int f = 0; f < 2; ++f) {
+          const int h = e >> 2, i = (e & 3) + f;
+          const float x = p[h][i] * q4_scale(vm[h][k][i]);
+          hi[f] = (_Float16)x;
+          if constexpr (PARTS == 2) {
+            const _Float16 rest = (_Float16)(x - (float)hi[f]);
+            part[f] = low ? rest : hi[f];
+          } else {
+            part[f] = hi[f];
+          }
         }
+        top = __builtin_elementwise_max(top, hi);
+        pw[k][e] = part[0];
+        pw[k][e + 1] = part[1];
       }
+    }
+    const bool far = (float)top[0] > kQ4Limit || (float)top[1] > kQ4Limit || big > kQ4Limit / kQ4Floor;
+    if (__builtin_expect(!__any(far), 1)) break;
+    float m = kNegBig;
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        uint32_t o[4];
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {  // page e / 2, token pair e % 2
-          const uint32_t x0 = r.v[e >> 1][(e & 1) * G + k];
-          const uint32_t x1 = t & 2 ? x0 >> 8 : x0;
-          o[e] = t & 1 ? q4_pair<PARTS, true>(x1) : q4_pair<PARTS, false>(x1);
-        }
-        w.o[nc][k][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q4_operand(o[0], o[1], o[2], o[3]), b, w.o[nc][k][t], 0, 0, 0);
+      for (int i = 0; i < 4; ++i) {
+        float s = kQ4Floor;
+#pragma unroll
+        for (int k = 0; k < G; ++k) s = fmaxf(s, q4_scale(vm[h][k][i]));
+        m = fmaxf(m, fmaf(S[h][i], w.sc, __builtin_amdgcn_logf(s)) - kQ4Start);
       }
+    m = max_xor32(max_xor16(m));
+    const float M = fmaxf(w.M, m), f = fast_exp2(w.M - M);
+    w.M = M;
+    w.l *= f;
+#pragma unroll
+    for (int k = 0; k < G; ++k) {
+      w.y[k] *= f;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) w.o[k][t] *= f;
     }
   }
-}
-
-// The walk over pages [p0, p1) (p0 even): page ids 64 at a time in a register, the next step's pages loaded
-// before this one's products. all: keys below it are seen by every column.
-template <int HD, int PARTS, int NC>
-__device__ __forceinline__ void q4_walk(const Q4Args& a, int b, int hk, int p0, int p1, int all, int lane,
-                                        Q4Wave<HD, PARTS, NC>& w) {
-  constexpr int PB = q4_page_bytes(HD);
-  if (p0 >= p1) return;
-  const int32_t* table = a.page_table + (int64_t)b * a.pt_stride;
-  const int64_t step = (int64_t)a.Hk * PB;
-  const uint8_t* kb = a.k_pool + (int64_t)hk * PB;
-  const uint8_t* vb = a.v_pool + (int64_t)hk * PB;
-  auto ids_at = [&](int p) { return p + lane < p1 ? table[p + lane] : -1; };
-  int ids = ids_at(p0), base = p0;
-  Q4Raw<HD> cur, next;
-  auto fetch = [&](int p, Q4Raw<HD>& r) {  // pages p and p + 1; returns which are there
-    if (p - base >= 64) {
-      base += 64;
-      ids = ids_at(base);
-    }
-    int live = 0;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int id = q4_block(__builtin_amdgcn_readlane(ids, p - base + h), a.num_blocks);
-      live |= (id >= 0) << h;
-      const int64_t off = (int64_t)(id >= 0 ? id : 0) * step;
-      q4_load_page<HD>(kb + off, vb + off, lane, r, h);
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w.l += p[h][i];
+#pragma unroll
+  for (int k = 0; k < G; ++k) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w.y[k] = fmaf(p[e >> 2][e & 3], q4_centre(vm[e >> 2][k][e & 3]), w.y[k]);
+    if constexpr (PARTS == 1) {  // -7.5 w, as rounded
+      const f16x2 mid = {(_Float16)-7.5f, (_Float16)-7.5f};
+#pragma unroll
+      for (int e = 0; e < 8; e += 2)
+        w.y[k] = __builtin_amdgcn_fdot2(__builtin_bit_cast(h16x2, f16x2{pw[k][e], pw[k][e + 1]}),
+                                        __builtin_bit_cast(h16x2, mid), w.y[k], false);
     }
-    return live;
-  };
-  int live = fetch(p0, cur);
-  for (int p = p0; p < p1; p += 2) {
-    int live_next = 0;
-    if (p + 2 < p1) live_next = fetch(p + 2, next);
-    const int key0 = p * kQ4Tokens;
-    if (live == 3 && key0 + 32 <= all)
-      q4_step<HD, PARTS, NC, false>(cur, w, key0, live, lane);
-    else
-      q4_step<HD, PARTS, NC, true>(cur, w, key0, live, lane);
-    cur = next;
-    live = live_next;
   }
+  uint32_t vw[2][2 * G];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) P::v_words(pg + h * P::BYTES, lane, vw[h]);
+#pragma unroll
+  for (int k = 0; k < G; ++k)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      uint32_t x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {  // page e / 2, token pair e % 2
+        const uint32_t x0 = vw[e >> 1][(e & 1) * G + k], x1 = t & 2 ? x0 >> 8 : x0;
+        x[e] = t & 1 ? q4_pair<PARTS, true>(x1) : q4_pair<PARTS, false>(x1);
+      }
+      w.o[k][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q4_operand(x[0], x[1], x[2], x[3]), pw[k], w.o[k][t], 0, 0, 0);
+    }
 }
 
 // A tile's walk is done: the lanes' sums joined. Leaves in lane (g, c) the 16 values d = 64 k + 16 g ..
 // + 15 of column c's unnormalised row per group, and l.
-template <int HD, int PARTS, int NC>
-__device__ __forceinline__ void q4_join(Q4Wave<HD, PARTS, NC>& w, int nc, float (&o)[HD / kQ4Group][16], float& l) {
+template <int HD, int PARTS>
+__device__ __forceinline__ void q4_join(Q4Wave<HD, PARTS>& w, float (&o)[HD / kQ4Group][16], float& l) {
   constexpr int G = HD / kQ4Group;
-  l = sum_xor32(sum_xor16(w.l[nc]));
+  l = sum_xor32(sum_xor16(w.l));
 #pragma unroll
   for (int k = 0; k < G; ++k) {
-    const float y = sum_xor32(sum_xor16(w.y[nc][k]));
+    const float y = sum_xor32(sum_xor16(w.y[k]));
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float v = w.o[nc][k][t][i];
+        float v = w.o[k][t][i];
         if constexpr (PARTS == 2) v += dpp<0x128>(v);
         o[k][4 * i + t] = fmaf(v, (t & 1) ? kQ4Unit<PARTS> / 16.f : kQ4Unit<PARTS>, y);
       }
@@ -467,12 +480,24 @@ __device__ __forceinline__ Q4Unit q4_unit(const Q4Args& a) {
 }
 
 constexpr int kQ4Waves = 4;
+constexpr int kQ4MaxNarrow = 32;  // rows that the narrow kernel takes (two tiles of 16)
 
-// Each wavefront has NC column tiles of its own and walks all of the workgroup's keys.
-template <typename IO, int HD, int PARTS, int NC>
-__global__ __launch_bounds__(64 * kQ4Waves) void q4_wide_kernel(const Q4Args a) {
-  constexpr int G = HD / kQ4Group;
+// Each wavefront has a column tile of its own, and the workgroup walks the keys together: stages of 64 keys
+// go from the pools straight into LDS (global_load_lds, one page per wavefront), two stages ahead in a ring
+// of three, with one barrier a stage. Read from memory by each wavefront for itself, the pages' pairs alone
+// (16 bytes that 16 lanes share) cost more load instructions than the codes.
+constexpr int kQ4WideWaves = 4;
+constexpr int kQ4StagePages = kQ4WideWaves, kQ4Ring = 3;
+constexpr uint32_t kQ4StageMask = (1u << kQ4StagePages) - 1;
+
+template <typename IO, int HD, int PARTS>
+__global__ __launch_bounds__(64 * kQ4WideWaves, 3) void q4_wide_kernel(const Q4Args a) {
+  using P = Q4Staged<HD>;
+  constexpr int G = HD / kQ4Group, PB = q4_page_bytes(HD);
   constexpr int ROWS = 16 / PARTS;  // rows of a column tile
+  constexpr int STAGE = kQ4StagePages * P::BYTES;
+  constexpr int LOADS = HD == 128 ? 3 : 2;  // load instructions of a page
+  __shared__ __attribute__((aligned(16))) uint8_t ring[kQ4Ring * STAGE];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int g = lane >> 4, c = lane & 15;
   const Q4Unit u = q4_unit(a);
@@ -480,51 +505,103 @@ __global__ __launch_bounds__(64 * kQ4Waves) void q4_wide_kernel(const Q4Args a) 
   const int rows = a.T * a.group;
   int keys = L < a.max_pages * kQ4Tokens ? L : a.max_pages * kQ4Tokens;
   keys = keys > 0 ? keys : 0;
-  // the pages that the wavefront's rows see, and the workgroup's share of them
-  const int first = (u.tile * kQ4Waves + wave) * NC * ROWS;
-  const int end = first + NC * ROWS < rows ? first + NC * ROWS : rows;
-  int most = 0, all = 0;
-  if (first < rows) {
-    all = valid_keys(L, C, first / a.group);
-    most = valid_keys(L, C, (end - 1) / a.group);
-    most = most < keys ? most : keys;
-    all = all < keys ? all : keys;
-  }
-  const int pages = (most + kQ4Tokens - 1) / kQ4Tokens;
+  auto seen = [&](int row) {  // keys that the row sees
+    const int n = valid_keys(L, C, row / a.group);
+    return n < keys ? n : keys;
+  };
+  // what the workgroup's rows see together, and its share of the pages
+  const int wg_first = u.tile * kQ4WideWaves * ROWS;
+  const int wg_end = wg_first + kQ4WideWaves * ROWS < rows ? wg_first + kQ4WideWaves * ROWS : rows;
+  const int pages = (seen(wg_end - 1) + kQ4Tokens - 1) / kQ4Tokens;
   const int p0 = u.split * a.split_pages;
   int p1 = a.splits > 1 ? p0 + a.split_pages : pages;
   p1 = p1 < pages ? p1 : pages;
   if (a.splits > 1 && p0 >= p1) return;  // no record: the merge knows how far each row's pages reach
-  Q4Wave<HD, PARTS, NC> w;
-  const int tile0 = first / ROWS;
-#pragma unroll
-  for (int nc = 0; nc < NC; ++nc) q4_setup<IO, HD, PARTS, NC>(a, u.b, u.hk, tile0 + nc, L, C, keys, lane, w, nc);
-  q4_walk<HD, PARTS, NC>(a, u.b, u.hk, p0, p1, all, lane, w);
-#pragma unroll
-  for (int nc = 0; nc < NC; ++nc) {
-    const int row = q4_row<PARTS>(tile0 + nc, c);
-    float o[G][16], l;
-    q4_join<HD, PARTS, NC>(w, nc, o, l);
-    if (row >= rows || c >= ROWS) continue;
-    if (a.splits > 1) {
-      float* rec = q4_record<HD>(a, u.b, u.hk, row, u.split);
-      if (g == 0) {
-        rec[0] = w.M[nc];
-        rec[1] = l;
+  // what the wavefront's rows see: all of them, some of them
+  const int first = wg_first + wave * ROWS;
+  const int end = first + ROWS < rows ? first + ROWS : rows;
+  const int all = first < rows ? seen(first) : 0, most = first < rows ? seen(end - 1) : 0;
+  Q4Wave<HD, PARTS> w;
+  const int tile = first / ROWS;
+  q4_setup<IO, HD, PARTS>(a, u.b, u.hk, tile, L, C, keys, lane, w);
+
+  if (p0 < p1) {
+    const int32_t* table = a.page_table + (int64_t)u.b * a.pt_stride;
+    const int64_t step = (int64_t)a.Hk * PB;
+    const uint8_t* kb = a.k_pool + (int64_t)u.hk * PB;
+    const uint8_t* vb = a.v_pool + (int64_t)u.hk * PB;
+    int ids = -1, base = p0 - 64;  // blocks of pages base .. base + 63 (-1: none), and which there are
+    uint64_t there = 0;
+    // per-lane source of what a page's last load fetches: the pairs and, at head_dim 64, the codes of both
+    const uint8_t* meta_src = (lane & (4 * G) ? vb : kb) + q4_codes_bytes(HD) + (lane & (4 * G - 1)) * 16;
+    const uint8_t* code_src = (lane < 32 ? kb : vb) + (lane & 31) * 16;
+    const uint32_t k_off = (uint32_t)(c * 4 + g) * 16, v_off = (uint32_t)lane * 16;
+    const int stages = (p1 - p0 + kQ4StagePages - 1) / kQ4StagePages;
+    uint32_t live = 0;  // pages of the ring's stages that are there, kQ4StagePages bits a slot
+    auto issue = [&](int st, int slot) {
+      const int pg = p0 + st * kQ4StagePages;
+      if (pg - base >= 64) {
+        base = pg;
+        ids = pg + lane < p1 ? q4_block(table[pg + lane], a.num_blocks) : -1;
+        there = __ballot(ids >= 0);
       }
-#pragma unroll
-      for (int k = 0; k < G; ++k)
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          *reinterpret_cast<f32x2*>(rec + 2 + 64 * k + 16 * g + 2 * i) = f32x2{o[k][2 * i], o[k][2 * i + 1]};
-    } else {
-      const int i = row / a.group, j = row - i * a.group;
-      IO* out = static_cast<IO*>(a.out) + (int64_t)u.b * a.o_sb + (int64_t)(u.hk * a.group + j) * a.o_sh + (int64_t)i * a.o_st;
-      const float f = l > 0.f || l != l ? 1.f / l : 0.f;
-#pragma unroll
-      for (int k = 0; k < G; ++k) q4_store16<IO>(out + 64 * k + 16 * g, o[k], f);
-      if (a.lse != nullptr && g == 0) *q4_lse(a, u.b, u.hk, row) = l > 0.f ? w.M[nc] + __builtin_amdgcn_logf(l) : INFINITY;
+      live = (live & ~(kQ4StageMask << kQ4StagePages * slot)) |
+             ((uint32_t)(there >> (pg - base)) & kQ4StageMask) << kQ4StagePages * slot;
+      const int mine = __builtin_amdgcn_readlane(ids, pg - base + wave);
+      const int64_t off = (int64_t)(mine >= 0 ? mine : 0) * step;  // (pages that are not there: block 0's bytes, unseen)
+      uint8_t* dst = ring + slot * STAGE + wave * P::BYTES;
+      if constexpr (HD == 128) {
+        stage_load16(kb + off, k_off, dst);
+        stage_load16(vb + off, v_off, dst + P::CODES);
+      } else {
+        stage_load16_at(code_src + off, dst);
+      }
+      if (lane < 8 * G) stage_load16_at(meta_src + off, dst + 2 * P::CODES);
+    };
+    auto compute = [&](int st, int slot) {
+#pragma unroll 1
+      for (int h = 0; h < kQ4StagePages; h += 2) {
+        const int key0 = (p0 + st * kQ4StagePages + h) * kQ4Tokens;
+        const int bits = (int)(live >> (kQ4StagePages * slot + h)) & 3;
+        const uint8_t* pg = ring + slot * STAGE + h * P::BYTES;
+        if (key0 >= most || bits == 0) continue;
+        q4_step<HD, PARTS>(pg, w, key0, bits != 3 || key0 + 32 > all, bits, lane);
+      }
+    };
+    issue(0, 0);
+    issue(1, 1);
+    for (int st = 0, slot = 0; st < stages; ++st) {
+      vm_wait<LOADS>();  // this wavefront's page of stage st has arrived; the barrier: everybody's, and stage
+      lds_read_wait();   // st - 1, whose slot is filled next, has been read
+      __builtin_amdgcn_s_barrier();
+      issue(st + 2, slot == 0 ? 2 : slot - 1);
+      compute(st, slot);
+      slot = slot == 2 ? 0 : slot + 1;
     }
+    vm_wait<0>();  // nothing may still be on its way into LDS when the workgroup ends
+  }
+  const int row = q4_row<PARTS>(tile, c);
+  float o[G][16], l;
+  q4_join<HD, PARTS>(w, o, l);
+  if (row >= rows || c >= ROWS) return;
+  if (a.splits > 1) {
+    float* rec = q4_record<HD>(a, u.b, u.hk, row, u.split);
+    if (g == 0) {
+      rec[0] = w.M;
+      rec[1] = l;
+    }
+#pragma unroll
+    for (int k = 0; k < G; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        *reinterpret_cast<f32x2*>(rec + 2 + 64 * k + 16 * g + 2 * i) = f32x2{o[k][2 * i], o[k][2 * i + 1]};
+  } else {
+    const int i = row / a.group, j = row - i * a.group;
+    IO* out = static_cast<IO*>(a.out) + (int64_t)u.b * a.o_sb + (int64_t)(u.hk * a.group + j) * a.o_sh + (int64_t)i * a.o_st;
+    const float f = l > 0.f || l != l ? 1.f / l : 0.f;
+#pragma unroll
+    for (int k = 0; k < G; ++k) q4_store16<IO>(out + 64 * k + 16 * g, o[k], f);
+    if (a.lse != nullptr && g == 0) *q4_lse(a, u.b, u.hk, row) = l > 0.f ? w.M + __builtin_amdgcn_logf(l) : INFINITY;
   }
 }
 
@@ -910,51 +987,85 @@ __device__ __forceinline__ int q4_splits_of(const Q4Args& a, int b, int i) {
   return (n + a.split_pages * kQ4Tokens - 1) / (a.split_pages * kQ4Tokens);
 }
 
-// Records of a row's splits -> its output and log2 denominator. One wavefront per row.
-template <typename IO, int HD>
-__global__ __launch_bounds__(256) void q4_merge_kernel(const Q4Args a, int64_t total) {
-  const int64_t x = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (x >= total) return;
-  const int lane = threadIdx.x & 63;
-  const int rows = a.T * a.group;
-  const int row = (int)(x % rows);
-  const int hk = (int)(x / rows % a.Hk), b = (int)(x / rows / a.Hk);
-  const float* rec = q4_record<HD>(a, b, hk, row, 0);
-  const int i = row / a.group, j = row - i * a.group;
-  const int splits = q4_splits_of(a, b, i);
-  float M = kNegBig;
-  for (int s = 0; s < splits; ++s) M = fmaxf(M, rec[(int64_t)s * (HD + 2)]);
-  constexpr int E = HD / 64;
-  float l = 0.f, o[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = 0.f;
-  for (int s = 0; s < splits; ++s) {
-    const float* p = rec + (int64_t)s * (HD + 2);
-    const float f = fast_exp2(p[0] - M);
-    l = fmaf(f, p[1], l);
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = fmaf(f, p[2 + lane + 64 * e], o[e]);
+// A row's splits: lane s reads (M, l) of split s (of 64 at a time); their weights 2^(M_s - M) stay in the lanes.
+// Returns M and l.
+template <int HD>
+__device__ __forceinline__ void q4_row_state(const float* rec, int splits, int lane, float& M, float& l) {
+  M = kNegBig;
+  for (int s = lane; s < splits; s += 64) M = fmaxf(M, rec[(int64_t)s * (HD + 2)]);
+  M = wave_max(M);
+  l = 0.f;
+  for (int s = lane; s < splits; s += 64) {
+    const f32x2 r = *reinterpret_cast<const f32x2*>(rec + (int64_t)s * (HD + 2));
+    l = fmaf(fast_exp2(r[0] - M), r[1], l);
   }
-  IO* out = static_cast<IO*>(a.out) + (int64_t)b * a.o_sb + (int64_t)(hk * a.group + j) * a.o_sh + (int64_t)i * a.o_st;
-#pragma unroll
-  for (int e = 0; e < E; ++e) Elem<IO>::store(out + lane + 64 * e, l > 0.f || l != l ? o[e] / l : 0.f);
-  if (a.lse != nullptr && lane == 0) *q4_lse(a, b, hk, row) = l > 0.f ? M + __builtin_amdgcn_logf(l) : INFINITY;
+  l = wave_sum(l);
 }
 
-// Decode totals: each key's weight, from the scores left in the workspace. A block that two rows of
-// the page table share is added to by both, hence the atomic; otherwise each slot gets one addition.
-__global__ __launch_bounds__(256) void q4_decode_weights_kernel(const Q4Args a) {
-  const int b = blockIdx.z, hk = blockIdx.y;
-  const int t = blockIdx.x * 256 + threadIdx.x;
+// Records of the splits -> outputs and, for decode totals, the keys' weights from the scores that the first
+// kernel left in the workspace. The first `merges` workgroups merge, one wavefront per row; of the others each
+// adds 256 keys' weights of one KV head, having formed its rows' denominators from the records by itself (a
+// launch less than in two steps). A block that two rows of the page table share is added to by both, hence
+// the atomic; otherwise each slot gets one addition.
+template <typename IO, int HD>
+__global__ __launch_bounds__(256) void q4_finish_kernel(const Q4Args a, int64_t total, int merges, int chunks) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int rows = a.T * a.group;
+  if ((int)blockIdx.x < merges) {
+    const int64_t x = (int64_t)blockIdx.x * 4 + wave;
+    if (x >= total) return;
+    const int row = (int)(x % rows);
+    const int hk = (int)(x / rows % a.Hk), b = (int)(x / rows / a.Hk);
+    const float* rec = q4_record<HD>(a, b, hk, row, 0);
+    const int i = row / a.group, j = row - i * a.group;
+    const int splits = q4_splits_of(a, b, i);
+    float M, l;
+    q4_row_state<HD>(rec, splits, lane, M, l);
+    constexpr int E = HD / 64;
+    float o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
+#pragma unroll 8
+    for (int s = 0; s < splits; ++s) {
+      const float* p = rec + (int64_t)s * (HD + 2);
+      const float f = fast_exp2(p[0] - M);
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = fmaf(f, p[2 + lane + 64 * e], o[e]);
+    }
+    IO* out = static_cast<IO*>(a.out) + (int64_t)b * a.o_sb + (int64_t)(hk * a.group + j) * a.o_sh + (int64_t)i * a.o_st;
+#pragma unroll
+    for (int e = 0; e < E; ++e) Elem<IO>::store(out + lane + 64 * e, l > 0.f || l != l ? o[e] / l : 0.f);
+    if (a.lse != nullptr && lane == 0) *q4_lse(a, b, hk, row) = l > 0.f ? M + __builtin_amdgcn_logf(l) : INFINITY;
+    return;
+  }
+  __shared__ float lse[kQ4MaxNarrow];
+  int x = (int)blockIdx.x - merges;
+  const int chunk = x % chunks;
+  x /= chunks;
+  const int hk = x % a.Hk, b = x / a.Hk;
   const int L = a.seq_lens[b], C = a.cur_lens[b];
   int n = valid_keys(L, C, 0);
   n = n < a.max_pages * kQ4Tokens ? n : a.max_pages * kQ4Tokens;
-  if (t >= n || C < 1) return;
+  const int t = chunk * 256 + threadIdx.x;
+  if (chunk * 256 >= n || C < 1) return;
+  if (a.splits > 1) {
+    const int splits = q4_splits_of(a, b, 0);
+    for (int j = wave; j < a.group; j += 4) {
+      float M, l;
+      q4_row_state<HD>(q4_record<HD>(a, b, hk, j, 0), splits, lane, M, l);
+      if (lane == 0) lse[j] = l > 0.f ? M + __builtin_amdgcn_logf(l) : INFINITY;
+    }
+  } else if ((int)threadIdx.x < a.group) {
+    lse[threadIdx.x] = *q4_lse(a, b, hk, threadIdx.x);
+  }
+  __syncthreads();
+  if (t >= n) return;
   const int id = q4_block(a.page_table[(int64_t)b * a.pt_stride + t / kQ4Tokens], a.num_blocks);
   if (id < 0) return;
   float sum = 0.f;
-  for (int j = 0; j < a.group; ++j)
-    sum += fast_exp2(a.scores[((int64_t)b * a.H + hk * a.group + j) * a.score_stride + t] - *q4_lse(a, b, hk, j));
+  const float* mine = a.scores + ((int64_t)b * a.H + hk * a.group) * a.score_stride + t;
+#pragma unroll 4
+  for (int j = 0; j < a.group; ++j) sum += fast_exp2(mine[j * a.score_stride] - lse[j]);
   atomicAdd(a.weights + ((int64_t)id * a.Hk + hk) * kQ4Tokens + (t & (kQ4Tokens - 1)), sum);
 }
 
@@ -989,17 +1100,17 @@ __global__ __launch_bounds__(256) void q4_chunk_weights_kernel(const Q4Args a) {
   for (int h = 0; h < 2; ++h) q4_k_operands<HD, PARTS>(r.k[h], kf[h]);
   float sum[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
   for (int tile = i0 * a.group / ROWS; tile * ROWS < real; ++tile) {
-    Q4Wave<HD, PARTS, 1> w;
-    q4_setup<IO, HD, PARTS, 1>(a, b, hk, tile, L, C, keys, lane, w, 0);
+    Q4Wave<HD, PARTS> w;
+    q4_setup<IO, HD, PARTS>(a, b, hk, tile, L, C, keys, lane, w);
     const int row = q4_row<PARTS>(tile, c);
     const float lse = row < real && c < ROWS ? *q4_lse(a, b, hk, row < rows ? row : rows - 1) : INFINITY;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const f32x4 S = q4_scores<HD, PARTS, 1>(kf[h], r.km[h], w, 0);
+      const f32x4 S = q4_scores<HD, PARTS>(kf[h], r.km[h], w.q, w.qs);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float p = fast_exp2(fmaf(S[i], w.sc[0], -lse));
-        sum[h][i] += row < real && c < ROWS && (p0 + h) * kQ4Tokens + 4 * g + i < w.n[0] ? p : 0.f;
+        const float p = fast_exp2(fmaf(S[i], w.sc, -lse));
+        sum[h][i] += row < real && c < ROWS && (p0 + h) * kQ4Tokens + 4 * g + i < w.n ? p : 0.f;
       }
     }
   }
@@ -1017,7 +1128,7 @@ __global__ __launch_bounds__(256) void q4_chunk_weights_kernel(const Q4Args a) {
 // Host side
 // ---------------------------------------------------------------------------------------------
 struct Q4Plan {
-  int parts, nc, rows_per_tile;
+  int parts, rows_per_tile;
   bool wide;
   int tiles, splits, split_pages;
   int64_t rows;
@@ -1032,15 +1143,14 @@ static Q4Plan q4_plan(int io_dtype, int32_t batch, int32_t heads, int32_t kv_hea
   const int rpt = p.parts == 2 ? 8 : 16;
   p.rows = (int64_t)query_len * (heads / kv_heads);
   p.wide = p.rows > 2 * rpt;
-  p.nc = p.wide ? 2 : 1;
-  p.rows_per_tile = p.wide ? kQ4Waves * p.nc * rpt : rpt;
+  p.rows_per_tile = p.wide ? kQ4WideWaves * rpt : rpt;
   p.tiles = (int)((p.rows + p.rows_per_tile - 1) / p.rows_per_tile);
   const int64_t units = (int64_t)batch * kv_heads * p.tiles;
   const int64_t target = 2 * (int64_t)pa_host::device_cu_count();
   const int64_t want = units > 0 ? (target + units - 1) / units : 1;
   int pages = (int)((max_pages + want - 1) / want);
   const int least = p.wide ? 16 : 64;
-  if (!p.wide && pages > 128) pages = 128;  // requests of very different lengths: ranges end together
+  if (!p.wide && pages > 96) pages = 96;  // requests of very different lengths: ranges end together
   pages = pages < least ? least : pages;
   pages = (pages + 7) / 8 * 8;
   p.split_pages = pages;
@@ -1060,26 +1170,24 @@ template <typename IO, int HD, int PARTS>
 static void launch_q4(const Q4Args& a, const Q4Plan& p, hipStream_t stream) {
   const dim3 grid((unsigned)((int64_t)a.B * a.Hk * p.tiles * p.splits));
   if (p.wide)
-    q4_wide_kernel<IO, HD, PARTS, 2><<<grid, 64 * kQ4Waves, 0, stream>>>(a);
+    q4_wide_kernel<IO, HD, PARTS><<<grid, 64 * kQ4WideWaves, 0, stream>>>(a);
   else if (p.rows == 1)
     q4_narrow_kernel<IO, HD, PARTS, 1><<<grid, 64 * kQ4Waves, 0, stream>>>(a);
   else if (p.rows <= 4)
     q4_narrow_kernel<IO, HD, PARTS, 4><<<grid, 64 * kQ4Waves, 0, stream>>>(a);
   else
     q4_narrow_kernel<IO, HD, PARTS, 16 / PARTS><<<grid, 64 * kQ4Waves, 0, stream>>>(a);
-  if (p.splits > 1) {
+  // totals of decode steps that one workgroup saw whole are done in place
+  const bool totals = a.scores != nullptr && !(p.splits == 1 && p.tiles == 1);
+  if (p.splits > 1 || totals) {
     const int64_t total = (int64_t)a.B * a.Hk * a.T * a.group;
-    q4_merge_kernel<IO, HD><<<(unsigned)((total + 3) / 4), 256, 0, stream>>>(a, total);
+    const int merges = p.splits > 1 ? (int)((total + 3) / 4) : 0, chunks = (a.max_pages * kQ4Tokens + 255) / 256;
+    const int64_t wgs = merges + (totals ? (int64_t)chunks * a.Hk * a.B : 0);
+    q4_finish_kernel<IO, HD><<<(unsigned)wgs, 256, 0, stream>>>(a, total, merges, chunks);
   }
-  if (a.weights != nullptr) {
-    if (a.scores != nullptr) {
-      if (p.splits == 1 && p.tiles == 1) return;  // done in place
-      const dim3 wg((unsigned)((a.max_pages * kQ4Tokens + 255) / 256), a.Hk, a.B);
-      q4_decode_weights_kernel<<<wg, 256, 0, stream>>>(a);
-    } else {
-      const dim3 wg((unsigned)((a.max_pages + 7) / 8), a.Hk, a.B);
-      q4_chunk_weights_kernel<IO, HD, PARTS><<<wg, 256, 0, stream>>>(a);
-    }
+  if (a.weights != nullptr && a.scores == nullptr) {
+    const dim3 wg((unsigned)((a.max_pages + 7) / 8), a.Hk, a.B);
+    q4_chunk_weights_kernel<IO, HD, PARTS><<<wg, 256, 0, stream>>>(a);
   }
 }
 
@@ -1122,7 +1230,9 @@ extern "C" int pa_q4_attention(const void* q, int64_t q_stride_b, int64_t q_stri
   PA_CHECK_ARG(max_pages <= (1 << 26) && (int64_t)query_len * (num_heads / kv_heads) <= (1 << 26) && kv_heads <= 65535 &&
                    batch <= 65535, "pa_q4_attention: sizes beyond the kernels' 32-bit indices");
   const Q4Plan p = q4_plan(io_dtype, batch, num_heads, kv_heads, query_len, head_dim, max_pages, weights != nullptr && max_pages > 0);
-  PA_CHECK_ARG((int64_t)batch * kv_heads * p.tiles * p.splits <= 0x7fffffffLL, "pa_q4_attention: grid too large");
+  PA_CHECK_ARG((int64_t)batch * kv_heads * p.tiles * p.splits <= 0x7fffffffLL &&
+                   (int64_t)batch * kv_heads * (p.rows / 4 + 1 + max_pages / 16 + 1) <= 0x7fffffffLL,
+               "pa_q4_attention: grid too large");
   if (p.bytes && (workspace == nullptr || workspace_bytes < p.bytes))
     PA_FAIL(PA_ERR_WORKSPACE, "pa_q4_attention: workspace too small: need %zu bytes, have %zu", p.bytes, workspace_bytes);
   PA_CHECK_ARG((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "pa_q4_attention: the workspace must be 16-byte aligned");
