@@ -67,7 +67,23 @@ struct Q4Args {
 
 constexpr float kQ4Start = 4.f;         // log2 of p * max(s) when M is set
 constexpr float kQ4Limit = 32768.f;     // p * max(s, 2^-14) beyond which M is set again
+constexpr short kQ4LimitBits = 0x7800;    // kQ4Limit as a half
 constexpr float kQ4Floor = 6.103515625e-5f;  // 2^-14
+// A zero that the compiler does not know: half * float + zero is one v_fma_mix_f32, which reads the half in
+// place, where a product alone is a conversion and a multiplication.
+__device__ __forceinline__ float q4_zero() {
+  float z = 0.f;
+  asm("" : "+v"(z));
+  return z;
+}
+// Two products of a weight and a pair's scale as fp16: v_fma_mixlo_f16 and v_fma_mixhi_f16. (Told apart by
+// the empty asm, or the two become one vector of conversions and multiplications, five instructions.)
+__device__ __forceinline__ f16x2 q4_weights(float p0, uint32_t m0, float p1, uint32_t m1) {
+  _Float16 lo = (_Float16)(p0 * q4_scale(m0));
+  asm("" : "+v"(lo));
+  return f16x2{lo, (_Float16)(p1 * q4_scale(m1))};
+}
+
 // Codes as the matrix cores take them. As fp16 subnormals (c 2^-24) they cost one AND, but the cores align
 // a product by its operands' exponents without normalising them, so that a sum keeps 7 to 10 bits fewer
 // than fp32, and sums of uncentred codes cancel against 7.5 times their weights: 2^-17 of the largest term,
@@ -75,6 +91,7 @@ constexpr float kQ4Floor = 6.103515625e-5f;  // 2^-14
 // normal and centred: 5e-7 for 1024 keys' output where the subnormals left 5e-5.
 template <int PARTS> constexpr float kQ4Unit = PARTS == 2 ? 512.f : 16777216.f;  // 1 / the value of code 1
 template <int PARTS> constexpr int kQ4UnitLog2 = PARTS == 2 ? 9 : 24;
+typedef short s16x2 __attribute__((ext_vector_type(2)));
 typedef __fp16 h16x2 __attribute__((ext_vector_type(2)));  // v_dot2_f32_f16's operand
 template <int PARTS, bool ODD>
 __device__ __forceinline__ uint32_t q4_pair(uint32_t word) {
@@ -224,7 +241,8 @@ template <int HD, int PARTS>
 __device__ __forceinline__ f32x4 q4_scores(const f16x8 (&kf)[HD / 32], const u32x4 (&km)[HD / kQ4Group], const f16x8 (&q)[HD / 32],
                                            const float (&qs)[HD / kQ4Group]) {
   constexpr int G = HD / kQ4Group;
-  f32x4 S = {0.f, 0.f, 0.f, 0.f};
+  const float zero = q4_zero();
+  f32x4 S = {zero, zero, zero, zero};
 #pragma unroll
   for (int k = 0; k < G; ++k) {
     const float q0 = qs[k], start = PARTS == 2 ? 0.f : -7.5f * q0;  // (PARTS = 2: the codes are centred)
@@ -233,7 +251,7 @@ __device__ __forceinline__ f32x4 q4_scores(const f16x8 (&kf)[HD / 32], const u32
     acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[2 * k + 1], q[2 * k + 1], acc, 0, 0, 0);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      S[i] = fmaf(q4_scale(km[k][i]), acc[i], k == 0 ? q4_centre(km[k][i]) * q0 : fmaf(q4_centre(km[k][i]), q0, S[i]));
+      S[i] = fmaf(q4_scale(km[k][i]), acc[i], fmaf(q4_centre(km[k][i]), q0, S[i]));
   }
   if constexpr (PARTS == 2) {
 #pragma unroll
@@ -329,7 +347,7 @@ __device__ __forceinline__ void q4_step(const uint8_t* pg, Q4Wave<HD, PARTS>& w,
 #pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {
     float big = 0.f;
-    f16x2 top = {(_Float16)0.f, (_Float16)0.f};
+    s16x2 top = {0, 0};  // (halves from 0 on are ordered as integers)
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -341,25 +359,25 @@ __device__ __forceinline__ void q4_step(const uint8_t* pg, Q4Wave<HD, PARTS>& w,
     for (int k = 0; k < G; ++k) {
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
+        const int h = e >> 2, i = e & 3;
         f16x2 hi, part;
+        if constexpr (PARTS == 1) {
+          hi = part = q4_weights(p[h][i], vm[h][k][i], p[h][i + 1], vm[h][k][i + 1]);
+        } else {
 #pragma unroll
-        for (int f = 0; f < 2; ++f) {
-          const int h = e >> 2, i = (e & 3) + f;
-          const float x = p[h][i] * q4_scale(vm[h][k][i]);
-          hi[f] = (_Float16)x;
-          if constexpr (PARTS == 2) {
+          for (int f = 0; f < 2; ++f) {
+            const float x = p[h][i + f] * q4_scale(vm[h][k][i + f]);
+            hi[f] = (_Float16)x;
             const _Float16 rest = (_Float16)(x - (float)hi[f]);
             part[f] = low ? rest : hi[f];
-          } else {
-            part[f] = hi[f];
           }
         }
-        top = __builtin_elementwise_max(top, hi);
+        top = __builtin_elementwise_max(top, __builtin_bit_cast(s16x2, hi));
         pw[k][e] = part[0];
         pw[k][e + 1] = part[1];
       }
     }
-    const bool far = (float)top[0] > kQ4Limit || (float)top[1] > kQ4Limit || big > kQ4Limit / kQ4Floor;
+    const bool far = top[0] > kQ4LimitBits || top[1] > kQ4LimitBits || big > kQ4Limit / kQ4Floor;
     if (__builtin_expect(!__any(far), 1)) break;
     float m = kNegBig;
 #pragma unroll
@@ -367,6 +385,7 @@ __device__ __forceinline__ void q4_step(const uint8_t* pg, Q4Wave<HD, PARTS>& w,
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float s = kQ4Floor;
+        asm volatile("" : "+v"(s));  // (or the maxima and logarithms are taken before the loop, in every step)
 #pragma unroll
         for (int k = 0; k < G; ++k) s = fmaxf(s, q4_scale(vm[h][k][i]));
         m = fmaxf(m, fmaf(S[h][i], w.sc, __builtin_amdgcn_logf(s)) - kQ4Start);
