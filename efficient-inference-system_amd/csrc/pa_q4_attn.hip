@@ -63,6 +63,9 @@ struct Q4Args {
   float* lse;           // totals: log2 of each row's denominator
   float* scores;        // decode totals: log2-domain scores [B, H, score_stride]
   int64_t score_stride;
+  f16x8* q_ops;         // chunk totals: the row tiles' operands [tile][HD / 32][64 lanes], and per lane
+  f32x4* q_aux;         // (qs of the groups, sc, keys seen)
+  int32_t op_tiles;     // tiles of 16 / PARTS rows per (request, KV head) there
 };
 
 constexpr float kQ4Start = 4.f;         // log2 of p * max(s) when M is set
@@ -99,43 +102,6 @@ __device__ __forceinline__ uint32_t q4_pair(uint32_t word) {
   if constexpr (PARTS == 1) return masked;
   constexpr _Float16 up = (_Float16)32768.f, mid = (_Float16)((ODD ? -16.f : -1.f) * 7.5f / 512.f);
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(f16x2, masked), f16x2{up, up}, f16x2{mid, mid}));
-}
-
-// One step's page data of a lane.
-template <int HD>
-struct Q4Raw {
-  static constexpr int G = HD / kQ4Group, W = HD / 32;
-  uint32_t k[2][W], v[2][2 * G];
-  u32x4 km[2][G], vm[2][G];
-};
-
-template <int HD>
-__device__ __forceinline__ void q4_load_page(const uint8_t* kp, const uint8_t* vp, int lane, Q4Raw<HD>& r, int h) {
-  constexpr int G = HD / kQ4Group, W = HD / 32;
-  const int g = lane >> 4, c = lane & 15;
-  const uint32_t* kc = reinterpret_cast<const uint32_t*>(kp) + (c * 4 + g) * W;
-  const uint32_t* vc = reinterpret_cast<const uint32_t*>(vp) + lane * 2 * G;
-  if constexpr (HD == 128) {
-    const u32x4 a = *reinterpret_cast<const u32x4*>(kc), b = *reinterpret_cast<const u32x4*>(vc);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      r.k[h][i] = a[i];
-      r.v[h][i] = b[i];
-    }
-  } else {
-    const u32x2 a = *reinterpret_cast<const u32x2*>(kc), b = *reinterpret_cast<const u32x2*>(vc);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      r.k[h][i] = a[i];
-      r.v[h][i] = b[i];
-    }
-  }
-#pragma unroll
-  for (int a = 0; a < G; ++a) {
-    const int off = q4_codes_bytes(HD) + (a * kQ4Tokens + 4 * g) * 4;
-    r.km[h][a] = *reinterpret_cast<const u32x4*>(kp + off);
-    r.vm[h][a] = *reinterpret_cast<const u32x4*>(vp + off);
-  }
 }
 
 // A wavefront's column tile: operands, sums and running state.
@@ -543,6 +509,12 @@ __global__ __launch_bounds__(64 * kQ4WideWaves, 3) void q4_wide_kernel(const Q4A
   Q4Wave<HD, PARTS> w;
   const int tile = first / ROWS;
   q4_setup<IO, HD, PARTS>(a, u.b, u.hk, tile, L, C, keys, lane, w);
+  if (a.q_ops != nullptr && u.split == 0) {  // for q4_chunk_weights_kernel
+    const int64_t at = ((int64_t)u.b * a.Hk + u.hk) * a.op_tiles + tile;
+#pragma unroll
+    for (int s = 0; s < HD / 32; ++s) a.q_ops[(at * (HD / 32) + s) * 64 + lane] = w.q[s];
+    a.q_aux[at * 64 + lane] = f32x4{w.qs[0], w.qs[G - 1], w.sc, __int_as_float(w.n)};
+  }
 
   if (p0 < p1) {
     const int32_t* table = a.page_table + (int64_t)u.b * a.pt_stride;
@@ -1088,59 +1060,101 @@ __global__ __launch_bounds__(256) void q4_finish_kernel(const Q4Args a, int64_t 
   atomicAdd(a.weights + ((int64_t)id * a.Hk + hk) * kQ4Tokens + (t & (kQ4Tokens - 1)), sum);
 }
 
-// Totals of a chunk: the scores formed again, page pair by page pair, the rows' weights summed. One
-// wavefront per (request, KV head, two pages); K operands stay in registers over all rows.
-template <typename IO, int HD, int PARTS>
-__global__ __launch_bounds__(256) void q4_chunk_weights_kernel(const Q4Args a) {
-  constexpr int W = HD / 32, PB = q4_page_bytes(HD);
-  constexpr int ROWS = PARTS == 2 ? 8 : 16;
+// Totals of a chunk: the scores formed again, four pages (64 keys) per workgroup whose operands and pairs stay
+// in registers; the workgroup's wavefronts take the row tiles in turn and their sums meet in LDS in a fixed
+// order. READY: the tiles' q operands are in the workspace, left by the wide kernel (formed here they cost as
+// much as the scores). A block that two rows of the page table share is added to by both, hence the atomic;
+// otherwise each slot gets one addition.
+constexpr int kQ4SumWaves = 8, kQ4SumPages = 4;
+
+template <typename IO, int HD, int PARTS, bool READY>
+__global__ __launch_bounds__(64 * kQ4SumWaves) void q4_chunk_weights_kernel(const Q4Args a) {
+  constexpr int G = HD / kQ4Group, W = HD / 32, PB = q4_page_bytes(HD), PG = kQ4SumPages;
+  constexpr int ROWS = 16 / PARTS;
+  __shared__ float part[kQ4SumWaves][PG * kQ4Tokens];
   const int b = blockIdx.z, hk = blockIdx.y;
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
-  const int p0 = 2 * ((int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6));
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int p0 = PG * (int)blockIdx.x, key0 = p0 * kQ4Tokens;
   const int L = a.seq_lens[b], C = a.cur_lens[b];
-  int keys = L < a.max_pages * kQ4Tokens ? L : a.max_pages * kQ4Tokens;
-  if (p0 * kQ4Tokens >= keys || C < 1) return;
-  const int real = (C < a.T ? C : a.T) * a.group;  // rows behind it are padding
-  const int rows = a.T * a.group;
-  // rows that see the first of these keys: p0 * 16 < L - C + 1 + i
-  int i0 = p0 * kQ4Tokens - (L - C);
+  const int keys = L < a.max_pages * kQ4Tokens ? L : a.max_pages * kQ4Tokens;
+  if (key0 >= keys || C < 1) return;
+  const int rows = a.T * a.group, real = (C < a.T ? C : a.T) * a.group;  // rows behind `real` are padding
+  // the first row that sees the first of these keys: key0 < L - C + 1 + i
+  int i0 = key0 - (L - C);
   i0 = i0 > 0 ? i0 : 0;
   const int32_t* table = a.page_table + (int64_t)b * a.pt_stride;
-  int id[2];
-  Q4Raw<HD> r;
+  int id[PG];
+  f16x8 kf[PG][W];
+  u32x4 km[PG][G];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < PG; ++h) {
     id[h] = p0 + h < a.max_pages ? q4_block(__builtin_amdgcn_readfirstlane(table[p0 + h]), a.num_blocks) : -1;
-    const int64_t off = ((int64_t)(id[h] >= 0 ? id[h] : 0) * a.Hk + hk) * PB;
-    q4_load_page<HD>(a.k_pool + off, a.v_pool + off, lane, r, h);
+    const uint8_t* kp = a.k_pool + ((int64_t)(id[h] >= 0 ? id[h] : 0) * a.Hk + hk) * PB;
+    uint32_t kw[W];
+    q4_load_words(kp + (c * 4 + g) * (4 * W), kw);
+    q4_k_operands<HD, PARTS>(kw, kf[h]);
+#pragma unroll
+    for (int k = 0; k < G; ++k)
+      km[h][k] = *reinterpret_cast<const u32x4*>(kp + q4_codes_bytes(HD) + (k * kQ4Tokens + 4 * g) * 4);
   }
-  f16x8 kf[2][W];
+  float sum[PG][4];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) q4_k_operands<HD, PARTS>(r.k[h], kf[h]);
-  float sum[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-  for (int tile = i0 * a.group / ROWS; tile * ROWS < real; ++tile) {
-    Q4Wave<HD, PARTS> w;
-    q4_setup<IO, HD, PARTS>(a, b, hk, tile, L, C, keys, lane, w);
+  for (int h = 0; h < PG; ++h)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[h][i] = 0.f;
+  for (int tile = (int)((int64_t)i0 * a.group / ROWS) + wave; tile * ROWS < real; tile += kQ4SumWaves) {
+    f16x8 q[W];
+    float qs[G], sc;
+    int n;
+    if constexpr (READY) {
+      const int64_t at = ((int64_t)b * a.Hk + hk) * a.op_tiles + tile;
+#pragma unroll
+      for (int s = 0; s < W; ++s) q[s] = a.q_ops[(at * W + s) * 64 + lane];
+      const f32x4 x = a.q_aux[at * 64 + lane];
+#pragma unroll
+      for (int k = 0; k < G; ++k) qs[k] = x[k];
+      sc = x[2];
+      n = __float_as_int(x[3]);
+    } else {
+      Q4Wave<HD, PARTS> w;
+      q4_setup<IO, HD, PARTS>(a, b, hk, tile, L, C, keys, lane, w);
+#pragma unroll
+      for (int s = 0; s < W; ++s) q[s] = w.q[s];
+#pragma unroll
+      for (int k = 0; k < G; ++k) qs[k] = w.qs[k];
+      sc = w.sc;
+      n = w.n;
+    }
     const int row = q4_row<PARTS>(tile, c);
-    const float lse = row < real && c < ROWS ? *q4_lse(a, b, hk, row < rows ? row : rows - 1) : INFINITY;
+    const float lse = row < real && c < ROWS ? *q4_lse(a, b, hk, row < rows ? row : rows - 1) : INFINITY;  // (2^-inf: 0)
+    const bool masked = __any(n < key0 + PG * kQ4Tokens);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const f32x4 S = q4_scores<HD, PARTS>(kf[h], r.km[h], w.q, w.qs);
+    for (int h = 0; h < PG; ++h) {
+      const f32x4 S = q4_scores<HD, PARTS>(kf[h], km[h], q, qs);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float p = fast_exp2(fmaf(S[i], w.sc, -lse));
-        sum[h][i] += row < real && c < ROWS && (p0 + h) * kQ4Tokens + 4 * g + i < w.n ? p : 0.f;
+        const float p = fast_exp2(fmaf(S[i], sc, -lse));
+        sum[h][i] += masked && key0 + h * kQ4Tokens + 4 * g + i >= n ? 0.f : p;
       }
     }
   }
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
+  for (int h = 0; h < PG; ++h)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float s = group_sum<16>(sum[h][i]);
-      if (c == i && id[h] >= 0 && (p0 + h) * kQ4Tokens + 4 * g + i < keys)
-        atomicAdd(a.weights + ((int64_t)id[h] * a.Hk + hk) * kQ4Tokens + 4 * g + i, s);
+      if (c == i) part[wave][h * kQ4Tokens + 4 * g + i] = s;
     }
+  __syncthreads();
+  const int t = threadIdx.x;
+  if (t < PG * kQ4Tokens && key0 + t < keys) {
+    const int block = q4_block(table[p0 + t / kQ4Tokens], a.num_blocks);
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < kQ4SumWaves; ++w) s += part[w][t];
+    if (block >= 0) atomicAdd(a.weights + ((int64_t)block * a.Hk + hk) * kQ4Tokens + (t & (kQ4Tokens - 1)), s);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -1151,7 +1165,8 @@ struct Q4Plan {
   bool wide;
   int tiles, splits, split_pages;
   int64_t rows;
-  size_t rec, lse, scores, score_stride, bytes;
+  size_t rec, lse, scores, score_stride, ops, aux, bytes;  // (the parts in floats)
+  int op_tiles;
 };
 
 // Which kernel, how many row tiles and key ranges, and the workspace.
@@ -1165,8 +1180,9 @@ static Q4Plan q4_plan(int io_dtype, int32_t batch, int32_t heads, int32_t kv_hea
   p.rows_per_tile = p.wide ? kQ4WideWaves * rpt : rpt;
   p.tiles = (int)((p.rows + p.rows_per_tile - 1) / p.rows_per_tile);
   const int64_t units = (int64_t)batch * kv_heads * p.tiles;
-  const int64_t target = 2 * (int64_t)pa_host::device_cu_count();
-  const int64_t want = units > 0 ? (target + units - 1) / units : 1;
+  // workgroups that the GPU holds; more ranges than fit would wait for a second round
+  const int64_t target = (p.wide ? (head_dim == 64 ? 4 : 3) : 2) * (int64_t)pa_host::device_cu_count();
+  const int64_t want = units <= 0 ? 1 : p.wide ? (target / units > 1 ? target / units : 1) : (target + units - 1) / units;
   int pages = (int)((max_pages + want - 1) / want);
   const int least = p.wide ? 16 : 64;
   if (!p.wide && pages > 96) pages = 96;  // requests of very different lengths: ranges end together
@@ -1178,10 +1194,15 @@ static Q4Plan q4_plan(int io_dtype, int32_t batch, int32_t heads, int32_t kv_hea
   p.lse = weights ? (size_t)batch * kv_heads * p.rows : 0;
   p.score_stride = (size_t)(max_pages + (max_pages & 1)) * kQ4Tokens;
   p.scores = weights && query_len == 1 && !p.wide ? (size_t)batch * heads * p.score_stride : 0;
+  p.op_tiles = p.tiles * kQ4WideWaves;
+  const size_t ops = weights && p.wide ? (size_t)batch * kv_heads * p.op_tiles * 64 : 0;
+  p.ops = ops * (head_dim / 32) * (sizeof(f16x8) / sizeof(float));
+  p.aux = ops * (sizeof(f32x4) / sizeof(float));
   auto up = [](size_t n) { return (n + 63) / 64 * 64; };
   p.rec = up(p.rec);
   p.lse = up(p.lse);
-  p.bytes = (p.rec + p.lse + p.scores) * sizeof(float);
+  p.scores = up(p.scores);
+  p.bytes = (p.rec + p.lse + p.scores + p.ops + p.aux) * sizeof(float);
   return p;
 }
 
@@ -1205,8 +1226,11 @@ static void launch_q4(const Q4Args& a, const Q4Plan& p, hipStream_t stream) {
     q4_finish_kernel<IO, HD><<<(unsigned)wgs, 256, 0, stream>>>(a, total, merges, chunks);
   }
   if (a.weights != nullptr && a.scores == nullptr) {
-    const dim3 wg((unsigned)((a.max_pages + 7) / 8), a.Hk, a.B);
-    q4_chunk_weights_kernel<IO, HD, PARTS><<<wg, 256, 0, stream>>>(a);
+    const dim3 wg((unsigned)((a.max_pages + kQ4SumPages - 1) / kQ4SumPages), a.Hk, a.B);
+    if (a.q_ops != nullptr)
+      q4_chunk_weights_kernel<IO, HD, PARTS, true><<<wg, 64 * kQ4SumWaves, 0, stream>>>(a);
+    else
+      q4_chunk_weights_kernel<IO, HD, PARTS, false><<<wg, 64 * kQ4SumWaves, 0, stream>>>(a);
   }
 }
 
@@ -1272,6 +1296,10 @@ extern "C" int pa_q4_attention(const void* q, int64_t q_stride_b, int64_t q_stri
   a.lse = p.lse ? ws + p.rec : nullptr;
   a.scores = p.scores ? ws + p.rec + p.lse : nullptr;
   a.score_stride = (int64_t)p.score_stride;
+  float* ops = ws + p.rec + p.lse + p.scores;
+  a.q_ops = p.ops && a.weights ? reinterpret_cast<f16x8*>(ops) : nullptr;
+  a.q_aux = reinterpret_cast<f32x4*>(ops + p.ops);
+  a.op_tiles = p.op_tiles;
   hipStream_t stream = static_cast<hipStream_t>(stream_);
   if (io_dtype == PA_DTYPE_F32) {
     if (head_dim == 64) launch_q4<float, 64, 2>(a, p, stream); else launch_q4<float, 128, 2>(a, p, stream);
