@@ -74,19 +74,24 @@ __global__ __launch_bounds__(kSelThreads) void q4_choose_kernel(const Q4EvictArg
     return id < 0 ? 0u : q4_rank(a.weights[((int64_t)id * a.Hk + hk) * kQ4Tokens + (t & (kQ4Tokens - 1))]);
   };
   const int in_lds = cand < a.held ? cand : a.held;
-  for (int t = tid; t < in_lds; t += kSelThreads) held[t] = total_at(t);
-  __syncthreads();
-  auto rank = [&](int t) { return t < in_lds ? held[t] : total_at(t); };
-
   int want = a.keep - a.window;  // of the candidates
   uint32_t prefix = 0;
   for (int shift = 24; shift >= 0 && want > 0; shift -= 8) {
     for (int i = lane; i < 256; i += 64) hist[wave][i] = 0;
     __syncthreads();
-    const uint32_t mask = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-    for (int t = tid; t < cand; t += kSelThreads) {
-      const uint32_t u = rank(t);
-      if ((u & mask) == prefix) atomicAdd(&hist[wave][u >> shift & 255], 1);
+    if (shift == 24) {  // the totals come from memory, four at a time on their way
+#pragma unroll 4
+      for (int t = tid; t < cand; t += kSelThreads) {
+        const uint32_t u = total_at(t);
+        if (t < in_lds) held[t] = u;
+        atomicAdd(&hist[wave][u >> 24], 1);
+      }
+    } else {
+      const uint32_t mask = 0xffffffffu << (shift + 8);
+      for (int t = tid; t < cand; t += kSelThreads) {
+        const uint32_t u = t < in_lds ? held[t] : total_at(t);
+        if ((u & mask) == prefix) atomicAdd(&hist[wave][u >> shift & 255], 1);
+      }
     }
     __syncthreads();
     if (tid < 256) {
@@ -124,6 +129,7 @@ __global__ __launch_bounds__(kSelThreads) void q4_choose_kernel(const Q4EvictArg
     want -= found_above;
     __syncthreads();
   }
+  auto rank = [&](int t) { return t < in_lds ? held[t] : total_at(t); };
   // kept: totals above `prefix`, and the first `want` equal to it (none where nothing was wanted)
   const bool any = a.keep > a.window;
   const int per = ((cand + kSelWaves - 1) / kSelWaves + 63) / 64 * 64;
@@ -208,12 +214,26 @@ __global__ __launch_bounds__(256) void q4_move_kernel(const Q4EvictArgs a, int p
   for (int e = 0; e < 4; ++e) {
     const int te = __shfl(t, 4 * g + e), fe = __shfl(from, 4 * g + e);
     const int ke = te & (kQ4Tokens - 1);
-    const uint16_t* vs = reinterpret_cast<const uint16_t*>(a.v_pool + (int64_t)fe * stride + head) +
-                         (((ke >> 2) * 16 + c) * 2 + (ke >> 1 & 1)) * G * 2 + (ke & 1);
+    // word p of the token's quadruple, both groups; its half is the token's
+    const uint32_t* vs = reinterpret_cast<const uint32_t*>(a.v_pool + (int64_t)fe * stride + head) +
+                         (((ke >> 2) * 16 + c) * 2 + (ke >> 1 & 1)) * G;
+    uint32_t word[G];
+    if (te >= 0 && fe >= 0) {
+      if constexpr (G == 2) {
+        const u32x2 x = *reinterpret_cast<const u32x2*>(vs);
+        word[0] = x[0];
+        word[1] = x[1];
+      } else {
+        word[0] = vs[0];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < G; ++i) word[i] = 0;
+    }
     ok |= (uint32_t)(te >= 0) << e;
 #pragma unroll
     for (int i = 0; i < G; ++i) {
-      const uint32_t w = te >= 0 && fe >= 0 ? vs[2 * i] : 0u;
+      const uint32_t w = ke & 1 ? word[i] >> 16 : word[i] & 0xffffu;
       v[e >> 1][i] = e & 1 ? v[e >> 1][i] | w << 16 : w;
     }
   }
