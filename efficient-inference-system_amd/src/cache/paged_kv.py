@@ -75,6 +75,8 @@ class KVStorage:
 
 
 class LayerBlockPool:
+    is_q4 = False  # blocks of 4-bit pages (src/cache/q4_kv.py)
+
     def __init__(
         self,
         block_size: int,
@@ -113,6 +115,10 @@ class LayerBlockPool:
         self.device = torch.device(device)
         self._grow(self.initial_blocks)
 
+    def _block_shape(self) -> tuple:
+        """Shape of one block of K or V."""
+        return (self.num_heads, self.block_size, self.head_dim)
+
     def _grow(self, min_extra_blocks: int) -> None:
         if self.num_heads is None or self.head_dim is None or self.dtype is None or self.device is None:
             raise ValueError("Pool must be initialized before growth.")
@@ -126,7 +132,7 @@ class LayerBlockPool:
         if self.storage is not None:
             # Same logical growth, as a longer view of fixed storage: the new blocks are zeroed
             # (the storage may hold an earlier pool's data) and existing blocks keep their place.
-            tail = (self.num_heads, self.block_size, self.head_dim)
+            tail = self._block_shape()
             old_cap = self.capacity_blocks
             self.storage.ensure(tail, self.dtype, self.device, old_cap + grow_by, keep=old_cap)
             self.storage.k[old_cap:old_cap + grow_by].zero_()
@@ -134,8 +140,7 @@ class LayerBlockPool:
             self.k_blocks = self.storage.k[: old_cap + grow_by]
             self.v_blocks = self.storage.v[: old_cap + grow_by]
         else:
-            new_k = torch.zeros(grow_by, self.num_heads, self.block_size, self.head_dim, dtype=self.dtype,
-                                device=self.device)
+            new_k = torch.zeros(grow_by, *self._block_shape(), dtype=self.dtype, device=self.device)
             new_v = torch.zeros_like(new_k)
             if self.k_blocks is None:
                 self.k_blocks = new_k
@@ -180,6 +185,20 @@ class LayerBlockPool:
         self.free_block_ids.extend(block_ids)
         self.mutations += 1
 
+    def put_rows(self, blocks: torch.Tensor, offsets: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
+        """Rows [n, heads, head_dim] of host tensors into token offsets[i] of block blocks[i]."""
+        for pool_blocks, new in ((self.k_blocks, k), (self.v_blocks, v)):
+            pool_blocks[blocks, :, offsets, :] = new.to(pool_blocks.dtype)
+
+    def tiles(self, ids: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """K and V of the given blocks as values, [n, heads, block_size, head_dim] each."""
+        return self.k_blocks.index_select(0, ids), self.v_blocks.index_select(0, ids)
+
+    def token_bytes(self) -> int:
+        """Bytes of one token's K and V."""
+        kb = self.k_blocks
+        return kb.shape[1] * kb.shape[3] * 2 * kb.element_size()
+
     def bytes_per_block(self) -> int:
         if self.k_blocks is None:
             return 0
@@ -212,8 +231,7 @@ class PagedKVCacheState:
         bs = self.pool.block_size
         pos = torch.arange(start, start + length)
         blocks = torch.tensor(self.block_ids, dtype=torch.long)[pos // bs]
-        for pool_blocks, new in ((self.pool.k_blocks, k_new), (self.pool.v_blocks, v_new)):
-            pool_blocks[blocks, :, pos % bs, :] = new[0, :, :length, :].transpose(0, 1).to(pool_blocks.dtype)
+        self.pool.put_rows(blocks, pos % bs, k_new[0, :, :length, :].transpose(0, 1), v_new[0, :, :length, :].transpose(0, 1))
 
     def release(self) -> None:
         self.pool.release_blocks(list(self.block_ids))
@@ -223,8 +241,7 @@ class PagedKVCacheState:
     def live_bytes(self) -> int:
         if self.pool.k_blocks is None:
             return 0
-        kb = self.pool.k_blocks
-        return self.seq_len * kb.shape[1] * kb.shape[3] * 2 * kb.element_size()
+        return self.seq_len * self.pool.token_bytes()
 
     def reserved_bytes(self) -> int:
         return len(self.block_ids) * self.pool.bytes_per_block()
@@ -383,10 +400,41 @@ class BatchedPagedKVCache:
         app = [max(min(n, T), 0) for n in lengths]
         prev = self.host_append(app, T, H, Hd, k_new.dtype, k_new.device)
         page_table, seq32, seq64, slots = self._pack(k_new.device, T, prev, app, True)
-        if any(app):
+        if any(app) and pool.is_q4:
+            from src.kernels.hip_q4_attention import kv_append_q4_hip
+
+            kv_append_q4_hip(k_new, v_new, pool.k_blocks, pool.v_blocks, slots, weights=pool.weights)
+        elif any(app):
             kv_append_hip(k_new, v_new, pool.k_blocks, pool.v_blocks, slots)
         self._meta = (self._signature(), page_table, seq32)
         return seq64
+
+    def evict(self, keep: int, window: int, limit: int | None = None) -> list[torch.Tensor | None]:
+        """Cut every state of more than `limit` cached keys (default: keep) back to `keep` keys per KV head:
+        the newest `window` and, of the others, those of the largest attention weight so far. The pool must
+        hold 4-bit pages with weights (src/cache/q4_kv.py). The kept rows move to new blocks, the old ones
+        are released. Returns per state the kept keys' old indices, int32 [heads, keep], or None."""
+        if not self.pool.is_q4 or not self.pool.track_weights:
+            raise ValueError("evict needs a pool of 4-bit pages that keeps the keys' attention weights")
+        if keep < 1 or not 0 <= window <= keep:
+            raise ValueError(f"keep ({keep}) must be positive and hold the window ({window})")
+        limit = keep if limit is None else max(limit, keep)
+        rows = [i for i, st in enumerate(self.states) if st.seq_len > limit]
+        if len({id(self.states[i]) for i in rows}) != len(rows):
+            raise ValueError("a state appears twice in the batch")
+        if not rows:
+            return [None] * len(self.states)
+        states = [self.states[i] for i in rows]
+        fresh = [[self.pool.allocate_block() for _ in range(-(-keep // self.pool.block_size))] for _ in states]
+        kept = self.pool.evict_rows([list(st.block_ids) for st in states], [st.seq_len for st in states], fresh, keep, window)
+        out: list[torch.Tensor | None] = [None] * len(self.states)
+        for i, st, new, index in zip(rows, states, fresh, kept):
+            self.pool.release_blocks(list(st.block_ids))
+            st.block_ids[:] = new
+            st.seq_len = keep
+            out[i] = index
+        self._meta = None
+        return out
 
     # ------------------------------------------------------------------------------------------
     def page_table_tensor(self, device: torch.device | None = None) -> torch.Tensor:

@@ -2,7 +2,9 @@
 
 Differences from the reference, all additive:
   - the default attention backend is "hip_paged" (the reference's is "triton_paged");
-  - ModelConfig.kv_cache_dtype (None = the model dtype) selects a bf16 KV pool under an fp32 model;
+  - ModelConfig.kv_cache_dtype (None = the model dtype) selects a bf16 KV pool under an fp32 model, or
+    ("int4") pools of 4-bit pages, with track_attention_weights also the keys' accumulated attention weights;
+  - KVEviction: when and to what a request's cached keys are cut back;
   - benchmark_serving_request_mix() is the request mix of the end-to-end continuous-batching
     benchmark (200 Poisson requests at 32 req/s), which differs from default_serving_request_mix().
 """
@@ -52,6 +54,20 @@ def benchmark_serving_request_mix() -> list[RequestWorkloadProfile]:
 ATTENTION_BACKENDS = frozenset({"paged_reference", "hip_paged"})
 
 
+@dataclass(frozen=True)
+class KVEviction:
+    """A request of more than `limit` cached keys is cut back to `keep` of them per KV head: the newest
+    `window`, and of the others those of the largest attention weight so far. Needs a model with
+    kv_cache_dtype "int4" and track_attention_weights."""
+    limit: int
+    keep: int
+    window: int
+
+    def __post_init__(self):
+        if not 0 <= self.window <= self.keep <= self.limit or self.keep < 1:
+            raise ValueError(f"KVEviction wants 0 <= window <= keep <= limit and keep >= 1, got {self}")
+
+
 @dataclass
 class ModelConfig:
     vocab_size: int = 5000
@@ -66,7 +82,8 @@ class ModelConfig:
     kv_pool_initial_blocks: int = 64
     kv_pool_growth_factor: float = 2.0
     enable_attention_correctness_checks: bool = False
-    kv_cache_dtype: torch.dtype | None = None
+    kv_cache_dtype: torch.dtype | str | None = None
+    track_attention_weights: bool = False
 
 
 @dataclass

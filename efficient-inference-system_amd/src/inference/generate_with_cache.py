@@ -13,7 +13,8 @@ both sides (the argmax is inside the timed step, as in the reference):
     last token at position prompt_length + generated - 1. The per-layer states of the active
     requests are batched afresh every round; a request's states persist across rounds.
 On the hip_paged backend every decode round replays a captured graph that ends in the argmax, so
-a round reads back only the active requests' token ids.
+a round reads back only the active requests' token ids. With `eviction` (a model over 4-bit pages that keeps
+attention weights) requests past its limit are cut back after every step, outside the timed sections.
 """
 from __future__ import annotations
 
@@ -21,6 +22,7 @@ import numpy as np
 import torch
 
 from src.cache.paged_kv import BatchedPagedKVCache, PagedKVCacheState
+from src.config import KVEviction
 from src.utils.timing import timed_section
 
 
@@ -95,7 +97,8 @@ def _memory(device: torch.device) -> tuple[int, int]:
 
 
 @torch.no_grad()
-def generate_with_cache(model, prompt_ids: torch.Tensor, max_new_tokens, prompt_lengths: torch.Tensor | None = None):
+def generate_with_cache(model, prompt_ids: torch.Tensor, max_new_tokens, prompt_lengths: torch.Tensor | None = None,
+                        eviction: KVEviction | None = None):
     device = prompt_ids.device
     B, width = prompt_ids.shape
     gen = _Generation(prompt_ids, _per_request(prompt_lengths, B, width), _per_request(max_new_tokens, B, 0))
@@ -116,6 +119,8 @@ def generate_with_cache(model, prompt_ids: torch.Tensor, max_new_tokens, prompt_
     first = tokens.tolist()
     gen.take([r for r in range(B) if gen.limits[r] > 0], [first[r] for r in range(B) if gen.limits[r] > 0])
     gen.keep_states(caches, B)
+    if eviction is not None:
+        model.evict_kv_caches(caches, eviction)
 
     step_times: list[float] = []
     step_sizes: list[int] = []
@@ -132,6 +137,8 @@ def generate_with_cache(model, prompt_ids: torch.Tensor, max_new_tokens, prompt_
         step_sizes.append(len(active))
         gen.adopt(active, batched)
         gen.take(active, tokens.tolist())
+        if eviction is not None:
+            model.evict_kv_caches(batched, eviction)
 
     live, reserved, fragmentation = gen.kv_bytes(model)
     allocated, peak = _memory(device)

@@ -24,18 +24,7 @@ import torch
 
 from src.kernels import _lib
 from src.kernels.hip_paged_attention import _call_workspace, _check_out, _require_i32, _stream_ptr, native_call
-
-BLOCK = 16
-GROUP = 64
-HEAD_DIMS = (64, 128)
-
-
-def page_bytes(head_dim: int) -> int:
-    """Bytes of one page of one KV head (as pa_q4_page_bytes, without the library)."""
-    if head_dim not in HEAD_DIMS:
-        raise ValueError(f"4-bit pages hold head_dim 64 or 128, got {head_dim}")
-    return BLOCK * (head_dim // 2 + 4 * (head_dim // GROUP))
-
+from src.kernels.reference_q4 import BLOCK, HEAD_DIMS, page_bytes
 
 def _on_device(device: torch.device):
     """The device of the operands as the current one, for a launch on its stream."""

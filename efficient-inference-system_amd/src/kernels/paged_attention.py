@@ -4,7 +4,8 @@ Same signature and contract as src/kernels/paged_attention.py:13-51 of the refer
 `paged_attention(backend, q [B, H, T, Hd], kv_cache, current_lengths) -> [B, H, T, Hd]`, called
 after `kv_cache.append_batch(...)`. current_lengths is normalised to an int32 device tensor
 (None -> T, int -> that value, tensor -> cast), then query_len 1 goes to the decode kernel and
-anything longer to the chunked-prefill kernel.
+anything longer to the chunked-prefill kernel; a cache whose pool holds 4-bit pages goes to the kernels
+that read those, and to its weights, if it keeps them, each key's attention weight is added.
 
 Backends: "paged_reference" (torch, any device) and "hip_paged" (libpaged_hip.so on a HIP device).
 Unlike the reference, which silently sends CPU tensors to its torch loop, "hip_paged" refuses
@@ -70,6 +71,11 @@ def paged_attention(
         return torch.zeros_like(q)
     page_table, seq_lens = kv_cache.device_metadata(q.device)
     cur = _lengths_tensor(current_lengths, batch_size, query_len, q.device)
+    if pool.is_q4:
+        from src.kernels.hip_q4_attention import paged_attention_decode_q4_hip, paged_attention_prefill_q4_hip
+
+        attend = paged_attention_decode_q4_hip if query_len == 1 else paged_attention_prefill_q4_hip
+        return attend(q, pool.k_blocks, pool.v_blocks, page_table, seq_lens, cur, weights=pool.weights)
     if query_len == 1:
         return paged_attention_decode_hip(q, pool.k_blocks, pool.v_blocks, page_table, seq_lens, cur)
     return paged_attention_prefill_hip(q, pool.k_blocks, pool.v_blocks, page_table, seq_lens, cur)

@@ -47,8 +47,9 @@ def paged_attention_reference(
         if ids.numel() < nblocks:
             raise IndexError(f"request {batch_idx}: {ids.numel()} blocks cannot hold {seq_len} tokens")
         # [nblocks, H, bs, Hd] -> [H, nblocks*bs, Hd] -> first seq_len keys
-        k = state.pool.k_blocks.index_select(0, ids).permute(1, 0, 2, 3).reshape(num_heads, nblocks * bs, head_dim)
-        v = state.pool.v_blocks.index_select(0, ids).permute(1, 0, 2, 3).reshape(num_heads, nblocks * bs, head_dim)
+        k, v = (t.permute(1, 0, 2, 3).reshape(-1, nblocks * bs, head_dim) for t in state.pool.tiles(ids))
+        if k.shape[0] != num_heads:  # query heads that share KV heads
+            k, v = (t.repeat_interleave(num_heads // t.shape[0], 0) for t in (k, v))
         k = k[:, :seq_len].to(q.dtype).contiguous()
         v = v[:, :seq_len].to(q.dtype).contiguous()
         qb = q[batch_idx].contiguous()  # [H, T, Hd]
@@ -61,5 +62,11 @@ def paged_attention_reference(
         has_key = allowed.any(dim=1).view(1, query_len, 1)
         weights = torch.where(has_key, weights, torch.zeros_like(weights))
         out[batch_idx] = torch.matmul(weights, v)
+        totals = getattr(state.pool, "weights", None)
+        if totals is not None:  # the keys' weights from the real rows, summed over the heads of each KV head
+            added = weights[:, :max(min(cur[batch_idx], query_len), 0)].float().sum(1)
+            added = added.unflatten(0, (totals.shape[1], -1)).sum(1)
+            added = torch.nn.functional.pad(added, (0, nblocks * bs - seq_len)).unflatten(1, (nblocks, bs))
+            totals.index_add_(0, ids, added.transpose(0, 1).contiguous())
     del pool
     return out

@@ -385,7 +385,7 @@ class GraphedStep:
                 and all(isinstance(c, BatchedPagedKVCache) for c in kv_caches)):
             return False
         B, T = input_ids.shape
-        if bucket_for(T) is None:
+        if bucket_for(T) is None or kv_caches[0].pool.is_q4:  # (4-bit pools: eager steps)
             return False
         states0 = kv_caches[0].states
         if len({id(st) for st in states0}) != len(states0):

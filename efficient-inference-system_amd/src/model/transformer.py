@@ -2,7 +2,8 @@
 
 TinyTransformerLM: token + learned position embeddings, pre-LayerNorm blocks (attention, GELU
 MLP), final LayerNorm, bias-free lm_head; one LayerBlockPool per layer, created lazily, each a
-view of a per-layer KVStorage the model keeps (fixed device addresses). Module and parameter
+view of a per-layer KVStorage the model keeps (fixed device addresses); with kv_cache_dtype "int4" the pools
+hold 4-bit pages (src/cache/q4_kv.py), whose steps run eagerly. Module and parameter
 names match the reference so state dicts load across the two. On the "hip_paged" backend, cached
 steps over per-layer batched caches (decode steps and prefill chunks up to 256 tokens) replay
 captured HIP graphs (src/model/graph_decode.py); everything else runs eagerly.
@@ -17,7 +18,8 @@ try:  # native host checks (csrc/host/paged_host.cpp); the Python versions below
     from src.cache import _paged_host as _host
 except ImportError:
     _host = None
-from src.config import ATTENTION_BACKENDS
+from src.cache.q4_kv import Q4BlockPool
+from src.config import ATTENTION_BACKENDS, KVEviction
 from src.model.attention import CausalSelfAttention
 
 
@@ -56,12 +58,17 @@ class TinyTransformerLM(nn.Module):
         kv_pool_initial_blocks: int = 64,
         kv_pool_growth_factor: float = 2.0,
         enable_attention_correctness_checks: bool = False,
-        kv_cache_dtype: torch.dtype | None = None,
+        kv_cache_dtype: torch.dtype | str | None = None,
         kv_pool_reserve_blocks: int | None = None,
+        track_attention_weights: bool = False,
     ):
         super().__init__()
         if attention_backend not in ATTENTION_BACKENDS:
             raise ValueError(f"Unsupported attention backend: {attention_backend}")
+        if isinstance(kv_cache_dtype, str) and kv_cache_dtype != "int4":
+            raise ValueError(f"kv_cache_dtype is a torch dtype, \"int4\" or None, got {kv_cache_dtype!r}")
+        if track_attention_weights and kv_cache_dtype != "int4":
+            raise ValueError("track_attention_weights needs kv_cache_dtype \"int4\"")
         self.vocab_size = vocab_size
         self.max_seq_len = max_seq_len
         self.attention_backend = attention_backend
@@ -70,6 +77,7 @@ class TinyTransformerLM(nn.Module):
         self.kv_pool_growth_factor = kv_pool_growth_factor
         self.enable_attention_correctness_checks = enable_attention_correctness_checks
         self.kv_cache_dtype = kv_cache_dtype
+        self.track_attention_weights = track_attention_weights
         self.num_heads = num_heads
         self.head_dim = d_model // num_heads
         self.token_emb = nn.Embedding(vocab_size, d_model)
@@ -88,7 +96,14 @@ class TinyTransformerLM(nn.Module):
         self._graph_step = None
 
     def _ensure_layer_block_pools(self) -> list[LayerBlockPool]:
-        if self.layer_block_pools is None:
+        if self.layer_block_pools is None and self.kv_cache_dtype == "int4":
+            self.layer_block_pools = [
+                Q4BlockPool(self.kv_block_size, self.kv_pool_initial_blocks, self.kv_pool_growth_factor,
+                            track_weights=self.track_attention_weights,
+                            storage=self._kv_storages[i] if self._kv_storages else None)
+                for i in range(len(self.blocks))
+            ]
+        elif self.layer_block_pools is None:
             self.layer_block_pools = [
                 LayerBlockPool(
                     block_size=self.kv_block_size,
@@ -122,7 +137,8 @@ class TinyTransformerLM(nn.Module):
         from src.model.graph_decode import T_BUCKETS
 
         device = torch.device(device)
-        if device.type != "cuda" or self.attention_backend != "hip_paged" or self._kv_storages is None:
+        if (device.type != "cuda" or self.attention_backend != "hip_paged" or self._kv_storages is None
+                or self.kv_cache_dtype == "int4"):
             return 0
         runner = self._graph_runner()
         before = runner.captures
@@ -168,6 +184,16 @@ class TinyTransformerLM(nn.Module):
         for cache in request_caches:
             if isinstance(cache, PagedKVCacheState):
                 cache.release()
+
+    def evict_kv_caches(self, kv_caches, eviction: KVEviction) -> int:
+        """Cut the requests of the per-layer batched caches (or single states) back as `eviction` says;
+        returns how many (request, layer) caches were cut."""
+        cut = 0
+        for cache in kv_caches or ():
+            if isinstance(cache, PagedKVCacheState):
+                cache = BatchedPagedKVCache([cache], cache.pool)
+            cut += sum(x is not None for x in cache.evict(eviction.keep, eviction.window, eviction.limit))
+        return cut
 
     def release_kv_caches(self, kv_caches) -> None:
         if kv_caches is None:

@@ -32,6 +32,7 @@ import numpy as np
 import torch
 
 from src.cache.paged_kv import BatchedPagedKVCache, PagedKVCacheState
+from src.config import KVEviction
 from src.utils.timing import timed_section
 
 
@@ -119,13 +120,15 @@ def _kv_bytes_per_token(model) -> int:
 class StepExecutor:
     """Runs planned steps on `model`. keep_logits: also return each step's logits (for tests;
     on the graph path this copies them out of the graph); observer(plan, tokens, logits, event):
-    called after every step."""
+    called after every step; eviction: cut the step's requests back after it (a model over 4-bit pages that
+    keeps attention weights)."""
 
-    def __init__(self, model, device, keep_logits: bool = False, observer=None):
+    def __init__(self, model, device, keep_logits: bool = False, observer=None, eviction: KVEviction | None = None):
         self.model = model
         self.device = device
         self.keep_logits = keep_logits
         self.observer = observer
+        self.eviction = eviction
 
     def _execute(self, plan: StepPlan) -> tuple[list[int], torch.Tensor | None, float]:
         caches = _layer_batches(self.model, plan.requests)
@@ -134,6 +137,8 @@ class StepExecutor:
                 plan.token_ids, caches, position_offset=plan.positions, current_lengths=plan.lengths,
                 select_rows=plan.rows, return_logits=self.keep_logits)
         tokens = [int(t) for t in tokens.tolist()]  # the step's only device->host read
+        if self.eviction is not None:
+            self.model.evict_kv_caches(caches, self.eviction)
         _adopt(plan.requests, caches)
         return tokens, logits, timer.elapsed_ms
 
