@@ -629,7 +629,7 @@ struct Q4Batch {
   static constexpr int G = HD / kQ4Group, W = HD / 32;
   // pages that share a softmax: 8 at most, which 190 registers hold at head_dim 128 (16 spill)
   static constexpr int COLS = 16 / PARTS, PG = COLS / GP < 8 ? COLS / GP : 8;
-  static constexpr int PAGES = PG < 4 ? 4 : PG, NB = PAGES / PG;
+  static constexpr int PAGES = PG == 1 ? 2 : PG < 4 ? 4 : PG, NB = PAGES / PG;
   uint32_t k[PAGES][W], v[PAGES][2 * G];
   u32x4 km[NB][G], vm[NB][G];
   int live[NB];  // this lane's pages: 1 where the page is there
@@ -722,6 +722,7 @@ __global__ __launch_bounds__(64 * kQ4Waves, 2) void q4_narrow_kernel(const Q4Arg
 
   f32x4 start[G], o[G][4];
   float y[G], l = 0.f, M = kNegBig;
+  const float zero = q4_zero();
 #pragma unroll
   for (int k = 0; k < G; ++k) {
     const float s0 = PARTS == 2 ? 0.f : -7.5f * qs[k];
@@ -802,26 +803,25 @@ __global__ __launch_bounds__(64 * kQ4Waves, 2) void q4_narrow_kernel(const Q4Arg
           }
         }
       }
+      // what a row does not see takes part with score -inf and the pair (0, 0)
       f32x4 S[NB];
-      bool see[NB][4];
       u32x4 vm[NB][G];
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
-        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+        f32x4 x = {zero, zero, zero, zero};
 #pragma unroll
-        for (int k = 0; k < G; ++k) {
+        for (int k = 0; k < G; ++k)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            x[i] = fmaf(q4_scale(r.km[nb][k][i]), acc[nb][k][i],
-                        k == 0 ? q4_centre(r.km[nb][k][i]) * qs[k] : fmaf(q4_centre(r.km[nb][k][i]), qs[k], x[i]));
-          vm[nb][k] = r.vm[nb][k];
-        }
+            x[i] = fmaf(q4_scale(r.km[nb][k][i]), acc[nb][k][i], fmaf(q4_centre(r.km[nb][k][i]), qs[k], x[i]));
         const int key = (p + nb * PG + page_in) * kQ4Tokens + 4 * g;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if constexpr (PARTS == 2) x[i] += dpp<0x128>(x[i]);
-          see[nb][i] = r.live[nb] && key + i < n;
-          S[nb][i] = see[nb][i] ? x[i] * sc : -INFINITY;
+          const bool see = r.live[nb] && key + i < n;
+          S[nb][i] = see ? x[i] * sc : -INFINITY;
+#pragma unroll
+          for (int k = 0; k < G; ++k) vm[nb][k][i] = see ? r.vm[nb][k][i] : 0u;
         }
         if (scores != nullptr && p + nb * PG + page_in < p1)
           *reinterpret_cast<f32x4*>(scores + (p + nb * PG + page_in) * kQ4Tokens) = S[nb];
@@ -830,29 +830,55 @@ __global__ __launch_bounds__(64 * kQ4Waves, 2) void q4_narrow_kernel(const Q4Arg
         next_ids(p + PAGES);
         load_k(p + PAGES);
       }
-      float pr[NB][4], far = 0.f;
-      float vs[NB][4];
+      float pr[NB][4];
+      uint32_t w[NB][G][2];
+#pragma unroll 1
+      for (int pass = 0; pass < 2; ++pass) {  // (as in q4_step)
+        float big = 0.f;
+        s16x2 top = {0, 0};
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
+        for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float m = kQ4Floor;
+          for (int i = 0; i < 4; ++i) {
+            pr[nb][i] = fast_exp2(S[nb][i] - M);
+            big = fmaxf(big, pr[nb][i]);
+          }
 #pragma unroll
-          for (int k = 0; k < G; ++k) m = fmaxf(m, q4_scale(vm[nb][k][i]));
-          vs[nb][i] = see[nb][i] ? m : 0.f;
-          pr[nb][i] = fast_exp2(S[nb][i] - M);
-          far = fmaxf(far, pr[nb][i] * vs[nb][i]);
+          for (int k = 0; k < G; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+              f16x2 hi, part;
+              if constexpr (PARTS == 1) {
+                hi = part = q4_weights(pr[nb][i], vm[nb][k][i], pr[nb][i + 1], vm[nb][k][i + 1]);
+              } else {
+#pragma unroll
+                for (int f = 0; f < 2; ++f) {
+                  const float x = pr[nb][i + f] * q4_scale(vm[nb][k][i + f]);
+                  hi[f] = (_Float16)x;
+                  const _Float16 rest = (_Float16)(x - (float)hi[f]);
+                  part[f] = low ? rest : hi[f];
+                }
+              }
+              top = __builtin_elementwise_max(top, __builtin_bit_cast(s16x2, hi));
+              w[nb][k][i / 2] = __builtin_bit_cast(uint32_t, part);
+            }
         }
-      if (__builtin_expect(__any(far > kQ4Limit), 0)) {
+        const bool far = top[0] > kQ4LimitBits || top[1] > kQ4LimitBits || big > kQ4Limit / kQ4Floor;
+        if (__builtin_expect(!__any(far), 1)) break;
         float m = kNegBig;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            m = fmaxf(m, see[nb][i] ? S[nb][i] + __builtin_amdgcn_logf(vs[nb][i]) - kQ4Start : kNegBig);
+          for (int i = 0; i < 4; ++i) {
+            float s = kQ4Floor;
+            asm volatile("" : "+v"(s));
+#pragma unroll
+            for (int k = 0; k < G; ++k) s = fmaxf(s, q4_scale(vm[nb][k][i]));
+            m = fmaxf(m, S[nb][i] + __builtin_amdgcn_logf(s) - kQ4Start);
+          }
         m = row_max<GP>(max_xor32(max_xor16(m)));
-        const float top = fmaxf(M, m), f = fast_exp2(M - top);
-        M = top;
+        const float now = fmaxf(M, m), f = fast_exp2(M - now);
+        M = now;
         l *= f;
 #pragma unroll
         for (int k = 0; k < G; ++k) {
@@ -860,34 +886,20 @@ __global__ __launch_bounds__(64 * kQ4Waves, 2) void q4_narrow_kernel(const Q4Arg
 #pragma unroll
           for (int t = 0; t < 4; ++t) o[k][t] *= f;
         }
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) pr[nb][i] = fast_exp2(S[nb][i] - M);
       }
-      uint32_t w[NB][G][2];
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) l += pr[nb][i];
 #pragma unroll
         for (int k = 0; k < G; ++k) {
-          _Float16 h[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t m = vm[nb][k][i];
-            const float x = see[nb][i] ? pr[nb][i] * q4_scale(m) : 0.f;
-            y[k] = fmaf(pr[nb][i], see[nb][i] ? q4_centre(m) : 0.f, y[k]);
-            h[i] = (_Float16)x;
-            if constexpr (PARTS == 2) {
-              const _Float16 rest = (_Float16)(x - (float)h[i]);
-              h[i] = low ? rest : h[i];
-            } else {
-              y[k] = fmaf(-7.5f, (float)h[i], y[k]);
-            }
+          for (int i = 0; i < 4; ++i) y[k] = fmaf(pr[nb][i], q4_centre(vm[nb][k][i]), y[k]);
+          if constexpr (PARTS == 1) {
+            const h16x2 mid = {(__fp16)-7.5f, (__fp16)-7.5f};
+            y[k] = __builtin_amdgcn_fdot2(__builtin_bit_cast(h16x2, w[nb][k][0]), mid, y[k], false);
+            y[k] = __builtin_amdgcn_fdot2(__builtin_bit_cast(h16x2, w[nb][k][1]), mid, y[k], false);
           }
-          w[nb][k][0] = __builtin_bit_cast(uint32_t, f16x2{h[0], h[1]});
-          w[nb][k][1] = __builtin_bit_cast(uint32_t, f16x2{h[2], h[3]});
         }
       }
       q4_narrow_values<HD, PARTS, GP, LAST>(r, w, o, cnt, std::make_integer_sequence<int, PAGES / 2>());
