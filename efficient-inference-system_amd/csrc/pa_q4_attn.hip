@@ -1196,7 +1196,8 @@ static Q4Plan q4_plan(int io_dtype, int32_t batch, int32_t heads, int32_t kv_hea
   const int64_t target = (p.wide ? (head_dim == 64 ? 4 : 3) : 2) * (int64_t)pa_host::device_cu_count();
   const int64_t want = units <= 0 ? 1 : p.wide ? (target / units > 1 ? target / units : 1) : (target + units - 1) / units;
   int pages = (int)((max_pages + want - 1) / want);
-  const int least = p.wide ? 16 : 64;
+  // a second launch merges ranges: 64 pages (one batch or two per wavefront) are not worth it, 128 are
+  const int least = p.wide ? 16 : max_pages <= 64 ? 64 : 32;
   if (!p.wide && pages > 96) pages = 96;  // requests of very different lengths: ranges end together
   pages = pages < least ? least : pages;
   pages = (pages + 7) / 8 * 8;
