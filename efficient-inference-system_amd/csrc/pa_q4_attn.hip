@@ -79,12 +79,15 @@ __device__ __forceinline__ float q4_zero() {
   asm("" : "+v"(z));
   return z;
 }
-// Two products of a weight and a pair's scale as fp16: v_fma_mixlo_f16 and v_fma_mixhi_f16. (Told apart by
-// the empty asm, or the two become one vector of conversions and multiplications, five instructions.)
+// Two products of a weight and a pair's scale as fp16: v_fma_mixlo_f16 and v_fma_mixhi_f16. (The empty asm
+// keep the two apart, or they become a vector of conversions and multiplications, five instructions, and
+// the word whole, or its high half is formed again where it is used next.)
 __device__ __forceinline__ f16x2 q4_weights(float p0, uint32_t m0, float p1, uint32_t m1) {
   _Float16 lo = (_Float16)(p0 * q4_scale(m0));
   asm("" : "+v"(lo));
-  return f16x2{lo, (_Float16)(p1 * q4_scale(m1))};
+  uint32_t both = __builtin_bit_cast(uint32_t, f16x2{lo, (_Float16)(p1 * q4_scale(m1))});
+  asm("" : "+v"(both));
+  return __builtin_bit_cast(f16x2, both);
 }
 
 // Codes as the matrix cores take them. As fp16 subnormals (c 2^-24) they cost one AND, but the cores align
@@ -307,7 +310,7 @@ __device__ __forceinline__ void q4_step(const uint8_t* pg, Q4Wave<HD, PARTS>& w,
       }
   }
   float p[2][4];
-  f16x8 pw[G];
+  uint32_t pw[G][4];
   // weights and, per group, w = p s as fp16 (PARTS = 2: this column's part of it); again with another M where
   // one is too large (never more than once)
 #pragma unroll 1
@@ -339,8 +342,7 @@ __device__ __forceinline__ void q4_step(const uint8_t* pg, Q4Wave<HD, PARTS>& w,
           }
         }
         top = __builtin_elementwise_max(top, __builtin_bit_cast(s16x2, hi));
-        pw[k][e] = part[0];
-        pw[k][e + 1] = part[1];
+        pw[k][e / 2] = __builtin_bit_cast(uint32_t, part);
       }
     }
     const bool far = top[0] > kQ4LimitBits || top[1] > kQ4LimitBits || big > kQ4Limit / kQ4Floor;
@@ -376,18 +378,17 @@ __device__ __forceinline__ void q4_step(const uint8_t* pg, Q4Wave<HD, PARTS>& w,
 #pragma unroll
     for (int e = 0; e < 8; ++e) w.y[k] = fmaf(p[e >> 2][e & 3], q4_centre(vm[e >> 2][k][e & 3]), w.y[k]);
     if constexpr (PARTS == 1) {  // -7.5 w, as rounded
-      const f16x2 mid = {(_Float16)-7.5f, (_Float16)-7.5f};
+      const h16x2 mid = {(__fp16)-7.5f, (__fp16)-7.5f};
 #pragma unroll
-      for (int e = 0; e < 8; e += 2)
-        w.y[k] = __builtin_amdgcn_fdot2(__builtin_bit_cast(h16x2, f16x2{pw[k][e], pw[k][e + 1]}),
-                                        __builtin_bit_cast(h16x2, mid), w.y[k], false);
+      for (int e = 0; e < 4; ++e) w.y[k] = __builtin_amdgcn_fdot2(__builtin_bit_cast(h16x2, pw[k][e]), mid, w.y[k], false);
     }
   }
   uint32_t vw[2][2 * G];
 #pragma unroll
   for (int h = 0; h < 2; ++h) P::v_words(pg + h * P::BYTES, lane, vw[h]);
 #pragma unroll
-  for (int k = 0; k < G; ++k)
+  for (int k = 0; k < G; ++k) {
+    const f16x8 b = q4_operand(pw[k][0], pw[k][1], pw[k][2], pw[k][3]);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       uint32_t x[4];
@@ -396,8 +397,9 @@ __device__ __forceinline__ void q4_step(const uint8_t* pg, Q4Wave<HD, PARTS>& w,
         const uint32_t x0 = vw[e >> 1][(e & 1) * G + k], x1 = t & 2 ? x0 >> 8 : x0;
         x[e] = t & 1 ? q4_pair<PARTS, true>(x1) : q4_pair<PARTS, false>(x1);
       }
-      w.o[k][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q4_operand(x[0], x[1], x[2], x[3]), pw[k], w.o[k][t], 0, 0, 0);
+      w.o[k][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q4_operand(x[0], x[1], x[2], x[3]), b, w.o[k][t], 0, 0, 0);
     }
+  }
 }
 
 // A tile's walk is done: the lanes' sums joined. Leaves in lane (g, c) the 16 values d = 64 k + 16 g ..
@@ -475,6 +477,20 @@ constexpr int kQ4WideWaves = 4;
 constexpr int kQ4StagePages = kQ4WideWaves, kQ4Ring = 3;
 constexpr uint32_t kQ4StageMask = (1u << kQ4StagePages) - 1;
 
+// The request whose place in the order of falling cached lengths is `place` (equal lengths in the batch's
+// order), for batches of up to 64: the longest requests' tiles start first, so that the grid's end is filled
+// with short ones.
+__device__ __forceinline__ int q4_by_length(const int32_t* lens, int B, int place, int lane) {
+  if (B > 64) return place;
+  const int mine = lane < B ? lens[lane] : -0x7fffffff;
+  int before = 0;
+  for (int j = 0; j < B; ++j) {
+    const int other = __builtin_amdgcn_readlane(mine, j);
+    before += other > mine || (other == mine && j < lane);
+  }
+  return __builtin_ctzll(__ballot(lane < B && before == place));
+}
+
 template <typename IO, int HD, int PARTS>
 __global__ __launch_bounds__(64 * kQ4WideWaves, 3) void q4_wide_kernel(const Q4Args a) {
   using P = Q4Staged<HD>;
@@ -485,7 +501,8 @@ __global__ __launch_bounds__(64 * kQ4WideWaves, 3) void q4_wide_kernel(const Q4A
   __shared__ __attribute__((aligned(16))) uint8_t ring[kQ4Ring * STAGE];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int g = lane >> 4, c = lane & 15;
-  const Q4Unit u = q4_unit(a);
+  Q4Unit u = q4_unit(a);
+  u.b = __builtin_amdgcn_readfirstlane(q4_by_length(a.seq_lens, a.B, u.b, lane));
   const int L = a.seq_lens[u.b], C = a.cur_lens[u.b];
   const int rows = a.T * a.group;
   int keys = L < a.max_pages * kQ4Tokens ? L : a.max_pages * kQ4Tokens;
