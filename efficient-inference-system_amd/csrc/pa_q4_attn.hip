@@ -1024,9 +1024,11 @@ __device__ __forceinline__ void q4_row_state(const float* rec, int splits, int l
 
 // Records of the splits -> outputs and, for decode totals, the keys' weights from the scores that the first
 // kernel left in the workspace. The first `merges` workgroups merge, one wavefront per row; of the others each
-// adds 256 keys' weights of one KV head, having formed its rows' denominators from the records by itself (a
+// adds kQ4FinishKeys keys' weights of one KV head, having formed its rows' denominators from the records by itself (a
 // launch less than in two steps). A block that two rows of the page table share is added to by both, hence
 // the atomic; otherwise each slot gets one addition.
+constexpr int kQ4FinishKeys = 1024;  // (256, a key per thread, repeated the denominators too often: 34 -> 20 us)
+
 template <typename IO, int HD>
 __global__ __launch_bounds__(256) void q4_finish_kernel(const Q4Args a, int64_t total, int merges, int chunks) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -1060,14 +1062,14 @@ __global__ __launch_bounds__(256) void q4_finish_kernel(const Q4Args a, int64_t 
   }
   __shared__ float lse[kQ4MaxNarrow];
   int x = (int)blockIdx.x - merges;
-  const int chunk = x % chunks;
-  x /= chunks;
-  const int hk = x % a.Hk, b = x / a.Hk;
+  const int hk = x % a.Hk;
+  x /= a.Hk;
+  const int chunk = x % chunks, b = x / chunks;
   const int L = a.seq_lens[b], C = a.cur_lens[b];
   int n = valid_keys(L, C, 0);
   n = n < a.max_pages * kQ4Tokens ? n : a.max_pages * kQ4Tokens;
-  const int t = chunk * 256 + threadIdx.x;
-  if (chunk * 256 >= n || C < 1) return;
+  const int t0 = chunk * kQ4FinishKeys;
+  if (t0 >= n || C < 1) return;
   if (a.splits > 1) {
     const int splits = q4_splits_of(a, b, 0);
     for (int j = wave; j < a.group; j += 4) {
@@ -1079,14 +1081,16 @@ __global__ __launch_bounds__(256) void q4_finish_kernel(const Q4Args a, int64_t 
     lse[threadIdx.x] = *q4_lse(a, b, hk, threadIdx.x);
   }
   __syncthreads();
-  if (t >= n) return;
-  const int id = q4_block(a.page_table[(int64_t)b * a.pt_stride + t / kQ4Tokens], a.num_blocks);
-  if (id < 0) return;
-  float sum = 0.f;
-  const float* mine = a.scores + ((int64_t)b * a.H + hk * a.group) * a.score_stride + t;
+  const float* mine = a.scores + ((int64_t)b * a.H + hk * a.group) * a.score_stride;
+  const int t1 = t0 + kQ4FinishKeys < n ? t0 + kQ4FinishKeys : n;
 #pragma unroll 4
-  for (int j = 0; j < a.group; ++j) sum += fast_exp2(mine[j * a.score_stride] - lse[j]);
-  atomicAdd(a.weights + ((int64_t)id * a.Hk + hk) * kQ4Tokens + (t & (kQ4Tokens - 1)), sum);
+  for (int t = t0 + threadIdx.x; t < t1; t += 256) {
+    const int id = q4_block(a.page_table[(int64_t)b * a.pt_stride + t / kQ4Tokens], a.num_blocks);
+    float sum = 0.f;
+#pragma unroll 4
+    for (int j = 0; j < a.group; ++j) sum += fast_exp2(mine[j * a.score_stride + t] - lse[j]);
+    if (id >= 0) atomicAdd(a.weights + ((int64_t)id * a.Hk + hk) * kQ4Tokens + (t & (kQ4Tokens - 1)), sum);
+  }
 }
 
 // Totals of a chunk: the scores formed again, four pages (64 keys) per workgroup whose operands and pairs stay
@@ -1251,7 +1255,7 @@ static void launch_q4(const Q4Args& a, const Q4Plan& p, hipStream_t stream) {
   const bool totals = a.scores != nullptr && !(p.splits == 1 && p.tiles == 1);
   if (p.splits > 1 || totals) {
     const int64_t total = (int64_t)a.B * a.Hk * a.T * a.group;
-    const int merges = p.splits > 1 ? (int)((total + 3) / 4) : 0, chunks = (a.max_pages * kQ4Tokens + 255) / 256;
+    const int merges = p.splits > 1 ? (int)((total + 3) / 4) : 0, chunks = (a.max_pages * kQ4Tokens + kQ4FinishKeys - 1) / kQ4FinishKeys;
     const int64_t wgs = merges + (totals ? (int64_t)chunks * a.Hk * a.B : 0);
     q4_finish_kernel<IO, HD><<<(unsigned)wgs, 256, 0, stream>>>(a, total, merges, chunks);
   }
