@@ -15,8 +15,39 @@ struct Q4RowArgs {
   int32_t B, H, T;
 };
 
+// The row of a lane, HD / 8 lanes a row. CHUNK (calls of 16 tokens and more): a workgroup takes 256 / (HD / 8)
+// consecutive tokens of one head, K and V, so that the row's place is scalar arithmetic but for the token,
+// and a page, whose bytes interleave its tokens, is written by one workgroup or two. Otherwise (decode steps)
+// rows follow each other, and K and V are the halves of the grid's y axis. With the second order for chunks too the
+// index arithmetic, divisions in every lane, took as long as the quantisation.
+struct Q4Row {
+  int h, e;        // head, and which eight values
+  uint32_t b, j;   // request and token; j >= T: no row
+};
+template <int HD, bool CHUNK>
+__device__ __forceinline__ Q4Row q4_row_of(int H, int T) {
+  constexpr uint32_t LPR = HD / 8, TOKENS = 256 / LPR;
+  Q4Row r;
+  r.e = (int)(threadIdx.x % LPR);
+  if constexpr (CHUNK) {
+    uint32_t x = blockIdx.x;
+    r.h = (int)(x % (uint32_t)H);
+    x /= (uint32_t)H;
+    const uint32_t groups = ((uint32_t)T + TOKENS - 1) / TOKENS;
+    r.b = x / groups;
+    r.j = (x - r.b * groups) * TOKENS + threadIdx.x / LPR;
+  } else {
+    uint32_t x = (blockIdx.x * 256u + threadIdx.x) / LPR;
+    r.h = (int)(x % (uint32_t)H);
+    x /= (uint32_t)H;
+    r.b = x / (uint32_t)T;
+    r.j = x - r.b * (uint32_t)T;
+  }
+  return r;
+}
+
 // Eight lanes share a group of 64 values, lane i of them values 8 i .. 8 i + 7: the eight of one K
-// word, and two n-quadruples of V. K and V are the two halves of the grid's y axis.
+// word, and two n-quadruples of V.
 template <int HD>
 __device__ __forceinline__ void q4_row_place(int h, int H, int64_t blk, int tok, int e, uint32_t& kw, uint32_t& vw,
                                              uint32_t& meta, int64_t& page) {
@@ -47,18 +78,27 @@ __device__ __forceinline__ void q4_load8(const T* p, bool vec, float (&x)[8]) {
   }
 }
 
-// The code of x: (x - z) / s + 7.5 to the nearest, ties to even, in 0..15. Where the quotient is below 16
-// its fp32 value is within 2e-6 of the real one (8 x 3 roundings of 2^-24, and one of the sum), so it
-// decides unless it lies within 4e-6 of a border between two codes; there (about one value in 10^5) the
-// fp64 one does. Larger quotients are clamped whatever their error.
-__device__ __forceinline__ int q4_code(float x, float z, float s, float rs) {
-  const float y = (x - z) * rs + 7.5f;
-  const float n = rintf(y);
-  if (__builtin_expect(!(fabsf(fabsf(y - n) - 0.5f) > 4e-6f), 0)) {
-    const double d = ((double)x - (double)z) / (double)s + 7.5;
-    return (int)fmin(fmax(rint(d), 0.0), 15.0);
+// The codes of a lane's eight values: (x - z) / s + 7.5 to the nearest, ties to even, in 0..15. Where the
+// quotient is below 16 its fp32 value is within 2e-6 of the real one (8 x 2^-24 of the difference, 8 x 2^-23
+// of the reciprocal, 2^-21 of the sum), so it decides unless it lies within 4e-6 of a border between two codes; there (about one value
+// in 10^5, one check for the eight) the fp64 one does. Larger quotients are clamped whatever their error.
+__device__ __forceinline__ void q4_codes(const float (&x)[8], float z, float s, uint32_t (&c)[8]) {
+  const float rs = __builtin_amdgcn_rcpf(s);
+  float y[8], far = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    y[i] = fmaf(x[i] - z, rs, 7.5f);
+    const float n = rintf(y[i]);
+    far = fmaxf(far, fabsf(y[i] - n));
+    c[i] = (uint32_t)(int)__builtin_amdgcn_fmed3f(n, 0.f, 15.f);
   }
-  return (int)fminf(fmaxf(n, 0.f), 15.f);
+  if (__builtin_expect(far > 0.5f - 4e-6f, 0)) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const double d = ((double)x[i] - (double)z) / (double)s + 7.5;
+      c[i] = (uint32_t)(int)fmin(fmax(rint(d), 0.0), 15.0);
+    }
+  }
 }
 
 // Scale and centre of a group. The products round to fp32 before they round to halves: left to itself the
@@ -71,36 +111,23 @@ __device__ __forceinline__ void q4_pair_of(float hi, float lo, _Float16& s, _Flo
   z = (_Float16)zf;
 }
 
-// Quantising append: per (row, head, group) s = half((hi - lo) / 15), z = half((hi + lo) / 2) of the values
-// clamped to half's range, then the codes. Bound by HBM for long chunks (a row is read once, written
-// as 4.5 bits a value) and by latency for decode steps.
-template <typename T, int HD>
-__global__ __launch_bounds__(256) void q4_append_kernel(const Q4RowArgs a, uint32_t total, int vec) {
-  constexpr int LPR = HD / 8;  // lanes per row
-  const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
-  if (idx >= total) return;  // (whole rows: 8 or 16 lanes each)
-  const bool is_v = blockIdx.y != 0;
-  const uint32_t rh = idx / LPR;
-  const int e = (int)(idx % LPR);
-  const uint32_t row = rh / (uint32_t)a.H;  // b * T + j
-  const int h = (int)(rh - row * (uint32_t)a.H);
-  const uint32_t b = row / (uint32_t)a.T, j = row - b * (uint32_t)a.T;
-  const int32_t slot = a.slots[row];
-  float x[8];
-  const T* src = static_cast<const T*>(is_v ? a.v_new : a.k_new) + (int64_t)b * a.sb + (int64_t)h * a.sh +
-                 (int64_t)j * a.st + 8 * e;
-  q4_load8(src, vec, x);
-  if (slot < 0) return;
-  const int64_t blk = (uint32_t)slot / kQ4Tokens;
-  if (blk >= a.num_blocks) return;
-  const int tok = slot & (kQ4Tokens - 1);
-
-  bool nan = false;
+// One row's eight values of K or V into its slot: per group s = half((hi - lo) / 15), z = half((hi + lo) / 2) of
+// the values clamped to half's range, then the codes.
+template <int HD>
+__device__ __forceinline__ void q4_put(uint8_t* p, float (&x)[8], bool is_v, int e, uint32_t kw, uint32_t vw, uint32_t meta) {
+  float odd = 0.f;  // NaN where a value is NaN (or infinite)
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    nan |= x[i] != x[i];
-    x[i] = fminf(fmaxf(x[i], -65504.f), 65504.f);
+  for (int i = 0; i < 8; ++i) odd = fmaf(x[i], 0.f, odd);
+  bool nan = false;
+  if (__builtin_expect(odd != odd, 0)) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      nan |= x[i] != x[i];
+      x[i] = x[i] != x[i] ? 0.f : x[i];
+    }
   }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = __builtin_amdgcn_fmed3f(x[i], -65504.f, 65504.f);
   float hi = x[0], lo = x[0];
 #pragma unroll
   for (int i = 1; i < 8; ++i) {
@@ -112,15 +139,14 @@ __global__ __launch_bounds__(256) void q4_append_kernel(const Q4RowArgs a, uint3
   _Float16 sh, zh;
   q4_pair_of(hi, lo, sh, zh);
   const bool bad = hi == INFINITY;
-  const float s = (float)sh, z = (float)zh, rs = 1.f / s;
+  const float s = (float)sh, z = (float)zh;
   uint32_t c[8];
+  if (bad || !(s > 0.f)) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) c[i] = bad || !(s > 0.f) ? 0u : (uint32_t)q4_code(x[i], z, s, rs);
-
-  uint32_t kw, vw, meta;
-  int64_t page;
-  q4_row_place<HD>(h, a.H, blk, tok, e, kw, vw, meta, page);
-  uint8_t* p = (is_v ? a.v_pool : a.k_pool) + page;
+    for (int i = 0; i < 8; ++i) c[i] = 0;
+  } else {
+    q4_codes(x, z, s, c);
+  }
   if (!is_v) {
     *reinterpret_cast<uint32_t*>(p + kw) = c[0] | c[2] << 4 | c[4] << 8 | c[6] << 12 | c[1] << 16 | c[3] << 20 |
                                            c[5] << 24 | c[7] << 28;
@@ -135,29 +161,39 @@ __global__ __launch_bounds__(256) void q4_append_kernel(const Q4RowArgs a, uint3
     zu = zu == 0x8000u ? 0u : zu;  // a centre of zero is +0, whatever zeros the row holds
     *reinterpret_cast<uint32_t*>(p + meta) = su | zu << 16;
   }
-  if (!is_v && e == 0 && a.weights != nullptr) a.weights[(blk * a.H + h) * kQ4Tokens + tok] = 0.f;
 }
 
-// The values that slots stand for, z + s (c - 7.5) rounded once to T; rows without a slot are zeros.
-template <typename T, int HD>
-__global__ __launch_bounds__(256) void q4_read_kernel(const Q4RowArgs a, uint32_t total) {
-  constexpr int LPR = HD / 8;
-  const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
-  if (idx >= total) return;
-  const bool is_v = blockIdx.y != 0;
-  const uint32_t rh = idx / LPR;
-  const int e = (int)(idx % LPR);
-  const uint32_t row = rh / (uint32_t)a.H;
-  const int h = (int)(rh - row * (uint32_t)a.H);
-  const uint32_t b = row / (uint32_t)a.T, j = row - b * (uint32_t)a.T;
-  const int32_t slot = a.slots[row];
+// Quantising append. Bound by HBM for long chunks (a row is read once, written as 4.5 bits a value) and by
+// latency for decode steps.
+template <typename T, int HD, bool CHUNK>
+__global__ __launch_bounds__(256) void q4_append_kernel(const Q4RowArgs a, uint32_t total, int vec) {
+  if (!CHUNK && blockIdx.x * 256u + threadIdx.x >= total) return;  // (whole rows: 8 or 16 lanes each)
+  const Q4Row at = q4_row_of<HD, CHUNK>(a.H, a.T);
+  if (CHUNK && at.j >= (uint32_t)a.T) return;
+  const int h = at.h, e = at.e;
+  const int32_t slot = a.slots[at.b * (uint32_t)a.T + at.j];
+  const int64_t src = (int64_t)at.b * a.sb + (int64_t)h * a.sh + (int64_t)at.j * a.st + 8 * e;
+  const bool first_v = !CHUNK && blockIdx.y != 0;
+  float x[2][8];
+  q4_load8(static_cast<const T*>(first_v ? a.v_new : a.k_new) + src, vec, x[0]);
+  if constexpr (CHUNK) q4_load8(static_cast<const T*>(a.v_new) + src, vec, x[1]);
+  if (slot < 0) return;
   const int64_t blk = (uint32_t)slot / kQ4Tokens;
+  if (blk >= a.num_blocks) return;
+  const int tok = slot & (kQ4Tokens - 1);
+  uint32_t kw, vw, meta;
+  int64_t page;
+  q4_row_place<HD>(h, a.H, blk, tok, e, kw, vw, meta, page);
+  q4_put<HD>((first_v ? a.v_pool : a.k_pool) + page, x[0], first_v, e, kw, vw, meta);
+  if constexpr (CHUNK) q4_put<HD>(a.v_pool + page, x[1], true, e, kw, vw, meta);
+  if (!first_v && e == 0 && a.weights != nullptr) a.weights[(blk * a.H + h) * kQ4Tokens + tok] = 0.f;
+}
+
+// One row's eight values of K or V, z + s (c - 7.5) rounded once to T.
+template <typename T, int HD>
+__device__ __forceinline__ void q4_get(const uint8_t* p, T* out, bool there, bool is_v, uint32_t kw, uint32_t vw, uint32_t meta) {
   float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (slot >= 0 && blk < a.num_blocks) {
-    uint32_t kw, vw, meta;
-    int64_t page;
-    q4_row_place<HD>(h, a.H, blk, slot & (kQ4Tokens - 1), e, kw, vw, meta, page);
-    const uint8_t* p = (is_v ? a.v_pool : a.k_pool) + page;
+  if (there) {
     uint32_t c;  // nibble i: value i
     if (!is_v) {
       const uint32_t w = *reinterpret_cast<const uint32_t*>(p + kw);
@@ -174,8 +210,6 @@ __global__ __launch_bounds__(256) void q4_read_kernel(const Q4RowArgs a, uint32_
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = fmaf(s, (float)(c >> (4 * i) & 15u) - 7.5f, z);
   }
-  T* out = static_cast<T*>(const_cast<void*>(is_v ? a.v_new : a.k_new)) + (int64_t)b * a.sb + (int64_t)h * a.sh +
-           (int64_t)j * a.st + 8 * e;
   if constexpr (sizeof(T) == 4) {
     reinterpret_cast<f32x4*>(out)[0] = f32x4{x[0], x[1], x[2], x[3]};
     reinterpret_cast<f32x4*>(out)[1] = f32x4{x[4], x[5], x[6], x[7]};
@@ -187,24 +221,48 @@ __global__ __launch_bounds__(256) void q4_read_kernel(const Q4RowArgs a, uint32_
   }
 }
 
-template <int HD>
-static void launch_append(const Q4RowArgs& a, int dtype, int vec, hipStream_t stream) {
-  const uint32_t total = (uint32_t)((int64_t)a.B * a.T * a.H * (HD / 8));
-  const dim3 grid((total + 255) / 256, 2);
-  if (dtype == PA_DTYPE_F32)
-    q4_append_kernel<float, HD><<<grid, 256, 0, stream>>>(a, total, vec);
-  else
-    q4_append_kernel<uint16_t, HD><<<grid, 256, 0, stream>>>(a, total, vec);
+// The values that slots stand for; rows without a slot are zeros.
+template <typename T, int HD, bool CHUNK>
+__global__ __launch_bounds__(256) void q4_read_kernel(const Q4RowArgs a, uint32_t total) {
+  if (!CHUNK && blockIdx.x * 256u + threadIdx.x >= total) return;
+  const Q4Row at = q4_row_of<HD, CHUNK>(a.H, a.T);
+  if (CHUNK && at.j >= (uint32_t)a.T) return;
+  const int32_t slot = a.slots[at.b * (uint32_t)a.T + at.j];
+  const int64_t blk = (uint32_t)slot / kQ4Tokens;
+  const bool there = slot >= 0 && blk < a.num_blocks;
+  uint32_t kw, vw, meta;
+  int64_t page;
+  q4_row_place<HD>(at.h, a.H, there ? blk : 0, slot & (kQ4Tokens - 1), at.e, kw, vw, meta, page);
+  const int64_t dst = (int64_t)at.b * a.sb + (int64_t)at.h * a.sh + (int64_t)at.j * a.st + 8 * at.e;
+  const bool first_v = !CHUNK && blockIdx.y != 0;
+  q4_get<T, HD>((first_v ? a.v_pool : a.k_pool) + page, static_cast<T*>(const_cast<void*>(first_v ? a.v_new : a.k_new)) + dst,
+                there, first_v, kw, vw, meta);
+  if constexpr (CHUNK) q4_get<T, HD>(a.v_pool + page, static_cast<T*>(const_cast<void*>(a.v_new)) + dst, there, true, kw, vw, meta);
 }
 
-template <int HD>
-static void launch_read(const Q4RowArgs& a, int dtype, hipStream_t stream) {
-  const uint32_t total = (uint32_t)((int64_t)a.B * a.T * a.H * (HD / 8));
-  const dim3 grid((total + 255) / 256, 2);
-  if (dtype == PA_DTYPE_F32)
-    q4_read_kernel<float, HD><<<grid, 256, 0, stream>>>(a, total);
+// Workgroups of a call in either order.
+constexpr int kChunkTokens = 16;
+static int64_t row_workgroups(int32_t B, int32_t T, int32_t H, int32_t HD) {
+  const int per = 256 / (HD / 8);  // rows of a workgroup
+  return T >= kChunkTokens ? (int64_t)B * ((T + per - 1) / per) * H : ((int64_t)B * T * H + per - 1) / per;
+}
+
+template <typename T, int HD>
+static void launch_append(const Q4RowArgs& a, int vec, hipStream_t stream) {
+  const unsigned n = (unsigned)row_workgroups(a.B, a.T, a.H, HD);
+  if (a.T >= kChunkTokens)
+    q4_append_kernel<T, HD, true><<<n, 256, 0, stream>>>(a, 0, vec);
   else
-    q4_read_kernel<uint16_t, HD><<<grid, 256, 0, stream>>>(a, total);
+    q4_append_kernel<T, HD, false><<<dim3(n, 2), 256, 0, stream>>>(a, (uint32_t)((int64_t)a.B * a.T * a.H * (HD / 8)), vec);
+}
+
+template <typename T, int HD>
+static void launch_read(const Q4RowArgs& a, hipStream_t stream) {
+  const unsigned n = (unsigned)row_workgroups(a.B, a.T, a.H, HD);
+  if (a.T >= kChunkTokens)
+    q4_read_kernel<T, HD, true><<<n, 256, 0, stream>>>(a, 0);
+  else
+    q4_read_kernel<T, HD, false><<<dim3(n, 2), 256, 0, stream>>>(a, (uint32_t)((int64_t)a.B * a.T * a.H * (HD / 8)));
 }
 
 static int check_rows(const char* what, const void* k, const void* v, int dtype, const void* k_pool, const void* v_pool,
@@ -220,7 +278,7 @@ static int check_rows(const char* what, const void* k, const void* v, int dtype,
   PA_CHECK_ARG(num_blocks == 0 || (k_pool && v_pool), "%s: null pool", what);
   PA_CHECK_ARG(((reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(v_pool)) & 15) == 0,
                "%s: the pools must be 16-byte aligned", what);
-  PA_CHECK_ARG((int64_t)batch * rows * heads * (head_dim / 8) <= 0x7fffff00LL, "%s: too many rows in one call", what);
+  PA_CHECK_ARG((int64_t)batch * rows <= 0x7fffffffLL && row_workgroups(batch, rows, heads, head_dim) <= 0x7fffff00LL / 256, "%s: too many rows in one call", what);
   return PA_OK;
 }
 
@@ -247,10 +305,11 @@ extern "C" int pa_q4_append(const void* k_new, const void* v_new, int64_t new_st
   const int64_t per = new_dtype == PA_DTYPE_F32 ? 4 : 8;  // elements of 16 bytes
   const int vec = ((reinterpret_cast<uintptr_t>(k_new) | reinterpret_cast<uintptr_t>(v_new)) & 15) == 0 &&
                   new_stride_b % per == 0 && new_stride_h % per == 0 && new_stride_t % per == 0;
-  if (head_dim == 64)
-    launch_append<64>(a, new_dtype, vec, static_cast<hipStream_t>(stream));
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (new_dtype == PA_DTYPE_F32)
+    head_dim == 64 ? launch_append<float, 64>(a, vec, st) : launch_append<float, 128>(a, vec, st);
   else
-    launch_append<128>(a, new_dtype, vec, static_cast<hipStream_t>(stream));
+    head_dim == 64 ? launch_append<uint16_t, 64>(a, vec, st) : launch_append<uint16_t, 128>(a, vec, st);
   PA_CHECK_LAUNCH("pa_q4_append");
   return PA_OK;
 }
@@ -271,10 +330,11 @@ extern "C" int pa_q4_read(const void* k_pool, const void* v_pool, int64_t num_bl
                "pa_q4_read: the outputs must start, and their rows follow each other, at multiples of 16 bytes");
   Q4RowArgs a{k_out, v_out, out_stride_b, out_stride_h, out_stride_t, static_cast<uint8_t*>(const_cast<void*>(k_pool)),
               static_cast<uint8_t*>(const_cast<void*>(v_pool)), nullptr, num_blocks, slot_mapping, batch, kv_heads, query_len};
-  if (head_dim == 64)
-    launch_read<64>(a, out_dtype, static_cast<hipStream_t>(stream));
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (out_dtype == PA_DTYPE_F32)
+    head_dim == 64 ? launch_read<float, 64>(a, st) : launch_read<float, 128>(a, st);
   else
-    launch_read<128>(a, out_dtype, static_cast<hipStream_t>(stream));
+    head_dim == 64 ? launch_read<uint16_t, 64>(a, st) : launch_read<uint16_t, 128>(a, st);
   PA_CHECK_LAUNCH("pa_q4_read");
   return PA_OK;
 }
