@@ -473,9 +473,14 @@ constexpr int kQ4MaxNarrow = 32;  // rows that the narrow kernel takes (two tile
 // go from the pools straight into LDS (global_load_lds, one page per wavefront), two stages ahead in a ring
 // of three, with one barrier a stage. Read from memory by each wavefront for itself, the pages' pairs alone
 // (16 bytes that 16 lanes share) cost more load instructions than the codes.
-constexpr int kQ4WideWaves = 4;
-constexpr int kQ4StagePages = kQ4WideWaves, kQ4Ring = 3;
-constexpr uint32_t kQ4StageMask = (1u << kQ4StagePages) - 1;
+//
+// HALVES = 2, for grids that leave the GPU room: eight wavefronts for the same four tiles, stages of 128 keys,
+// each half of the wavefronts taking its half of every stage, joined in LDS at the end. A step is a chain of
+// LDS reads, matrix instructions and exponentials that one wavefront a SIMD does not fill (4 x 256 rows of 8
+// heads x 64 over up to 512 keys, fp32: 26 -> 21.5 us; the same keys split over workgroups instead cost a
+// merging launch, 31 us).
+constexpr int kQ4WideWaves = 4;  // column tiles of a workgroup
+constexpr int kQ4Ring = 3;
 
 // The request whose place in the order of falling cached lengths is `place` (equal lengths in the batch's
 // order), for batches of up to 64: the longest requests' tiles start first, so that the grid's end is filled
@@ -491,15 +496,19 @@ __device__ __forceinline__ int q4_by_length(const int32_t* lens, int B, int plac
   return __builtin_ctzll(__ballot(lane < B && before == place));
 }
 
-template <typename IO, int HD, int PARTS>
-__global__ __launch_bounds__(64 * kQ4WideWaves, 3) void q4_wide_kernel(const Q4Args a) {
+template <typename IO, int HD, int PARTS, int HALVES>
+__global__ __launch_bounds__(64 * kQ4WideWaves * HALVES, HALVES == 2 ? 2 : 3) void q4_wide_kernel(const Q4Args a) {
   using P = Q4Staged<HD>;
   constexpr int G = HD / kQ4Group, PB = q4_page_bytes(HD);
   constexpr int ROWS = 16 / PARTS;  // rows of a column tile
-  constexpr int STAGE = kQ4StagePages * P::BYTES;
+  constexpr int SP = kQ4WideWaves * HALVES;  // pages of a stage
+  constexpr uint32_t SPMASK = (1u << SP) - 1;
+  constexpr int STAGE = SP * P::BYTES;
+  constexpr int JOIN = HALVES == 2 ? kQ4WideWaves * 64 * (16 * G + 2) * 4 : 0;  // the second half's sums
   constexpr int LOADS = HD == 128 ? 3 : 2;  // load instructions of a page
-  __shared__ __attribute__((aligned(16))) uint8_t ring[kQ4Ring * STAGE];
+  __shared__ __attribute__((aligned(16))) uint8_t ring[kQ4Ring * STAGE > JOIN ? kQ4Ring * STAGE : JOIN];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int half = wave / kQ4WideWaves, tile_wave = wave % kQ4WideWaves;
   const int g = lane >> 4, c = lane & 15;
   Q4Unit u = q4_unit(a);
   u.b = __builtin_amdgcn_readfirstlane(q4_by_length(a.seq_lens, a.B, u.b, lane));
@@ -520,13 +529,13 @@ __global__ __launch_bounds__(64 * kQ4WideWaves, 3) void q4_wide_kernel(const Q4A
   p1 = p1 < pages ? p1 : pages;
   if (a.splits > 1 && p0 >= p1) return;  // no record: the merge knows how far each row's pages reach
   // what the wavefront's rows see: all of them, some of them
-  const int first = wg_first + wave * ROWS;
+  const int first = wg_first + tile_wave * ROWS;
   const int end = first + ROWS < rows ? first + ROWS : rows;
   const int all = first < rows ? seen(first) : 0, most = first < rows ? seen(end - 1) : 0;
   Q4Wave<HD, PARTS> w;
   const int tile = first / ROWS;
   q4_setup<IO, HD, PARTS>(a, u.b, u.hk, tile, L, C, keys, lane, w);
-  if (a.q_ops != nullptr && u.split == 0) {  // for q4_chunk_weights_kernel
+  if (a.q_ops != nullptr && u.split == 0 && half == 0) {  // for q4_chunk_weights_kernel
     const int64_t at = ((int64_t)u.b * a.Hk + u.hk) * a.op_tiles + tile;
 #pragma unroll
     for (int s = 0; s < HD / 32; ++s) a.q_ops[(at * (HD / 32) + s) * 64 + lane] = w.q[s];
@@ -544,17 +553,17 @@ __global__ __launch_bounds__(64 * kQ4WideWaves, 3) void q4_wide_kernel(const Q4A
     const uint8_t* meta_src = (lane & (4 * G) ? vb : kb) + q4_codes_bytes(HD) + (lane & (4 * G - 1)) * 16;
     const uint8_t* code_src = (lane < 32 ? kb : vb) + (lane & 31) * 16;
     const uint32_t k_off = (uint32_t)(c * 4 + g) * 16, v_off = (uint32_t)lane * 16;
-    const int stages = (p1 - p0 + kQ4StagePages - 1) / kQ4StagePages;
-    uint32_t live = 0;  // pages of the ring's stages that are there, kQ4StagePages bits a slot
+    const int stages = (p1 - p0 + SP - 1) / SP;
+    uint32_t live = 0;  // pages of the ring's stages that are there, SP bits a slot
     auto issue = [&](int st, int slot) {
-      const int pg = p0 + st * kQ4StagePages;
+      const int pg = p0 + st * SP;
       if (pg - base >= 64) {
         base = pg;
         ids = pg + lane < p1 ? q4_block(table[pg + lane], a.num_blocks) : -1;
         there = __ballot(ids >= 0);
       }
-      live = (live & ~(kQ4StageMask << kQ4StagePages * slot)) |
-             ((uint32_t)(there >> (pg - base)) & kQ4StageMask) << kQ4StagePages * slot;
+      live = (live & ~(SPMASK << SP * slot)) |
+             ((uint32_t)(there >> (pg - base)) & SPMASK) << SP * slot;
       const int mine = __builtin_amdgcn_readlane(ids, pg - base + wave);
       const int64_t off = (int64_t)(mine >= 0 ? mine : 0) * step;  // (pages that are not there: block 0's bytes, unseen)
       uint8_t* dst = ring + slot * STAGE + wave * P::BYTES;
@@ -568,9 +577,9 @@ __global__ __launch_bounds__(64 * kQ4WideWaves, 3) void q4_wide_kernel(const Q4A
     };
     auto compute = [&](int st, int slot) {
 #pragma unroll 1
-      for (int h = 0; h < kQ4StagePages; h += 2) {
-        const int key0 = (p0 + st * kQ4StagePages + h) * kQ4Tokens;
-        const int bits = (int)(live >> (kQ4StagePages * slot + h)) & 3;
+      for (int h = half * kQ4WideWaves; h < (half + 1) * kQ4WideWaves; h += 2) {
+        const int key0 = (p0 + st * SP + h) * kQ4Tokens;
+        const int bits = (int)(live >> (SP * slot + h)) & 3;
         const uint8_t* pg = ring + slot * STAGE + h * P::BYTES;
         if (key0 >= most || bits == 0) continue;
         q4_step<HD, PARTS>(pg, w, key0, bits != 3 || key0 + 32 > all, bits, lane);
@@ -591,6 +600,27 @@ __global__ __launch_bounds__(64 * kQ4WideWaves, 3) void q4_wide_kernel(const Q4A
   const int row = q4_row<PARTS>(tile, c);
   float o[G][16], l;
   q4_join<HD, PARTS>(w, o, l);
+  if constexpr (HALVES == 2) {
+    __syncthreads();  // every wavefront has read its last stage
+    float* mine = reinterpret_cast<float*>(ring) + (tile_wave * 64 + lane) * (16 * G + 2);
+    if (half == 1) {
+      mine[0] = w.M;
+      mine[1] = l;
+#pragma unroll
+      for (int k = 0; k < G; ++k)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mine[2 + 16 * k + i] = o[k][i];
+    }
+    __syncthreads();
+    if (half == 1) return;
+    const float M = fmaxf(w.M, mine[0]), f0 = fast_exp2(w.M - M), f1 = fast_exp2(mine[0] - M);
+    w.M = M;
+    l = fmaf(f0, l, f1 * mine[1]);
+#pragma unroll
+    for (int k = 0; k < G; ++k)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[k][i] = fmaf(f0, o[k][i], f1 * mine[2 + 16 * k + i]);
+  }
   if (row >= rows || c >= ROWS) return;
   if (a.splits > 1) {
     float* rec = q4_record<HD>(a, u.b, u.hk, row, u.split);
@@ -620,7 +650,7 @@ __global__ __launch_bounds__(64 * kQ4WideWaves, 3) void q4_wide_kernel(const Q4A
 // through together: page t's scores are kept by the lanes of columns GP t' .. (t' = t % PG, PG = columns / GP), where
 // softmax, scales and running sums then cost one page's work for PG pages. For the second product page t's
 // weights turn back to the first GP columns by a DPP rotation of the row; the other columns' sums are
-// never read. VALU work per key falls from about 7 to 3 instructions per lane at one row (head_dim 128).
+// never read.
 //
 // A batch's loads are all issued before its products, and K's registers are filled again while the second
 // product runs: 16 KB and more in flight per wavefront.
@@ -644,7 +674,7 @@ __device__ __forceinline__ float row_sum(float x) {
 template <int HD, int PARTS, int GP>
 struct Q4Batch {
   static constexpr int G = HD / kQ4Group, W = HD / 32;
-  // pages that share a softmax: 8 at most, which 190 registers hold at head_dim 128 (16 spill)
+  // pages that share a softmax: 8 at most, which 213 to 223 registers hold at head_dim 128 (16 spill)
   static constexpr int COLS = 16 / PARTS, PG = COLS / GP < 8 ? COLS / GP : 8;
   static constexpr int PAGES = PG == 1 ? 2 : PG < 4 ? 4 : PG, NB = PAGES / PG;
   uint32_t k[PAGES][W], v[PAGES][2 * G];
@@ -1195,7 +1225,7 @@ __global__ __launch_bounds__(64 * kQ4SumWaves) void q4_chunk_weights_kernel(cons
 // ---------------------------------------------------------------------------------------------
 struct Q4Plan {
   int parts, rows_per_tile;
-  bool wide;
+  bool wide, halves;
   int tiles, splits, split_pages;
   int64_t rows;
   size_t rec, lse, scores, score_stride, ops, aux, bytes;  // (the parts in floats)
@@ -1217,13 +1247,16 @@ static Q4Plan q4_plan(int io_dtype, int32_t batch, int32_t heads, int32_t kv_hea
   const int64_t target = (p.wide ? (head_dim == 64 ? 4 : 3) : 2) * (int64_t)pa_host::device_cu_count();
   const int64_t want = units <= 0 ? 1 : p.wide ? (target / units > 1 ? target / units : 1) : (target + units - 1) / units;
   int pages = (int)((max_pages + want - 1) / want);
-  // a second launch merges ranges: 64 pages (one batch or two per wavefront) are not worth it, 128 are
-  const int least = p.wide ? 16 : max_pages <= 64 ? 64 : 32;
+  // A second launch merges ranges: 64 pages (one batch or two per wavefront) are not worth it, 128 are; nor
+  // are they for the wide kernel where its row tiles alone give every CU a workgroup.
+  const int least = p.wide ? (units >= pa_host::device_cu_count() ? 64 : 16) : max_pages <= 64 ? 64 : 32;
   if (!p.wide && pages > 96) pages = 96;  // requests of very different lengths: ranges end together
   pages = pages < least ? least : pages;
   pages = (pages + 7) / 8 * 8;
   p.split_pages = pages;
   p.splits = max_pages > pages ? (max_pages + pages - 1) / pages : 1;
+  // eight wavefronts to a workgroup while there are fewer than two workgroups a CU
+  p.halves = p.wide && units * p.splits < 2 * (int64_t)pa_host::device_cu_count();
   p.rec = p.splits > 1 ? (size_t)batch * kv_heads * p.rows * p.splits * (head_dim + 2) : 0;
   p.lse = weights ? (size_t)batch * kv_heads * p.rows : 0;
   p.score_stride = (size_t)(max_pages + (max_pages & 1)) * kQ4Tokens;
@@ -1243,8 +1276,10 @@ static Q4Plan q4_plan(int io_dtype, int32_t batch, int32_t heads, int32_t kv_hea
 template <typename IO, int HD, int PARTS>
 static void launch_q4(const Q4Args& a, const Q4Plan& p, hipStream_t stream) {
   const dim3 grid((unsigned)((int64_t)a.B * a.Hk * p.tiles * p.splits));
-  if (p.wide)
-    q4_wide_kernel<IO, HD, PARTS><<<grid, 64 * kQ4WideWaves, 0, stream>>>(a);
+  if (p.wide && p.halves)
+    q4_wide_kernel<IO, HD, PARTS, 2><<<grid, 2 * 64 * kQ4WideWaves, 0, stream>>>(a);
+  else if (p.wide)
+    q4_wide_kernel<IO, HD, PARTS, 1><<<grid, 64 * kQ4WideWaves, 0, stream>>>(a);
   else if (p.rows == 1)
     q4_narrow_kernel<IO, HD, PARTS, 1><<<grid, 64 * kQ4Waves, 0, stream>>>(a);
   else if (p.rows <= 4)
