@@ -117,6 +117,10 @@ def _call_workspace(device: torch.device, nbytes: int, kind: str) -> torch.Tenso
     memory, one per capture and stream, cleared by the first call that the graph replays. The stream
     that allocated a workspace is the only one that uses it, so that one dropped here (at most
     MAX_STREAM_WORKSPACES are held) is reused in stream order."""
+    if kind == "q4":
+        # A decode step's scores grow with the page table: sizes in powers of two, so that a growing context
+        # allocates a few times, and what the default stream keeps adds up to one more of the last size.
+        nbytes = 1 << max(nbytes - 1, 0).bit_length()
     stream = _stream_ptr(device)
     if stream == 0:
         return _workspace(device, nbytes, kind)
