@@ -508,7 +508,7 @@ __global__ __launch_bounds__(64 * kQ4WideWaves * HALVES, HALVES == 2 ? 2 : 3) vo
   constexpr int LOADS = HD == 128 ? 3 : 2;  // load instructions of a page
   __shared__ __attribute__((aligned(16))) uint8_t ring[kQ4Ring * STAGE > JOIN ? kQ4Ring * STAGE : JOIN];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int half = wave / kQ4WideWaves, tile_wave = wave % kQ4WideWaves;
+  const int half = HALVES == 2 ? wave / kQ4WideWaves : 0, tile_wave = HALVES == 2 ? wave % kQ4WideWaves : wave;
   const int g = lane >> 4, c = lane & 15;
   Q4Unit u = q4_unit(a);
   u.b = __builtin_amdgcn_readfirstlane(q4_by_length(a.seq_lens, a.B, u.b, lane));
