@@ -117,6 +117,7 @@ struct Q4Wave {
   int n;        // keys the column sees (a column without a row: 0x7fffffff)
   f32x4 o[G][4];
   float y[G], M, l;
+  f32x4 yw[G];  // PARTS = 1: -7.5 times the sum of w, every row of the product alike
 };
 
 template <typename IO>
@@ -200,6 +201,7 @@ __device__ __forceinline__ void q4_setup(const Q4Args& a, int b, int hk, int til
 #pragma unroll
   for (int k = 0; k < G; ++k) {
     w.y[k] = 0.f;
+    w.yw[k] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int t = 0; t < 4; ++t) w.o[k][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -365,6 +367,7 @@ __device__ __forceinline__ void q4_step(const uint8_t* pg, Q4Wave<HD, PARTS>& w,
 #pragma unroll
     for (int k = 0; k < G; ++k) {
       w.y[k] *= f;
+      w.yw[k] *= f;
 #pragma unroll
       for (int t = 0; t < 4; ++t) w.o[k][t] *= f;
     }
@@ -377,10 +380,10 @@ __device__ __forceinline__ void q4_step(const uint8_t* pg, Q4Wave<HD, PARTS>& w,
   for (int k = 0; k < G; ++k) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) w.y[k] = fmaf(p[e >> 2][e & 3], q4_centre(vm[e >> 2][k][e & 3]), w.y[k]);
-    if constexpr (PARTS == 1) {  // -7.5 w, as rounded
-      const h16x2 mid = {(__fp16)-7.5f, (__fp16)-7.5f};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) w.y[k] = __builtin_amdgcn_fdot2(__builtin_bit_cast(h16x2, pw[k][e]), mid, w.y[k], false);
+    if constexpr (PARTS == 1) {  // -7.5 w, as rounded; the matrix cores have the time (dot products: 213 -> 211 us)
+      constexpr _Float16 m = (_Float16)-7.5f;
+      w.yw[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f16x8{m, m, m, m, m, m, m, m},
+                                                       q4_operand(pw[k][0], pw[k][1], pw[k][2], pw[k][3]), w.yw[k], 0, 0, 0);
     }
   }
   uint32_t vw[2][2 * G];
@@ -410,7 +413,7 @@ __device__ __forceinline__ void q4_join(Q4Wave<HD, PARTS>& w, float (&o)[HD / kQ
   l = sum_xor32(sum_xor16(w.l));
 #pragma unroll
   for (int k = 0; k < G; ++k) {
-    const float y = sum_xor32(sum_xor16(w.y[k]));
+    const float y = sum_xor32(sum_xor16(w.y[k])) + w.yw[k][0];
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
