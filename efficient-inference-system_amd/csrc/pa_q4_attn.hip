@@ -367,7 +367,7 @@ __device__ __forceinline__ void q4_step(const uint8_t* pg, Q4Wave<HD, PARTS>& w,
 #pragma unroll
     for (int k = 0; k < G; ++k) {
       w.y[k] *= f;
-      w.yw[k] *= f;
+      if constexpr (PARTS == 1) w.yw[k] *= f;
 #pragma unroll
       for (int t = 0; t < 4; ++t) w.o[k][t] *= f;
     }
@@ -380,7 +380,7 @@ __device__ __forceinline__ void q4_step(const uint8_t* pg, Q4Wave<HD, PARTS>& w,
   for (int k = 0; k < G; ++k) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) w.y[k] = fmaf(p[e >> 2][e & 3], q4_centre(vm[e >> 2][k][e & 3]), w.y[k]);
-    if constexpr (PARTS == 1) {  // -7.5 w, as rounded; the matrix cores have the time (dot products: 213 -> 211 us)
+    if constexpr (PARTS == 1) {  // -7.5 w, as rounded: on the matrix cores, which have the time that v_dot2_f32_f16 takes (1%)
       constexpr _Float16 m = (_Float16)-7.5f;
       w.yw[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f16x8{m, m, m, m, m, m, m, m},
                                                        q4_operand(pw[k][0], pw[k][1], pw[k][2], pw[k][3]), w.yw[k], 0, 0, 0);
@@ -413,7 +413,8 @@ __device__ __forceinline__ void q4_join(Q4Wave<HD, PARTS>& w, float (&o)[HD / kQ
   l = sum_xor32(sum_xor16(w.l));
 #pragma unroll
   for (int k = 0; k < G; ++k) {
-    const float y = sum_xor32(sum_xor16(w.y[k])) + w.yw[k][0];
+    float y = sum_xor32(sum_xor16(w.y[k]));
+    if constexpr (PARTS == 1) y += w.yw[k][0];
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
