@@ -36,6 +36,7 @@ __device__ __forceinline__ uint32_t q4_rank(float f) {
 }
 
 constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64;
+constexpr int kSelHists = 8, kSelPitch = 257;  // 16k totals and these leave room for two workgroups a CU
 constexpr int kSelHeld = 32768;  // totals in LDS (128 KB); longer requests read them from memory in every pass
 
 __device__ __forceinline__ int wave_total(int x) {
@@ -44,16 +45,33 @@ __device__ __forceinline__ int wave_total(int x) {
   return x;
 }
 
-// The choice. Four passes of 8 bits narrow the (keep - window)-th largest total down (histograms per
-// wavefront: totals share their high bits, and one histogram would serialise on few addresses); then
-// each wavefront walks its contiguous part of the keys, the counts of the parts before it known, and
-// writes the places of the kept ones in order. No atomics reach memory, so the choice is exact.
+// Inclusive sums over the lanes.
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);  // row_shr:1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
+  return x;
+}
+
+// The choice. Passes of 8 bits narrow the (keep - window)-th largest total down until 64 or fewer share its
+// bits (two passes as a rule), which are compared with each other. Eight histograms for the lanes to take
+// turns at: totals share their high bits, and a wavefront's 64 additions to one address run one after the
+// other. Then each wavefront walks its contiguous part of the keys, the counts of the parts before it
+// known, and writes the places of the kept ones in order. No atomics reach memory, so the choice is exact.
+// 8 requests x 8 heads of 600 to 1000 keys 7.4 us, 16 x 32 heads of 2500 to 16384 keys 27.5 us (17 MB of totals
+// in 64-byte pieces: 11 us of it): latency, of two dependent loads and of the passes' barriers. Four passes
+// with a histogram per wavefront, which left 16k keys one workgroup a CU: 8.7 and 32.6 us.
 __global__ __launch_bounds__(kSelThreads) void q4_choose_kernel(const Q4EvictArgs a) {
   extern __shared__ uint32_t held[];  // the first a.held totals
-  __shared__ int hist[kSelWaves][256];
+  __shared__ int hist[kSelHists][kSelPitch];
   __shared__ int sums[2][kSelWaves];
-  __shared__ uint32_t found_digit;
-  __shared__ int found_above;
+  __shared__ int counts[2][256];
+  __shared__ uint32_t few[64];  // the totals left once there are so few
+  __shared__ uint32_t found;
+  __shared__ int few_count, found_want;
   const int hk = blockIdx.x % a.Hk, b = blockIdx.x / a.Hk;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int32_t* table = a.page_table + (int64_t)b * a.pt_stride;
@@ -76,58 +94,90 @@ __global__ __launch_bounds__(kSelThreads) void q4_choose_kernel(const Q4EvictArg
   const int in_lds = cand < a.held ? cand : a.held;
   int want = a.keep - a.window;  // of the candidates
   uint32_t prefix = 0;
-  for (int shift = 24; shift >= 0 && want > 0; shift -= 8) {
-    for (int i = lane; i < 256; i += 64) hist[wave][i] = 0;
-    __syncthreads();
-    if (shift == 24) {  // the totals come from memory, four at a time on their way
-#pragma unroll 4
-      for (int t = tid; t < cand; t += kSelThreads) {
-        const uint32_t u = total_at(t);
-        if (t < in_lds) held[t] = u;
-        atomicAdd(&hist[wave][u >> 24], 1);
+  int* const mine = hist[lane % kSelHists];
+  for (int i = tid; i < kSelHists * kSelPitch; i += kSelThreads) (&hist[0][0])[i] = 0;
+  __syncthreads();
+  if (want > 0) {  // the totals come from memory, eight at a time on their way
+    for (int t0 = tid; t0 < cand; t0 += 8 * kSelThreads) {
+      int id[8];
+      uint32_t u[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int t = t0 + i * kSelThreads;
+        id[i] = t < cand ? q4_block(table[t / kQ4Tokens], a.num_blocks) : -1;
       }
-    } else {
-      const uint32_t mask = 0xffffffffu << (shift + 8);
-      for (int t = tid; t < cand; t += kSelThreads) {
-        const uint32_t u = t < in_lds ? held[t] : total_at(t);
-        if ((u & mask) == prefix) atomicAdd(&hist[wave][u >> shift & 255], 1);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        u[i] = id[i] < 0 ? 0u : q4_rank(a.weights[((int64_t)id[i] * a.Hk + hk) * kQ4Tokens + (t0 & (kQ4Tokens - 1))]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int t = t0 + i * kSelThreads;
+        if (t < in_lds) held[t] = u[i];
+        if (t < cand) atomicAdd(&mine[u[i] >> 24], 1);
       }
     }
+  }
+  for (int shift = 24, turn = 0; shift >= 0 && want > 0; shift -= 8, turn ^= 1) {
+    const uint32_t seen = shift < 24 ? 0xffffffffu << (shift + 8) : 0u;
+    if (shift < 24)
+      for (int t = tid; t < cand; t += kSelThreads) {
+        const uint32_t u = t < in_lds ? held[t] : total_at(t);
+        if ((u & seen) == prefix) atomicAdd(&mine[u >> shift & 255], 1);
+      }
     __syncthreads();
     if (tid < 256) {
       int n = 0;
 #pragma unroll
-      for (int w = 0; w < kSelWaves; ++w) n += hist[w][tid];
-      hist[0][tid] = n;
+      for (int w = 0; w < kSelHists; ++w) {
+        n += hist[w][tid];
+        hist[w][tid] = 0;  // for the next pass
+      }
+      counts[turn][255 - tid] = n;  // the highest digit first
     }
+    if (tid == 0) few_count = 0;
     __syncthreads();
-    if (wave == 0) {  // the digit where the count from above passes `want`
-      int n[4], mine = 0;
+    // the digit where the count from above passes `want`: every wavefront finds it, four digits a lane
+    int n[4], sum = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        n[i] = hist[0][255 - 4 * lane - i];
-        mine += n[i];
+    for (int i = 0; i < 4; ++i) {
+      n[i] = counts[turn][4 * lane + i];
+      sum += n[i];
+    }
+    int above = wave_scan(sum) - sum, digit = -1, left = 0, before = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (above < want && above + n[i] >= want) {
+        digit = 255 - 4 * lane - i;
+        before = above;
+        left = n[i];
       }
-      int above = mine;  // inclusive prefix over the lanes
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int x = __shfl_up(above, o);
-        if (lane >= o) above += x;
+      above += n[i];
+    }
+    const int at = __builtin_ctzll(__ballot(digit >= 0));  // (one lane: want is at most the candidates left)
+    prefix |= (uint32_t)__builtin_amdgcn_readlane(digit, at) << shift;
+    want -= __builtin_amdgcn_readlane(before, at);
+    left = __builtin_amdgcn_readlane(left, at);
+    if (left <= 64 && shift > 0) {  // each compared with all, four by every wavefront
+      const uint32_t mask = 0xffffffffu << shift;
+      for (int t = tid; t < cand; t += kSelThreads) {
+        const uint32_t u = t < in_lds ? held[t] : total_at(t);
+        if ((u & mask) == prefix) few[atomicAdd(&few_count, 1)] = u;
       }
-      above -= mine;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (above < want && above + n[i] >= want) {
-          found_digit = 255u - 4u * lane - i;
-          found_above = above;
+      __syncthreads();
+      const uint32_t u = lane < left ? few[lane] : 0u;
+      for (int j = wave; j < left; j += kSelWaves) {
+        const uint32_t it = __builtin_amdgcn_readlane(u, j);
+        const int more = __popcll(__ballot(lane < left && u > it)), same = __popcll(__ballot(lane < left && u == it));
+        if (more < want && more + same >= want && lane == 0) {  // (equal ones write the same)
+          found = it;
+          found_want = want - more;
         }
-        above += n[i];
       }
+      __syncthreads();
+      prefix = found;
+      want = found_want;
+      break;
     }
-    __syncthreads();
-    prefix |= found_digit << shift;
-    want -= found_above;
-    __syncthreads();
   }
   auto rank = [&](int t) { return t < in_lds ? held[t] : total_at(t); };
   // kept: totals above `prefix`, and the first `want` equal to it (none where nothing was wanted)
@@ -169,7 +219,10 @@ __global__ __launch_bounds__(kSelThreads) void q4_choose_kernel(const Q4EvictArg
 }
 
 // The move: lane (g, c) = (lane / 16, lane % 16) takes the K words (c, g) and the V words (g, c) of the new
-// page, from wherever each token was. A page's rows behind the last kept one stay as they were.
+// page, from wherever each token was. A page's rows behind the last kept one stay as they were. Bound by
+// memory: a token's V codes are halves of words that it shares with three neighbours, so that a kept token
+// costs whole lines (16 x 32 heads x 128 cut to 2048 of up to 16384 keys: 106 us, some 600 MB at 5.6 TB/s, of
+// which 326 MB are the kept rows).
 template <int HD>
 __global__ __launch_bounds__(256) void q4_move_kernel(const Q4EvictArgs a, int pages, uint32_t total) {
   constexpr int G = HD / kQ4Group, W = HD / 32, PB = q4_page_bytes(HD), CB = q4_codes_bytes(HD);

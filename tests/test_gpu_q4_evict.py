@@ -148,3 +148,23 @@ def test_refusals(device):
                  (pool, pool, w, table, lens, fresh[:0])):
         with pytest.raises(ValueError):
             kq.evict_q4_hip(*args, keep=32, window=8)
+
+
+@pytest.mark.parametrize("cluster", [1, 2, 63, 64, 65, 200])
+@pytest.mark.parametrize("kinds", [1, 3, 1 << 16])
+def test_totals_that_share_their_high_bits(device, cluster, kinds):
+    """The border falls among `cluster` totals whose low 16 bits alone differ, in `kinds` ways; 100 are larger."""
+    rng = np.random.default_rng(cluster + kinds)
+
+    def weights(n):
+        w = rng.uniform(0, 0.5, (n, 2, 16)).astype(np.float32)
+        for h in range(2):
+            flat = rng.permutation(n * 16)
+            view = np.empty(n * 16, dtype=np.float32)
+            view[:] = w[:, h].reshape(-1)
+            view[flat[:100]] = rng.uniform(2, 90, 100)
+            view[flat[100:100 + cluster]] = (0x3f800000 + rng.integers(0, kinds, cluster)).astype(np.uint32).view(np.float32)
+            w[:, h] = view.reshape(n, 16)
+        return w
+
+    _run(device, rng, [600], 2, 64, 100 + cluster // 2 + 9, 9, weights=weights, spare=0)
