@@ -105,3 +105,34 @@ def test_refusals(device):
     with pytest.raises(TypeError):
         kq.kv_read_q4_hip(pool, pool, slots, dtype=torch.float16)
     assert not pool.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("centre", [0.0, 1.0, 30.0, 3000.0, -60000.0])
+def test_values_at_borders_and_a_step_beside_them(device, dtype, centre):
+    """Groups full of values at z + m s, m whole (a tie between two codes where that is exact), and of the next
+    number of the type on either side, about centres of 0 to 60000 steps and more."""
+    rng = np.random.default_rng(int(abs(centre)))
+    rows = 160
+    k = np.empty((rows, 64), dtype=np.float32)
+    for i in range(rows):
+        half = np.float32(2.0 ** rng.integers(-3, 4) * rng.uniform(4, 8))
+        ends = torch.tensor([centre * half / 7.5 + half, centre * half / 7.5 - half]).clamp(-65000, 65000).to(dtype).float().numpy()
+        s, z = (np.float64(np.float16(x)) for x in ((ends[0] - ends[1]) * np.float32(1 / 15), (ends[0] + ends[1]) * np.float32(0.5)))
+        at = torch.from_numpy(z + rng.integers(-7, 8, 62) * s).float().to(dtype)
+        step = torch.from_numpy(rng.integers(-1, 2, 62).astype(np.int32))
+        if dtype == torch.float32:
+            at = (at.view(torch.int32) + step).view(torch.float32)
+        else:
+            at = (at.view(torch.int16) + step.to(torch.int16)).view(torch.bfloat16)
+        k[i] = np.concatenate([ends, at.float().numpy()]).clip(ends.min(), ends.max())
+    t = torch.from_numpy(k).to(dtype).view(1, rows, 1, 64).transpose(1, 2).to(device)
+    pool = np.zeros((rows // 16, 1, q4.page_bytes(64)), dtype=np.uint8)
+    dk, dv = torch.from_numpy(pool.copy()).to(device), torch.from_numpy(pool.copy()).to(device)
+    kq.kv_append_q4_hip(t, t, dk, dv, torch.arange(rows, dtype=torch.int32, device=device))
+    vp = pool.copy()
+    for i in range(rows):
+        q4.put(pool, i // 16, 0, i % 16, k[i], True)
+        q4.put(vp, i // 16, 0, i % 16, k[i], False)
+    assert np.array_equal(dk.cpu().numpy(), pool)
+    assert np.array_equal(dv.cpu().numpy(), vp)
