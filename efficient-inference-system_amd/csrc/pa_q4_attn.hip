@@ -1127,16 +1127,17 @@ __global__ __launch_bounds__(256) void q4_finish_kernel(const Q4Args a, int64_t 
   }
 }
 
-// Totals of a chunk: the scores formed again, four pages (64 keys) per workgroup whose operands and pairs stay
-// in registers; the workgroup's wavefronts take the row tiles in turn and their sums meet in LDS in a fixed
-// order. READY: the tiles' q operands are in the workspace, left by the wide kernel (formed here they cost as
-// much as the scores). A block that two rows of the page table share is added to by both, hence the atomic;
-// otherwise each slot gets one addition.
-constexpr int kQ4SumWaves = 8, kQ4SumPages = 4;
+// Totals of a chunk: the scores formed again, PG pages per workgroup whose operands and pairs stay in registers;
+// the workgroup's wavefronts take the row tiles in turn, the next tile's operands on their way, and their
+// sums meet in LDS in a fixed order. READY: the tiles' q operands are in the workspace, left by the wide
+// kernel (formed here they cost as much as the scores). A block that two rows of the page table share is
+// added to by both, hence the atomic; otherwise each slot gets one addition. Bound by vector instructions, 170
+// to 16 matrix instructions a tile: 200 rows of 32 over 8 heads x 128 bf16 over 16.5k keys 72 us (370 TFLOP/s).
+constexpr int kQ4SumWaves = 8;
 
-template <typename IO, int HD, int PARTS, bool READY>
+template <typename IO, int HD, int PARTS, bool READY, int PG>
 __global__ __launch_bounds__(64 * kQ4SumWaves) void q4_chunk_weights_kernel(const Q4Args a) {
-  constexpr int G = HD / kQ4Group, W = HD / 32, PB = q4_page_bytes(HD), PG = kQ4SumPages;
+  constexpr int G = HD / kQ4Group, W = HD / 32, PB = q4_page_bytes(HD);
   constexpr int ROWS = 16 / PARTS;
   __shared__ float part[kQ4SumWaves][PG * kQ4Tokens];
   const int b = blockIdx.z, hk = blockIdx.y;
@@ -1170,19 +1171,37 @@ __global__ __launch_bounds__(64 * kQ4SumWaves) void q4_chunk_weights_kernel(cons
   for (int h = 0; h < PG; ++h)
 #pragma unroll
     for (int i = 0; i < 4; ++i) sum[h][i] = 0.f;
-  for (int tile = (int)((int64_t)i0 * a.group / ROWS) + wave; tile * ROWS < real; tile += kQ4SumWaves) {
-    f16x8 q[W];
-    float qs[G], sc;
-    int n;
+  // (the next tile's operands are loaded while this one's scores are formed; past the last one, its own)
+  f16x8 next[W];
+  f32x4 next_aux;
+  float next_lse;
+  const int last = (real - 1) / ROWS;
+  auto load = [&](int tile) {
+    tile = tile < last ? tile : last;
+    const int row = q4_row<PARTS>(tile, c);
+    next_lse = row < real && c < ROWS ? *q4_lse(a, b, hk, row < rows ? row : rows - 1) : INFINITY;  // (2^-inf: 0)
     if constexpr (READY) {
       const int64_t at = ((int64_t)b * a.Hk + hk) * a.op_tiles + tile;
 #pragma unroll
-      for (int s = 0; s < W; ++s) q[s] = a.q_ops[(at * W + s) * 64 + lane];
-      const f32x4 x = a.q_aux[at * 64 + lane];
+      for (int s = 0; s < W; ++s) next[s] = a.q_ops[(at * W + s) * 64 + lane];
+      next_aux = a.q_aux[at * 64 + lane];
+    }
+  };
+  int tile = (int)((int64_t)i0 * a.group / ROWS) + wave;
+  if (tile * ROWS < real) load(tile);
+  for (; tile * ROWS < real; tile += kQ4SumWaves) {
+    f16x8 q[W];
+    float qs[G], sc;
+    int n;
+    const float lse = next_lse;
+    if constexpr (READY) {
 #pragma unroll
-      for (int k = 0; k < G; ++k) qs[k] = x[k];
-      sc = x[2];
-      n = __float_as_int(x[3]);
+      for (int s = 0; s < W; ++s) q[s] = next[s];
+#pragma unroll
+      for (int k = 0; k < G; ++k) qs[k] = next_aux[k];
+      sc = next_aux[2];
+      n = __float_as_int(next_aux[3]);
+      load(tile + kQ4SumWaves);
     } else {
       Q4Wave<HD, PARTS> w;
       q4_setup<IO, HD, PARTS>(a, b, hk, tile, L, C, keys, lane, w);
@@ -1192,19 +1211,20 @@ __global__ __launch_bounds__(64 * kQ4SumWaves) void q4_chunk_weights_kernel(cons
       for (int k = 0; k < G; ++k) qs[k] = w.qs[k];
       sc = w.sc;
       n = w.n;
+      load(tile + kQ4SumWaves);
     }
-    const int row = q4_row<PARTS>(tile, c);
-    const float lse = row < real && c < ROWS ? *q4_lse(a, b, hk, row < rows ? row : rows - 1) : INFINITY;  // (2^-inf: 0)
-    const bool masked = __any(n < key0 + PG * kQ4Tokens);
+    auto add = [&](auto masked) {
 #pragma unroll
-    for (int h = 0; h < PG; ++h) {
-      const f32x4 S = q4_scores<HD, PARTS>(kf[h], km[h], q, qs);
+      for (int h = 0; h < PG; ++h) {
+        const f32x4 S = q4_scores<HD, PARTS>(kf[h], km[h], q, qs);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float p = fast_exp2(fmaf(S[i], sc, -lse));
-        sum[h][i] += masked && key0 + h * kQ4Tokens + 4 * g + i >= n ? 0.f : p;
+        for (int i = 0; i < 4; ++i) {
+          const float p = fast_exp2(fmaf(S[i], sc, -lse));
+          sum[h][i] += decltype(masked)::value && key0 + h * kQ4Tokens + 4 * g + i >= n ? 0.f : p;
+        }
       }
-    }
+    };
+    if (__any(n < key0 + PG * kQ4Tokens)) add(std::true_type()); else add(std::false_type());
   }
 #pragma unroll
   for (int h = 0; h < PG; ++h)
@@ -1299,11 +1319,19 @@ static void launch_q4(const Q4Args& a, const Q4Plan& p, hipStream_t stream) {
     q4_finish_kernel<IO, HD><<<(unsigned)wgs, 256, 0, stream>>>(a, total, merges, chunks);
   }
   if (a.weights != nullptr && a.scores == nullptr) {
-    const dim3 wg((unsigned)((a.max_pages + kQ4SumPages - 1) / kQ4SumPages), a.Hk, a.B);
-    if (a.q_ops != nullptr)
-      q4_chunk_weights_kernel<IO, HD, PARTS, true><<<wg, 64 * kQ4SumWaves, 0, stream>>>(a);
+    auto sum = [&](auto ready, auto pages) {
+      const dim3 wg((unsigned)((a.max_pages + pages - 1) / pages), a.Hk, a.B);
+      q4_chunk_weights_kernel<IO, HD, PARTS, decltype(ready)::value, decltype(pages)::value><<<wg, 64 * kQ4SumWaves, 0, stream>>>(a);
+    };
+    // a page each while four would leave CUs without a workgroup (3 x 61 rows of 24 over 3 heads x 64: 9.2 ->
+    // 5.9 us); otherwise four, which read the row tiles' operands the least often (two: 72 -> 84 us, see above)
+    const bool small = (int64_t)a.Hk * a.B * a.max_pages < 4 * pa_host::device_cu_count();
+    if (a.q_ops == nullptr)  // (up to two row tiles)
+      sum(std::false_type(), std::integral_constant<int, 1>());
+    else if (small)
+      sum(std::true_type(), std::integral_constant<int, 1>());
     else
-      q4_chunk_weights_kernel<IO, HD, PARTS, false><<<wg, 64 * kQ4SumWaves, 0, stream>>>(a);
+      sum(std::true_type(), std::integral_constant<int, 4>());
   }
 }
 
