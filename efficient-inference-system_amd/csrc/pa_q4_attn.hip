@@ -478,6 +478,11 @@ constexpr int kQ4MaxNarrow = 32;  // rows that the narrow kernel takes (two tile
 // of three, with one barrier a stage. Read from memory by each wavefront for itself, the pages' pairs alone
 // (16 bytes that 16 lanes share) cost more load instructions than the codes.
 //
+// Bound by vector instructions: a step of 32 keys takes some 200 (the codes' ANDs and shifts 80, the pairs' scales
+// and centres 64, exponentials and sums the rest) to 18 matrix instructions, 82% of the cycles that a CU has
+// work (4 x 512 rows of 32 heads x 128 bf16 over 512 to 1024 keys: 215 us, 460 TFLOP/s; 200 rows of 32 over 8 heads
+// over 16k keys: 140 us, 380). Two tiles a wavefront, which share the codes' part, take 256 registers: 240 us.
+//
 // HALVES = 2, for grids that leave the GPU room: eight wavefronts for the same four tiles, stages of 128 keys,
 // each half of the wavefronts taking its half of every stage, joined in LDS at the end. A step is a chain of
 // LDS reads, matrix instructions and exponentials that one wavefront a SIMD does not fill (4 x 256 rows of 8
@@ -658,6 +663,10 @@ __global__ __launch_bounds__(64 * kQ4WideWaves * HALVES, HALVES == 2 ? 2 : 3) vo
 //
 // A batch's loads are all issued before its products, and K's registers are filled again while the second
 // product runs: 16 KB and more in flight per wavefront.
+//
+// Bound by memory: 16 requests of 8k to 16k keys, 32 heads x 128 bf16, 577 MB read: 111 us, 5.2 TB/s (one column
+// of rows repeated sixteen times instead: 370 us; batches of one page: 227 us). 64 requests of 32 over 8 heads
+// to 16k with totals: 339 MB read, 41 MB of scores written, 85 us, 4.5 TB/s.
 // ---------------------------------------------------------------------------------------------
 template <int N>
 __device__ __forceinline__ uint32_t row_from(uint32_t x) {  // lane c of a 16-lane row: lane (c + N) % 16
@@ -1060,7 +1069,8 @@ __device__ __forceinline__ void q4_row_state(const float* rec, int splits, int l
 // kernel left in the workspace. The first `merges` workgroups merge, one wavefront per row; of the others each
 // adds kQ4FinishKeys keys' weights of one KV head, having formed its rows' denominators from the records by itself (a
 // launch less than in two steps). A block that two rows of the page table share is added to by both, hence
-// the atomic; otherwise each slot gets one addition.
+// the atomic; otherwise each slot gets one addition. 64 requests of 32 over 8 heads to 16k keys: 42 MB of scores
+// and 10 MB of records and totals, 21 us, bound by the records that every workgroup reads again.
 constexpr int kQ4FinishKeys = 1024;  // (256, a key per thread, repeated the denominators too often: 34 -> 20 us)
 
 template <typename IO, int HD>
@@ -1129,21 +1139,22 @@ __global__ __launch_bounds__(256) void q4_finish_kernel(const Q4Args a, int64_t 
 
 // Totals of a chunk: the scores formed again, PG pages per workgroup whose operands and pairs stay in registers;
 // the workgroup's wavefronts take the row tiles in turn, the next tile's operands on their way, and their
-// sums meet in LDS in a fixed order. READY: the tiles' q operands are in the workspace, left by the wide
+// sums meet in LDS in a fixed order; or (EACH) every wavefront has pages of its own and takes all tiles. READY: the tiles' q operands are in the workspace, left by the wide
 // kernel (formed here they cost as much as the scores). A block that two rows of the page table share is
 // added to by both, hence the atomic; otherwise each slot gets one addition. Bound by vector instructions, 170
 // to 16 matrix instructions a tile: 200 rows of 32 over 8 heads x 128 bf16 over 16.5k keys 72 us (370 TFLOP/s).
 constexpr int kQ4SumWaves = 8;
 
-template <typename IO, int HD, int PARTS, bool READY, int PG>
+template <typename IO, int HD, int PARTS, bool READY, int PG, bool EACH>
 __global__ __launch_bounds__(64 * kQ4SumWaves) void q4_chunk_weights_kernel(const Q4Args a) {
   constexpr int G = HD / kQ4Group, W = HD / 32, PB = q4_page_bytes(HD);
   constexpr int ROWS = 16 / PARTS;
+  constexpr int STEP = EACH ? 1 : kQ4SumWaves;  // from one row tile of a wavefront to its next
   __shared__ float part[kQ4SumWaves][PG * kQ4Tokens];
   const int b = blockIdx.z, hk = blockIdx.y;
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int p0 = PG * (int)blockIdx.x, key0 = p0 * kQ4Tokens;
+  const int p0 = PG * (EACH ? (int)blockIdx.x * kQ4SumWaves + wave : (int)blockIdx.x), key0 = p0 * kQ4Tokens;
   const int L = a.seq_lens[b], C = a.cur_lens[b];
   const int keys = L < a.max_pages * kQ4Tokens ? L : a.max_pages * kQ4Tokens;
   if (key0 >= keys || C < 1) return;
@@ -1187,9 +1198,9 @@ __global__ __launch_bounds__(64 * kQ4SumWaves) void q4_chunk_weights_kernel(cons
       next_aux = a.q_aux[at * 64 + lane];
     }
   };
-  int tile = (int)((int64_t)i0 * a.group / ROWS) + wave;
+  int tile = (int)((int64_t)i0 * a.group / ROWS) + (EACH ? 0 : wave);
   if (tile * ROWS < real) load(tile);
-  for (; tile * ROWS < real; tile += kQ4SumWaves) {
+  for (; tile * ROWS < real; tile += STEP) {
     f16x8 q[W];
     float qs[G], sc;
     int n;
@@ -1201,7 +1212,7 @@ __global__ __launch_bounds__(64 * kQ4SumWaves) void q4_chunk_weights_kernel(cons
       for (int k = 0; k < G; ++k) qs[k] = next_aux[k];
       sc = next_aux[2];
       n = __float_as_int(next_aux[3]);
-      load(tile + kQ4SumWaves);
+      load(tile + STEP);
     } else {
       Q4Wave<HD, PARTS> w;
       q4_setup<IO, HD, PARTS>(a, b, hk, tile, L, C, keys, lane, w);
@@ -1211,7 +1222,7 @@ __global__ __launch_bounds__(64 * kQ4SumWaves) void q4_chunk_weights_kernel(cons
       for (int k = 0; k < G; ++k) qs[k] = w.qs[k];
       sc = w.sc;
       n = w.n;
-      load(tile + kQ4SumWaves);
+      load(tile + STEP);
     }
     auto add = [&](auto masked) {
 #pragma unroll
@@ -1231,8 +1242,14 @@ __global__ __launch_bounds__(64 * kQ4SumWaves) void q4_chunk_weights_kernel(cons
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float s = group_sum<16>(sum[h][i]);
-      if (c == i) part[wave][h * kQ4Tokens + 4 * g + i] = s;
+      if (c != i) continue;
+      const int t = h * kQ4Tokens + 4 * g + i;
+      if constexpr (!EACH)
+        part[wave][t] = s;
+      else if (id[h] >= 0 && key0 + t < keys)
+        atomicAdd(a.weights + ((int64_t)id[h] * a.Hk + hk) * kQ4Tokens + 4 * g + i, s);
     }
+  if constexpr (EACH) return;
   __syncthreads();
   const int t = threadIdx.x;
   if (t < PG * kQ4Tokens && key0 + t < keys) {
@@ -1249,7 +1266,7 @@ __global__ __launch_bounds__(64 * kQ4SumWaves) void q4_chunk_weights_kernel(cons
 // ---------------------------------------------------------------------------------------------
 struct Q4Plan {
   int parts, rows_per_tile;
-  bool wide, halves;
+  bool wide, halves, four;
   int tiles, splits, split_pages;
   int64_t rows;
   size_t rec, lse, scores, score_stride, ops, aux, bytes;  // (the parts in floats)
@@ -1263,7 +1280,16 @@ static Q4Plan q4_plan(int io_dtype, int32_t batch, int32_t heads, int32_t kv_hea
   p.parts = io_dtype == PA_DTYPE_F32 ? 2 : 1;
   const int rpt = p.parts == 2 ? 8 : 16;
   p.rows = (int64_t)query_len * (heads / kv_heads);
-  p.wide = p.rows > 2 * rpt;
+  // More rows than two tiles: the wide kernel. Up to there the narrow one, whose tiles each read the keys for
+  // themselves, but for bf16 at head_dim 128, where more than four rows leave it batches of two pages: there from
+  // 512 keys on the wide one again, for one tile while it gives a CU at most one workgroup. 8 requests of
+  // 32 over 4 heads (8 rows), 512 / 2048 / 8192 keys: 13.9 / 22.9 / 31.0 -> 13.7 / 14.2 / 22.5 us; 64 of 48 over 8 (6 rows):
+  // 26.8 / 66.9 / 161 -> 19.8 / 57.8 / 208; 24 rows of 8 x 8 units, 512 / 1024 / 8192: 20.7 / 25.3 / 64.2 -> 15.6 / 17.4 /
+  // 41.3, at 128 7.8 -> 8.3; at head_dim 64 7.5 / 10.3 / 28.0 -> 12.5 / 13.5 / 27.2; fp32, 16 rows: 11.4 / 16.7 / 60.8 -> 17.4 /
+  // 18.9 / 53.8.
+  const bool early = p.parts == 1 && head_dim == 128 && p.rows > 4 && max_pages >= 32 && (!weights || query_len > 1 || (int64_t)batch * kv_heads * max_pages <= 16384) &&
+                     (p.rows > rpt || (int64_t)batch * kv_heads <= pa_host::device_cu_count());
+  p.wide = p.rows > 2 * rpt || early;
   p.rows_per_tile = p.wide ? kQ4WideWaves * rpt : rpt;
   p.tiles = (int)((p.rows + p.rows_per_tile - 1) / p.rows_per_tile);
   const int64_t units = (int64_t)batch * kv_heads * p.tiles;
@@ -1279,6 +1305,10 @@ static Q4Plan q4_plan(int io_dtype, int32_t batch, int32_t heads, int32_t kv_hea
   pages = (pages + 7) / 8 * 8;
   p.split_pages = pages;
   p.splits = max_pages > pages ? (max_pages + pages - 1) / pages : 1;
+  // One row: 8 (fp32) or 16 pages of columns to it, but four for many pages of bf16 at head_dim 128, whose batches
+  // are half the size (2 x 32 heads over 1024 / 4096 / 16384 keys 8.5 / 11.8 / 27.4 -> 9.1 / 12.2 / 25.9 us, 16 x 32
+  // 12.5 / 43.1 / 154 -> 13.0 / 40.1 / 145; fp32 53 -> 66).
+  p.four = p.parts == 1 && head_dim == 128 && units * max_pages >= 49152;
   // eight wavefronts to a workgroup while there are fewer than two workgroups a CU
   p.halves = p.wide && units * p.splits < 2 * (int64_t)pa_host::device_cu_count();
   p.rec = p.splits > 1 ? (size_t)batch * kv_heads * p.rows * p.splits * (head_dim + 2) : 0;
@@ -1304,7 +1334,7 @@ static void launch_q4(const Q4Args& a, const Q4Plan& p, hipStream_t stream) {
     q4_wide_kernel<IO, HD, PARTS, 2><<<grid, 2 * 64 * kQ4WideWaves, 0, stream>>>(a);
   else if (p.wide)
     q4_wide_kernel<IO, HD, PARTS, 1><<<grid, 64 * kQ4WideWaves, 0, stream>>>(a);
-  else if (p.rows == 1)
+  else if (p.rows == 1 && !p.four)
     q4_narrow_kernel<IO, HD, PARTS, 1><<<grid, 64 * kQ4Waves, 0, stream>>>(a);
   else if (p.rows <= 4)
     q4_narrow_kernel<IO, HD, PARTS, 4><<<grid, 64 * kQ4Waves, 0, stream>>>(a);
@@ -1319,19 +1349,32 @@ static void launch_q4(const Q4Args& a, const Q4Plan& p, hipStream_t stream) {
     q4_finish_kernel<IO, HD><<<(unsigned)wgs, 256, 0, stream>>>(a, total, merges, chunks);
   }
   if (a.weights != nullptr && a.scores == nullptr) {
-    auto sum = [&](auto ready, auto pages) {
-      const dim3 wg((unsigned)((a.max_pages + pages - 1) / pages), a.Hk, a.B);
-      q4_chunk_weights_kernel<IO, HD, PARTS, decltype(ready)::value, decltype(pages)::value><<<wg, 64 * kQ4SumWaves, 0, stream>>>(a);
+    // PG: a page while four would leave CUs without a workgroup (3 x 61 rows of 24 over 3 heads x 64: 9.2 -> 5.9 us),
+    // otherwise four, which read the row tiles' operands the least often (two: 72 -> 84 us at the size above).
+    // EACH: for few tiles, and for up to 32 where the pages fill the GPU (8 x 4 rows of 32 over 8 heads x 128 over
+    // 2048 keys, 32 x 12 of 32 heads, 4 x 200 of 32 heads, whole calls: 41 -> 25, 746 -> 194, 146 -> 119 us; but
+    // 3 x 61 as above 15 -> 28).
+    auto sum = [&](auto ready, auto pages, auto each) {
+      const int per = pages * (each ? kQ4SumWaves : 1);
+      const dim3 wg((unsigned)((a.max_pages + per - 1) / per), a.Hk, a.B);
+      q4_chunk_weights_kernel<IO, HD, PARTS, decltype(ready)::value, decltype(pages)::value, decltype(each)::value>
+          <<<wg, 64 * kQ4SumWaves, 0, stream>>>(a);
     };
-    // a page each while four would leave CUs without a workgroup (3 x 61 rows of 24 over 3 heads x 64: 9.2 ->
-    // 5.9 us); otherwise four, which read the row tiles' operands the least often (two: 72 -> 84 us, see above)
-    const bool small = (int64_t)a.Hk * a.B * a.max_pages < 4 * pa_host::device_cu_count();
-    if (a.q_ops == nullptr)  // (up to two row tiles)
-      sum(std::false_type(), std::integral_constant<int, 1>());
-    else if (small)
-      sum(std::true_type(), std::integral_constant<int, 1>());
-    else
-      sum(std::true_type(), std::integral_constant<int, 4>());
+    constexpr std::integral_constant<int, 1> one;
+    constexpr std::integral_constant<int, 4> four;
+    constexpr std::true_type yes;
+    constexpr std::false_type no;
+    const int64_t units = (int64_t)a.Hk * a.B * a.max_pages, cus = pa_host::device_cu_count();
+    const int64_t tiles = (p.rows + 16 / PARTS - 1) / (16 / PARTS);
+    if (tiles <= 4 || (tiles <= 32 && units >= 8 * cus)) {
+      const bool small = units < 4 * 4 * kQ4SumWaves * cus;
+      if (a.q_ops == nullptr)
+        small ? sum(no, one, yes) : sum(no, four, yes);
+      else
+        small ? sum(yes, one, yes) : sum(yes, four, yes);
+    } else {
+      units < 4 * cus ? sum(yes, one, no) : sum(yes, four, no);
+    }
   }
 }
 

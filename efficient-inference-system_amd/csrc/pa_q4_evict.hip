@@ -220,9 +220,8 @@ __global__ __launch_bounds__(kSelThreads) void q4_choose_kernel(const Q4EvictArg
 
 // The move: lane (g, c) = (lane / 16, lane % 16) takes the K words (c, g) and the V words (g, c) of the new
 // page, from wherever each token was. A page's rows behind the last kept one stay as they were. Bound by
-// memory: a token's V codes are halves of words that it shares with three neighbours, so that a kept token
-// costs whole lines (16 x 32 heads x 128 cut to 2048 of up to 16384 keys: 106 us, some 600 MB at 5.6 TB/s, of
-// which 326 MB are the kept rows).
+// memory: 16 x 32 heads x 128 cut to 2048 of up to 16384 keys, 337 MB read (163 MB of them kept: a token's V codes
+// are halves of words that three neighbours share) and 155 MB written: 106 us, 4.6 TB/s, the rate of a copy.
 template <int HD>
 __global__ __launch_bounds__(256) void q4_move_kernel(const Q4EvictArgs a, int pages, uint32_t total) {
   constexpr int G = HD / kQ4Group, W = HD / 32, PB = q4_page_bytes(HD), CB = q4_codes_bytes(HD);

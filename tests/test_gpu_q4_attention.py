@@ -303,3 +303,40 @@ def test_captured_replays_and_two_streams(device, T):
     torch.cuda.synchronize()
     for got, want in zip(gots, wants):
         assert all(torch.equal(g, want) for g in got)
+
+
+# Sizes on both sides of the launch rules' borders (rows of a KV head, width of the page table, units).
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("heads, T, width", [
+    ((2, 2), 1, 6200),    # a row, many pages
+    ((8, 1), 1, 40),      # five rows and more of a decode step, 512 keys and more
+    ((8, 1), 1, 4200),    # the same, totals by the scores
+    ((16, 2), 3, 31),     # a short chunk, few pages
+    ((16, 2), 3, 260),    # two tiles
+    ((6, 2), 1, 4200),
+    ((4, 2), 10, 4200),   # totals: pages of its own for a wavefront, four at a time
+    ((8, 2), 16, 300),    # up to 32 tiles
+    ((8, 1), 80, 20),     # more, few pages
+    ((8, 1), 80, 300),    # more, four pages at a time
+    ((2, 2), 70, 8),      # eight wavefronts to four tiles
+    ((2, 2), 70, 260),    # ranges of keys
+], ids=str)
+def test_launch_rules(device, dtype, hd, heads, T, width):
+    rng = np.random.default_rng(T + width)
+    cur = [T, max(1, T // 2), 1, T]
+    lens = [T + 37, T // 2 + 90, 1, T]
+    blocks = sum(-(-n // 16) for n in lens) + 2
+    kp, vp = filled_pools(rng, blocks, heads[1], hd)
+    _check(device, rng, dtype, *heads, hd, T, lens, cur, kp, vp, tables(rng, lens, blocks, width=width))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("T", [1, 3, 12])
+def test_groups_over_long_contexts(device, dtype, hd, T):
+    rng = np.random.default_rng(hd + T)
+    lens, cur = [2100, 905, 33], [T, T, min(T, 2)]
+    blocks = sum(-(-n // 16) for n in lens) + 2
+    kp, vp = filled_pools(rng, blocks, 2, hd)
+    _check(device, rng, dtype, 16, 2, hd, T, lens, cur, kp, vp, tables(rng, lens, blocks))
