@@ -25,8 +25,8 @@
 // inside fp16, above its subnormals for keys within 2^-18 of the heaviest. M cancels in O / l.
 //
 // Kernels:
-//   q4_narrow_kernel  up to one tile of rows: the workgroup's wavefronts split the keys and merge in LDS
-//                     (decode, short chunks).
+//   q4_narrow_kernel  a tile of rows: the workgroup's wavefronts split the keys and merge in LDS (decode,
+//                     chunks of up to two tiles).
 //   q4_wide_kernel    each wavefront has a tile of its own, and the workgroup's walk all keys together,
 //                     staged through LDS.
 //   Either splits the keys over several workgroups when the grid is small, as records (M, l, O) that
@@ -480,13 +480,13 @@ constexpr int kQ4MaxNarrow = 32;  // rows that the narrow kernel takes (two tile
 //
 // Bound by vector instructions: a step of 32 keys takes some 200 (the codes' ANDs and shifts 80, the pairs' scales
 // and centres 64, exponentials and sums the rest) to 18 matrix instructions, 82% of the cycles that a CU has
-// work (4 x 512 rows of 32 heads x 128 bf16 over 512 to 1024 keys: 215 us, 460 TFLOP/s; 200 rows of 32 over 8 heads
+// work (4 x 512 rows of 32 heads x 128 bf16 over 1024 to 4096 keys: 215 us, 460 TFLOP/s; 200 rows of 32 over 8 heads
 // over 16k keys: 140 us, 380). Two tiles a wavefront, which share the codes' part, take 256 registers: 240 us.
 //
 // HALVES = 2, for grids that leave the GPU room: eight wavefronts for the same four tiles, stages of 128 keys,
 // each half of the wavefronts taking its half of every stage, joined in LDS at the end. A step is a chain of
 // LDS reads, matrix instructions and exponentials that one wavefront a SIMD does not fill (4 x 256 rows of 8
-// heads x 64 over up to 512 keys, fp32: 26 -> 21.5 us; the same keys split over workgroups instead cost a
+// heads x 64 over up to 1024 keys, fp32: 26 -> 21.5 us; the same keys split over workgroups instead cost a
 // merging launch, 31 us).
 constexpr int kQ4WideWaves = 4;  // column tiles of a workgroup
 constexpr int kQ4Ring = 3;
@@ -664,9 +664,10 @@ __global__ __launch_bounds__(64 * kQ4WideWaves * HALVES, HALVES == 2 ? 2 : 3) vo
 // A batch's loads are all issued before its products, and K's registers are filled again while the second
 // product runs: 16 KB and more in flight per wavefront.
 //
-// Bound by memory: 16 requests of 8k to 16k keys, 32 heads x 128 bf16, 577 MB read: 111 us, 5.2 TB/s (one column
-// of rows repeated sixteen times instead: 370 us; batches of one page: 227 us). 64 requests of 32 over 8 heads
-// to 16k with totals: 339 MB read, 41 MB of scores written, 85 us, 4.5 TB/s.
+// Bound by memory: 16 requests of 512 to 32768 keys, 32 heads x 128 bf16, 577 MB read: 108 us, 5.3 TB/s (a page at
+// a time, its softmax repeated in every column, took 370 us where pages batched over the columns took 176).
+// 64 requests of 32 over 8 heads of 512 to 16384 keys with totals: 339 MB read, 41 MB of scores written, 85 us,
+// 4.5 TB/s.
 // ---------------------------------------------------------------------------------------------
 template <int N>
 __device__ __forceinline__ uint32_t row_from(uint32_t x) {  // lane c of a 16-lane row: lane (c + N) % 16
@@ -1069,8 +1070,8 @@ __device__ __forceinline__ void q4_row_state(const float* rec, int splits, int l
 // kernel left in the workspace. The first `merges` workgroups merge, one wavefront per row; of the others each
 // adds kQ4FinishKeys keys' weights of one KV head, having formed its rows' denominators from the records by itself (a
 // launch less than in two steps). A block that two rows of the page table share is added to by both, hence
-// the atomic; otherwise each slot gets one addition. 64 requests of 32 over 8 heads to 16k keys: 42 MB of scores
-// and 10 MB of records and totals, 21 us, bound by the records that every workgroup reads again.
+// the atomic; otherwise each slot gets one addition. 64 requests of 32 over 8 heads of 512 to 16384 keys: 42 MB of
+// scores and 10 MB of totals, 21 us, bound by the records that every workgroup reads again.
 constexpr int kQ4FinishKeys = 1024;  // (256, a key per thread, repeated the denominators too often: 34 -> 20 us)
 
 template <typename IO, int HD>
@@ -1281,14 +1282,19 @@ static Q4Plan q4_plan(int io_dtype, int32_t batch, int32_t heads, int32_t kv_hea
   const int rpt = p.parts == 2 ? 8 : 16;
   p.rows = (int64_t)query_len * (heads / kv_heads);
   // More rows than two tiles: the wide kernel. Up to there the narrow one, whose tiles each read the keys for
-  // themselves, but for bf16 at head_dim 128, where more than four rows leave it batches of two pages: there from
-  // 512 keys on the wide one again, for one tile while it gives a CU at most one workgroup. 8 requests of
-  // 32 over 4 heads (8 rows), 512 / 2048 / 8192 keys: 13.9 / 22.9 / 31.0 -> 13.7 / 14.2 / 22.5 us; 64 of 48 over 8 (6 rows):
-  // 26.8 / 66.9 / 161 -> 19.8 / 57.8 / 208; 24 rows of 8 x 8 units, 512 / 1024 / 8192: 20.7 / 25.3 / 64.2 -> 15.6 / 17.4 /
-  // 41.3, at 128 7.8 -> 8.3; at head_dim 64 7.5 / 10.3 / 28.0 -> 12.5 / 13.5 / 27.2; fp32, 16 rows: 11.4 / 16.7 / 60.8 -> 17.4 /
-  // 18.9 / 53.8.
-  const bool early = p.parts == 1 && head_dim == 128 && p.rows > 4 && max_pages >= 32 && (!weights || query_len > 1 || (int64_t)batch * kv_heads * max_pages <= 16384) &&
-                     (p.rows > rpt || (int64_t)batch * kv_heads <= pa_host::device_cu_count());
+  // themselves, but for bf16 at head_dim 128, where more than four rows leave it batches of two pages: there the
+  // wide one from 512 keys on, for one tile while it gives a CU at most one workgroup. Narrow -> wide in us:
+  //   8 requests x 4 KV heads x 8 rows, 512 / 2048 / 8192 keys   13.9 / 22.9 / 31.0 -> 13.7 / 14.2 / 22.5
+  //   64 x 8 x 6 rows                                           26.8 / 66.9 / 161 -> 19.8 / 57.8 / 208
+  //   8 x 8 x 24 rows, 512 / 1024 / 8192 (128: 7.8 -> 8.3)       20.7 / 25.3 / 64.2 -> 15.6 / 17.4 / 41.3
+  //   the same at head_dim 64                                  7.5 / 10.3 / 28.0 -> 12.5 / 13.5 / 27.2
+  //   8 x 8 x 16 rows, fp32                                    11.4 / 16.7 / 60.8 -> 17.4 / 18.9 / 53.8
+  // A decode step's totals come from the narrow kernel's scores at a lower price than from scores formed again,
+  // once there are many: 64 x 1 x 16 rows, 2048 / 8192 keys 38 / 50 -> 27 / 54.
+  const int64_t heads_of_all = (int64_t)batch * kv_heads;
+  const bool early = p.parts == 1 && head_dim == 128 && p.rows > 4 && max_pages >= 32 &&
+                     (p.rows > rpt || heads_of_all <= pa_host::device_cu_count()) &&
+                     (!weights || query_len > 1 || heads_of_all * max_pages <= 16384);
   p.wide = p.rows > 2 * rpt || early;
   p.rows_per_tile = p.wide ? kQ4WideWaves * rpt : rpt;
   p.tiles = (int)((p.rows + p.rows_per_tile - 1) / p.rows_per_tile);
