@@ -112,7 +112,10 @@ def _device_memory(device) -> dict:
 
 
 def _kv_bytes_per_token(model) -> int:
-    """KV bytes one token occupies over all layers (K and V rows of d_model elements)."""
+    """KV bytes one token occupies over all layers (K and V rows of d_model elements, or 4-bit rows)."""
+    pools = getattr(model, "layer_block_pools", None) or ()
+    if any(p.is_q4 and p.k_blocks is not None for p in pools):
+        return sum(p.token_bytes() for p in pools)
     elem = next(model.parameters()).element_size()
     return 2 * len(model.blocks) * model.blocks[0].attn.d_model * elem
 

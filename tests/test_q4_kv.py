@@ -160,3 +160,15 @@ def test_model_refusals():
         _model(kv_cache_dtype="int8")
     with pytest.raises(ValueError, match="track_attention_weights"):
         _model(track_attention_weights=True)
+
+
+def test_step_events_count_4_bit_bytes():
+    from src.serving.continuous_generate import run_prefill_chunk
+    from src.serving.request import InferenceRequest
+
+    model = _model(kv_cache_dtype="int4", track_attention_weights=True)
+    requests = [InferenceRequest(i, 0.0, n, 4, torch.arange(n)) for i, n in enumerate((12, 7))]
+    event = run_prefill_chunk(model, requests, 16, "cpu", 0.0, 0)
+    # 5 padded rows; a token takes 2 x 36 bytes and its total in each of 2 heads and 2 layers
+    assert event["padding_waste_tokens"] == 5
+    assert event["padding_waste_bytes_est"] == 5 * 2 * 2 * (2 * 36 + 4)
