@@ -25,8 +25,8 @@ size_t pa_q4_page_bytes(int32_t head_dim);
 
 /*
  * Quantising append: rows k_new[b, h, j, :], v_new[b, h, j, :] into slot slot_mapping[b * query_len + j]
- * (as pa_kv_append; negative slots and blocks outside the pool are skipped, two rows of one slot leave
- * either). Per group, values clamped to +-65504: s = half((hi - lo) / 15), z = half((hi + lo) / 2), the
+ * (as pa_kv_append; negative slots and blocks outside the pool are skipped, two rows of one slot in
+ * a call leave parts of both). Per group, values clamped to +-65504: s = half((hi - lo) / 15), z = half((hi + lo) / 2), the
  * difference, the sum and their products with 1/15 and 1/2 rounded to fp32 first; c = (x - z) / s + 7.5
  * rounded to the nearest, ties to even, exactly, in 0..15 (0 where s is 0). A centre of zero is +0. A group with a NaN gets NaN
  * for s and z. weights: the written slots' totals are cleared.
