@@ -546,9 +546,11 @@ __global__ __launch_bounds__(64 * kQ4WideWaves * HALVES, HALVES == 2 ? 2 : 3) vo
   q4_setup<IO, HD, PARTS>(a, u.b, u.hk, tile, L, C, keys, lane, w);
   if (a.q_ops != nullptr && u.split == 0 && half == 0) {  // for q4_chunk_weights_kernel
     const int64_t at = ((int64_t)u.b * a.Hk + u.hk) * a.op_tiles + tile;
+    // (padding may hold NaN and infinities: as zeros there)
+    const bool pad = (int64_t)q4_row<PARTS>(tile, c) >= (int64_t)(C < a.T ? C : a.T) * a.group;
 #pragma unroll
-    for (int s = 0; s < HD / 32; ++s) a.q_ops[(at * (HD / 32) + s) * 64 + lane] = w.q[s];
-    a.q_aux[at * 64 + lane] = f32x4{w.qs[0], w.qs[G - 1], w.sc, __int_as_float(w.n)};
+    for (int s = 0; s < HD / 32; ++s) a.q_ops[(at * (HD / 32) + s) * 64 + lane] = pad ? f16x8{} : w.q[s];
+    a.q_aux[at * 64 + lane] = f32x4{pad ? 0.f : w.qs[0], pad ? 0.f : w.qs[G - 1], w.sc, __int_as_float(w.n)};
   }
 
   if (p0 < p1) {
@@ -1217,10 +1219,11 @@ __global__ __launch_bounds__(64 * kQ4SumWaves) void q4_chunk_weights_kernel(cons
     } else {
       Q4Wave<HD, PARTS> w;
       q4_setup<IO, HD, PARTS>(a, b, hk, tile, L, C, keys, lane, w);
+      const bool pad = q4_row<PARTS>(tile, c) >= real;
 #pragma unroll
-      for (int s = 0; s < W; ++s) q[s] = w.q[s];
+      for (int s = 0; s < W; ++s) q[s] = pad ? f16x8{} : w.q[s];
 #pragma unroll
-      for (int k = 0; k < G; ++k) qs[k] = w.qs[k];
+      for (int k = 0; k < G; ++k) qs[k] = pad ? 0.f : w.qs[k];
       sc = w.sc;
       n = w.n;
       load(tile + STEP);

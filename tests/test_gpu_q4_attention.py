@@ -340,3 +340,27 @@ def test_groups_over_long_contexts(device, dtype, hd, T):
     blocks = sum(-(-n // 16) for n in lens) + 2
     kp, vp = filled_pools(rng, blocks, 2, hd)
     _check(device, rng, dtype, 16, 2, hd, T, lens, cur, kp, vp, tables(rng, lens, blocks))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("garbage", [float("nan"), float("inf")])
+@pytest.mark.parametrize("heads, T", [((4, 2), 3), ((4, 2), 12), ((8, 1), 80)], ids=str)
+def test_padded_rows_may_hold_anything(device, dtype, garbage, heads, T):
+    """NaN and infinities in q's rows behind a request's last new token: its real rows and the totals are those of
+    any other padding."""
+    rng = np.random.default_rng(T)
+    lens, cur = [T + 60, 40, 5], [T, 2, 0]
+    kp, vp = filled_pools(rng, 20, heads[1], 64)
+    table = tables(rng, lens, 20)
+    dk, dv = torch.from_numpy(kp).to(device), torch.from_numpy(vp).to(device)
+    q, _ = to_q(rng, (3, heads[0], T, 64), dtype)
+    outs, sums = [], []
+    for fill in (0.0, garbage):
+        for b, n in enumerate(cur):
+            q[b, :, n:] = fill
+        totals = torch.zeros(20, heads[1], 16, device=device)
+        outs.append(_call(device, q, dk, dv, table, lens, cur, totals))
+        sums.append(totals)
+    assert torch.equal(sums[0], sums[1])
+    for b, n in enumerate(cur):
+        assert torch.equal(outs[0][b, :, :n], outs[1][b, :, :n])
