@@ -84,3 +84,36 @@ def test_calls_of_nothing(device, native, monkeypatch):
     kept, lens = kq.evict_q4_hip(k, v, totals, table, none, torch.empty(0, 1, dtype=torch.int32, device=device), keep=4, window=1)
     assert kept.shape == (0, 2, 4) and lens.shape == (0,)
     assert all(torch.equal(a, b) for a, b in zip(was, (k, v, totals)))
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_output_over_the_queries_is_refused(device, native, monkeypatch):
+    if not native:
+        monkeypatch.setattr(kq, "native_call", lambda: None)
+    k, v, totals, table, L, _ = _state(device, [20, 30])
+    q = torch.randn(2, 4, 3, 64, device=device)
+    with pytest.raises(ValueError, match="out must not be q"):
+        kq.paged_attention_prefill_q4_hip(q, k, v, table, L, L * 0 + 3, weights=totals, out=q)
+
+
+def test_captured_eviction_of_long_tables(device):
+    """More totals than a kernel's default LDS holds, captured and replayed with other totals."""
+    n, keep = 20000, 500
+    k, v, totals, table, L, i32 = _state(device, [n], blocks=1300)
+    free = sorted(set(range(1300)) - set(table.flatten().tolist()))[:32]
+    fresh = i32([free])
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        kq.evict_q4_hip(k, v, totals, table, L, fresh, keep=keep, window=10)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        kept, lens = kq.evict_q4_hip(k, v, totals, table, L, fresh, keep=keep, window=10)
+    for seed in range(3):
+        totals.copy_(torch.rand(totals.shape, generator=torch.Generator().manual_seed(seed)))
+        state = [x.clone() for x in (k, v, totals)]
+        graph.replay()
+        torch.cuda.synchronize()
+        want, want_lens = kq.evict_q4_hip(*state, table, L, fresh, keep=keep, window=10)
+        assert torch.equal(kept, want) and torch.equal(lens, want_lens)
+        assert all(torch.equal(a, b) for a, b in zip(state, (k, v, totals)))
