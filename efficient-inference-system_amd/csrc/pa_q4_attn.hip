@@ -666,7 +666,7 @@ __global__ __launch_bounds__(64 * kQ4WideWaves * HALVES, HALVES == 2 ? 2 : 3) vo
 // A batch's loads are all issued before its products, and K's registers are filled again while the second
 // product runs: 16 KB and more in flight per wavefront.
 //
-// Bound by memory: 16 requests of 512 to 32768 keys, 32 heads x 128 bf16, 577 MB read: 108 us, 5.3 TB/s (a page at
+// Bound by memory: 16 requests of 512 to 32768 keys, 32 heads x 128 bf16, 577 MB read: 106 us, 5.4 TB/s (a page at
 // a time, its softmax repeated in every column, took 370 us where pages batched over the columns took 176).
 // 64 requests of 32 over 8 heads of 512 to 16384 keys with totals: 339 MB read, 41 MB of scores written, 85 us,
 // 4.5 TB/s.
