@@ -1142,10 +1142,11 @@ __global__ __launch_bounds__(256) void q4_finish_kernel(const Q4Args a, int64_t 
 
 // Totals of a chunk: the scores formed again, PG pages per workgroup whose operands and pairs stay in registers;
 // the workgroup's wavefronts take the row tiles in turn, the next tile's operands on their way, and their
-// sums meet in LDS in a fixed order; or (EACH) every wavefront has pages of its own and takes all tiles. READY: the tiles' q operands are in the workspace, left by the wide
-// kernel (formed here they cost as much as the scores). A block that two rows of the page table share is
-// added to by both, hence the atomic; otherwise each slot gets one addition. Bound by vector instructions, 170
-// to 16 matrix instructions a tile: 200 rows of 32 over 8 heads x 128 bf16 over 16.5k keys 72 us (370 TFLOP/s).
+// sums meet in LDS in a fixed order; or (EACH) every wavefront has pages of its own and takes all tiles. READY:
+// the tiles' q operands are in the workspace, left by the wide kernel (formed here they cost as much as the
+// scores). A block that two rows of the page table share is added to by both, hence the atomic; otherwise
+// each slot gets one addition. Bound by vector instructions, 170 to 16 matrix instructions a tile: 200 rows of 32
+// over 8 heads x 128 bf16 over 16.5k keys 72 us (370 TFLOP/s).
 constexpr int kQ4SumWaves = 8;
 
 template <typename IO, int HD, int PARTS, bool READY, int PG, bool EACH>

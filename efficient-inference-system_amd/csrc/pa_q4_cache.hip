@@ -19,7 +19,7 @@ struct Q4RowArgs {
 // consecutive tokens of one head, K and V, so that the row's place is scalar arithmetic but for the token,
 // and a page, whose bytes interleave its tokens, is written by one workgroup or two. Otherwise (decode steps)
 // rows follow each other, and K and V are the halves of the grid's y axis (in that order, with its divisions in
-// every lane, 4 x 512 rows of 32 heads x 128 bf16 were read in 12.6 us, not 9.8).
+// every lane, 4 x 512 rows of 32 heads x 128 bf16 are read in 12.6 us, not 9.8).
 struct Q4Row {
   int h, e;        // head, and which eight values
   uint32_t b, j;   // request and token; j >= T: no row
@@ -298,7 +298,8 @@ static int check_rows(const char* what, const void* k, const void* v, int dtype,
   PA_CHECK_ARG(num_blocks == 0 || (k_pool && v_pool), "%s: null pool", what);
   PA_CHECK_ARG(((reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(v_pool)) & 15) == 0,
                "%s: the pools must be 16-byte aligned", what);
-  PA_CHECK_ARG((int64_t)batch * rows <= 0x7fffffffLL && row_workgroups(batch, rows, heads, head_dim) <= 0x7fffff00LL / 256, "%s: too many rows in one call", what);
+  PA_CHECK_ARG((int64_t)batch * rows <= 0x7fffffffLL && row_workgroups(batch, rows, heads, head_dim) <= 0x7fffff00LL / 256,
+               "%s: too many rows in one call", what);
   return PA_OK;
 }
 
