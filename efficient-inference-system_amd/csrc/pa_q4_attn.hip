@@ -1418,7 +1418,6 @@ extern "C" int pa_q4_attention(const void* q, int64_t q_stride_b, int64_t q_stri
     PA_FAIL(PA_ERR_UNSUPPORTED, "pa_q4_attention: no 4-bit pages for head_dim %d (64 and 128)", head_dim);
   if (batch == 0 || query_len == 0) return PA_OK;
   PA_CHECK_ARG(q && out && seq_lens && cur_lens, "pa_q4_attention: null q/out/seq_lens/cur_lens");
-  PA_CHECK_ARG(q != out, "pa_q4_attention: out must not be q (a chunk's totals read q after the rows are written)");
   if (max_pages > 0) {
     PA_CHECK_ARG(page_table != nullptr && pt_stride >= max_pages, "pa_q4_attention: page table missing or stride < max_pages");
     PA_CHECK_ARG(k_pool && v_pool && num_blocks > 0, "pa_q4_attention: KV pool missing or empty");
@@ -1434,6 +1433,7 @@ extern "C" int pa_q4_attention(const void* q, int64_t q_stride_b, int64_t q_stri
   if (p.bytes && (workspace == nullptr || workspace_bytes < p.bytes))
     PA_FAIL(PA_ERR_WORKSPACE, "pa_q4_attention: workspace too small: need %zu bytes, have %zu", p.bytes, workspace_bytes);
   PA_CHECK_ARG((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "pa_q4_attention: the workspace must be 16-byte aligned");
+  PA_CHECK_ARG(q != out, "pa_q4_attention: out must not be q (a chunk's totals read q after the rows are written)");
 
   Q4Args a{};
   a.q = q; a.q_sb = q_stride_b; a.q_sh = q_stride_h; a.q_st = q_stride_t;
