@@ -38,8 +38,6 @@ BLOCK, GROUP = 16, 64
 DTYPES = {"fp32": torch.float32, "bf16": torch.bfloat16}
 DEV = "cuda"
 HALF_MAX = 65504.0
-PACKAGE = str(Path(__file__).resolve().parents[1] / "efficient-inference-system_amd")
-_kernels = None  # the package's 4-bit operators, once `own` has asked for them
 
 
 # ---------------------------------------------------------------------------------------------
@@ -302,17 +300,13 @@ def run(st):
     return {"append": _append, "decode": _attend, "prefill": _attend, "evict": _evict}[case["kind"]](st)
 
 
-def _own_kernels():
-    global _kernels
-    if _kernels is None:
-        sys.path.insert(0, PACKAGE)
-        from src.kernels import hip_q4_attention
-        _kernels = hip_q4_attention
-    return _kernels
-
-
 def _run_own(kind, st):
-    q4, case = _own_kernels(), st["case"]
+    path = str(Path(__file__).resolve().parents[1] / "efficient-inference-system_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    from src.kernels import hip_q4_attention as q4
+
+    case = st["case"]
     if kind == "append":
         q4.kv_append_q4_hip(st["k"], st["v"], st["k_pool"], st["v_pool"], st["slots"])
         return q4.kv_read_q4_hip(st["k_pool"], st["v_pool"], st["slots"], batch=case["batch"], dtype=DTYPES[case["io"]])
