@@ -52,6 +52,7 @@ only if a storage is reallocated. Set PAGED_HIP_GRAPHS=0 to run the eager forwar
 """
 from __future__ import annotations
 
+import gc
 import math
 import os
 import weakref
@@ -360,9 +361,18 @@ class _Captured:
         self.desc.close()
 
 
+def _no_runner() -> None:
+    return None
+
+
 class GraphedStep:
+    """A model's captured steps. The model owns its runner, so the runner refers to it weakly: a dropped model
+    and its graphs go at once, not when a cyclic collection finds them. Such a collection may fall inside a
+    later capture, where destroying a graph (it waits for the device, which a capture forbids) ends the process.
+    A copied or unpickled model has no runner and makes its own."""
+
     def __init__(self, model):
-        self.model = model
+        self._model = weakref.ref(model)
         self.captured: dict[tuple[int, int, bool], _Captured] = {}
         self.captures = 0
         self._attns = None
@@ -370,6 +380,16 @@ class GraphedStep:
         # the embedding weight, read per call only for its device (a Parameter keeps its identity
         # across .to() and load_state_dict)
         self._weight = model.token_emb.weight
+
+    @property
+    def model(self):
+        return self._model()
+
+    def __deepcopy__(self, memo) -> None:
+        return None
+
+    def __reduce__(self):
+        return _no_runner, ()
 
     def usable(self, input_ids, kv_caches) -> bool:
         """Whether a step over input_ids ([B, T], device tensor or host data) and these per-layer
@@ -487,8 +507,16 @@ class GraphedStep:
         # Each graph keeps its own private memory pool (a step's intermediates are small), so
         # dropping graphs never leaves a shared pool half-released.
         g = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(g):
-            cap.logits = self._static_forward(cap, pools)
+        # The capture allocates enough to start a cyclic collection, and what that finds may own device objects
+        # (a caller's graphs, pinned memory), whose release is illegal while a capture runs.
+        collecting = gc.isenabled()
+        gc.disable()
+        try:
+            with torch.cuda.graph(g):
+                cap.logits = self._static_forward(cap, pools)
+        finally:
+            if collecting:
+                gc.enable()
         cap.graph = g
         self.captures += 1
 
