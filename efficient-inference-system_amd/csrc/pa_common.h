@@ -5,6 +5,8 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <mutex>
+
 #include "paged_hip.h"
 
 namespace pa {
@@ -172,6 +174,9 @@ namespace pa_host {
 void set_error(const char* fmt, ...);
 void clear_error();
 int device_cu_count();  // compute units of the current device (cached per device)
+// Held over the launches of a call that hand data on through a workspace. Threads that share a stream share
+// its workspace: without it a second thread's first launch may come between a call's launches.
+std::mutex& workspace_mutex(const void* workspace);
 }  // namespace pa_host
 
 #define PA_FAIL(code, ...)                \

@@ -1456,6 +1456,7 @@ extern "C" int pa_q4_attention(const void* q, int64_t q_stride_b, int64_t q_stri
   a.q_aux = reinterpret_cast<f32x4*>(ops + p.ops);
   a.op_tiles = p.op_tiles;
   hipStream_t stream = static_cast<hipStream_t>(stream_);
+  const std::lock_guard<std::mutex> whole(pa_host::workspace_mutex(workspace));
   if (io_dtype == PA_DTYPE_F32) {
     if (head_dim == 64) launch_q4<float, 64, 2>(a, p, stream); else launch_q4<float, 128, 2>(a, p, stream);
   } else {

@@ -32,6 +32,13 @@ int device_cu_count() {
   return cached[dev];
 }
 
+// (Workspaces of at least 1 MiB, as the wrappers make them, fall on mutexes of their own; others may share one,
+// and then wait for each other's launches.)
+std::mutex& workspace_mutex(const void* workspace) {
+  static std::mutex all[64];
+  return all[(reinterpret_cast<uintptr_t>(workspace) >> 20) % 64];
+}
+
 }  // namespace pa_host
 
 extern "C" unsigned long long paged_internal_capture_id(void* stream) {

@@ -52,8 +52,9 @@ int pa_q4_read(const void* k_pool, const void* v_pool, int64_t num_blocks, const
  * key, the sum of its softmax weights over the KV head's query heads and the real rows (i < C) is added to
  * its slot's total (a block in several rows of the page table gets the sum of all, in no fixed order).
  * scale must be positive, and out must not overlap q. The workspace (16-byte aligned, pa_q4_attention_workspace_size bytes for the
- * same arguments, weights != 0 where totals are asked for) needs no initial state and keeps none; calls
- * that share one must not run concurrently.
+ * same arguments, weights != 0 where totals are asked for) needs no initial state and keeps none. Calls on one
+ * stream may share one, from several threads too (a call's launches follow each other undivided); calls
+ * on several streams must not.
  */
 int pa_q4_attention(const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t,
                     void* out, int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_t, int io_dtype,
