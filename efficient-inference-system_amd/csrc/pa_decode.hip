@@ -964,11 +964,14 @@ static int decode_entry(const void* q, int64_t q_stride_b, int64_t q_stride_h,
   if (((int64_t)batch + kXcds) * num_heads * nsplit > 0x7fffffffLL)
     PA_FAIL(PA_ERR_INVALID_ARGUMENT, "grid too large");
 
+  const bool merged = gangs == 0 && nsplit > 1 && a.counters == nullptr;  // by a second launch
+  std::unique_lock<std::mutex> whole;
+  if (merged) whole = std::unique_lock<std::mutex>(pa_host::workspace_mutex(workspace));
   const bool ok = io_dtype == PA_DTYPE_F32 ? dispatch_decode_fast_io<float>(a, kv_dtype, stream)
                                            : dispatch_decode_fast_io<uint16_t>(a, kv_dtype, stream);
   if (!ok) PA_FAIL(PA_ERR_UNSUPPORTED, "no decode kernel for head_dim %d", head_dim);
   PA_CHECK_LAUNCH("decode kernel");
-  if (gangs == 0 && nsplit > 1 && a.counters == nullptr) {
+  if (merged) {
     const dim3 grid((unsigned)((int64_t)batch * num_heads)), block(kWave);
     if (io_dtype == PA_DTYPE_F32)
       decode_merge_kernel<float><<<grid, block, 0, stream>>>(a);

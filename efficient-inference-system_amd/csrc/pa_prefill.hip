@@ -817,6 +817,8 @@ extern "C" int pa_prefill(const void* q, int64_t q_stride_b, int64_t q_stride_h,
   }
   if (units * nsplit > 0x7fffffffLL) PA_FAIL(PA_ERR_INVALID_ARGUMENT, "grid too large");
   const dim3 grid((unsigned)(units * nsplit));
+  std::unique_lock<std::mutex> whole;  // a split call's two launches
+  if (nsplit > 1) whole = std::unique_lock<std::mutex>(pa_host::workspace_mutex(workspace));
   bool ok;
   if (kv_dtype == PA_DTYPE_F32)
     ok = io_dtype == PA_DTYPE_F32 ? dispatch_prefill_io<float, float>(a, grid, stream)

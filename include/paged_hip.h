@@ -100,7 +100,7 @@ int pa_decode(const void* q, int64_t q_stride_b, int64_t q_stride_h,
  * not apply;
  * otherwise 0 when split_blocks == 0 or no request can need more than one split, else
  * PA_DECODE_COUNTER_BYTES + 4 * batch * num_heads * splits * (head_dim + 2)). No reference counterpart: the Triton decode path has no split-K.
- * Calls that share a workspace must not run concurrently (e.g. on different streams). */
+ * Calls on one stream may share a workspace, from several threads too; calls on several streams must not. */
 size_t pa_decode_workspace_size(int32_t batch, int32_t num_heads, int32_t head_dim,
                                 int32_t max_pages, int32_t split_blocks);
 
@@ -121,7 +121,7 @@ size_t pa_decode_workspace_size(int32_t batch, int32_t num_heads, int32_t head_d
  * (pa_decode_workspace_size: the counters and the records) exceeds the array fails with
  * PA_ERR_INVALID_ARGUMENT before any launch. The array starts at zero when the library is loaded
  * and every call leaves its counters zero, but every call on a device shares that device's
- * array: calls that overlap on one device (e.g. on two streams) race and must be serialised.
+ * array: calls that overlap on one device (on two streams) race and must be serialised.
  */
 int pa_decode_noalloc(const void* q, int64_t q_stride_b, int64_t q_stride_h,
                       void* out, int64_t out_stride_b, int64_t out_stride_h, int io_dtype,
@@ -154,8 +154,8 @@ int pa_decode_noalloc(const void* q, int64_t q_stride_b, int64_t q_stride_h,
  * PAGED_HIP_PREFILL_BALANCE=force takes it wherever it can run (as many workgroups per compute
  * unit as fit on larger grids), =off never. Every prefill workspace starts with
  * PA_PREFILL_COUNTER_BYTES of arrival counters that must be zero before its first use; every call
- * leaves them zero. Calls that
- * share a workspace must not run concurrently (e.g. on different streams).
+ * leaves them zero. Calls on
+ * one stream may share a workspace, from several threads too; calls on several streams must not.
  */
 int pa_prefill(const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t,
                void* out, int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_t,

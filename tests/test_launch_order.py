@@ -29,6 +29,9 @@ def stub(tmp_path_factory):
     ("q4 chunk with totals", 2),
     ("q4 decode over ranges of keys", 2),
     ("q4 decode over ranges of keys, with totals", 2),
+    ("split prefill", 2),
+    ("split decode", 2),
+    ("split decode in the library's scratch", 2),
 ])
 def test_a_calls_launches_are_not_divided(stub, name, launches):
     run = subprocess.run([sys.executable, str(HERE / "launch_order_calls.py"), str(stub), name], capture_output=True,
