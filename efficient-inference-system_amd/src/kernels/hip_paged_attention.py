@@ -28,6 +28,7 @@ except ImportError:  # not built: the Python versions run
 
 _workspaces: dict[tuple[int, str], torch.Tensor] = {}
 _retired_workspaces: list[torch.Tensor] = []
+_workspaces_lock = threading.Lock()
 # Workspaces off the default stream: (device, stream, kind) -> (capture, tensor), the latest used last.
 _stream_workspaces: dict[tuple[int, int, str], tuple[int, torch.Tensor]] = {}
 _stream_workspaces_lock = threading.Lock()
@@ -90,12 +91,13 @@ def _workspace(device: torch.device, nbytes: int, kind: str) -> torch.Tensor:
     and the kinds are kept apart (their layouts differ). A workspace replaced by a larger one stays allocated
     for the life of the process: a HIP graph a caller captured may hold its address."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
-    ws = _workspaces.get((idx, kind))
-    if ws is None or ws.numel() < nbytes:
-        if ws is not None:
-            _retired_workspaces.append(ws)
-        ws = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
-        _workspaces[(idx, kind)] = ws
+    with _workspaces_lock:  # (a second thread's allocation would replace, and free, the first one's)
+        ws = _workspaces.get((idx, kind))
+        if ws is None or ws.numel() < nbytes:
+            if ws is not None:
+                _retired_workspaces.append(ws)
+            ws = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
+            _workspaces[(idx, kind)] = ws
     return ws
 
 
