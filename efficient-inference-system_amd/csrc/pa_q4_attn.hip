@@ -1163,9 +1163,11 @@ __global__ __launch_bounds__(64 * kQ4SumWaves) void q4_chunk_weights_kernel(cons
   const int keys = L < a.max_pages * kQ4Tokens ? L : a.max_pages * kQ4Tokens;
   if (key0 >= keys || C < 1) return;
   const int rows = a.T * a.group, real = (C < a.T ? C : a.T) * a.group;  // rows behind `real` are padding
-  // the first row that sees the first of these keys: key0 < L - C + 1 + i
-  int i0 = key0 - (L - C);
+  // the first row that sees the first of these keys: key0 < L - C + 1 + i. Where none does (more new tokens
+  // claimed than there are keys and rows), its tile's operands need not be there.
+  int64_t i0 = (int64_t)key0 - ((int64_t)L - C);
   i0 = i0 > 0 ? i0 : 0;
+  if (i0 >= a.T) return;
   const int32_t* table = a.page_table + (int64_t)b * a.pt_stride;
   int id[PG];
   f16x8 kf[PG][W];
@@ -1202,7 +1204,7 @@ __global__ __launch_bounds__(64 * kQ4SumWaves) void q4_chunk_weights_kernel(cons
       next_aux = a.q_aux[at * 64 + lane];
     }
   };
-  int tile = (int)((int64_t)i0 * a.group / ROWS) + (EACH ? 0 : wave);
+  int tile = (int)(i0 * a.group / ROWS) + (EACH ? 0 : wave);
   if (tile * ROWS < real) load(tile);
   for (; tile * ROWS < real; tile += STEP) {
     f16x8 q[W];
