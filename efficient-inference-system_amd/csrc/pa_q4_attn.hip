@@ -546,11 +546,11 @@ __global__ __launch_bounds__(64 * kQ4WideWaves * HALVES, HALVES == 2 ? 2 : 3) vo
   q4_setup<IO, HD, PARTS>(a, u.b, u.hk, tile, L, C, keys, lane, w);
   if (a.q_ops != nullptr && u.split == 0 && half == 0) {  // for q4_chunk_weights_kernel
     const int64_t at = ((int64_t)u.b * a.Hk + u.hk) * a.op_tiles + tile;
-    // (padding may hold NaN and infinities: as zeros there)
+    // (padding may hold NaN and infinities: as zeros there, and it sees no key, whose values may be NaN too)
     const bool pad = (int64_t)q4_row<PARTS>(tile, c) >= (int64_t)(C < a.T ? C : a.T) * a.group;
 #pragma unroll
     for (int s = 0; s < HD / 32; ++s) a.q_ops[(at * (HD / 32) + s) * 64 + lane] = pad ? f16x8{} : w.q[s];
-    a.q_aux[at * 64 + lane] = f32x4{pad ? 0.f : w.qs[0], pad ? 0.f : w.qs[G - 1], w.sc, __int_as_float(w.n)};
+    a.q_aux[at * 64 + lane] = f32x4{pad ? 0.f : w.qs[0], pad ? 0.f : w.qs[G - 1], w.sc, __int_as_float(pad ? 0 : w.n)};
   }
 
   if (p0 < p1) {
@@ -1228,7 +1228,7 @@ __global__ __launch_bounds__(64 * kQ4SumWaves) void q4_chunk_weights_kernel(cons
 #pragma unroll
       for (int k = 0; k < G; ++k) qs[k] = pad ? 0.f : w.qs[k];
       sc = w.sc;
-      n = w.n;
+      n = pad ? 0 : w.n;
       load(tile + STEP);
     }
     auto add = [&](auto masked) {

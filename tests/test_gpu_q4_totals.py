@@ -1,5 +1,5 @@
 """Running totals of 4-bit attention where they can go wrong: workspaces full of rubbish, rows that see nothing beside
-long requests."""
+long requests, keys that no row sees."""
 import numpy as np
 import pytest
 import torch
@@ -73,3 +73,23 @@ def test_the_largest_claim(device, dtype, heads, T):
     kp, vp = filled_pools(rng, 140, heads[1], 64)
     q, qd = to_q(rng, (2, heads[0], T, 64), dtype)
     _check(device, q, qd, kp, vp, tables(rng, lens, 140), lens, cur, 64)
+
+
+@DTYPES
+@SHAPES
+def test_keys_behind_the_last_rows_view_may_hold_anything(device, dtype, heads, T, width):
+    """A request that claims more new tokens than the call has rows: the keys that its last row does not see are
+    NaN, and nothing of them reaches the totals."""
+    rng = np.random.default_rng(T + width)
+    lens, over = [T + 60, T + 30], [21, 4]
+    cur = [T + n for n in over]  # row i sees L - over - T + 1 + i keys
+    blocks = sum(-(-n // 16) for n in lens) + 2
+    kp, vp = filled_pools(rng, blocks, heads[1], 64)
+    table = tables(rng, lens, blocks, width=width)
+    clean = kp.copy(), vp.copy()
+    for b, n in enumerate(lens):
+        for t in range(n - over[b], n):
+            for pool in (kp, vp):
+                poison(pool, 64, table[b, t // 16], t % 16)
+    q, qd = to_q(rng, (2, heads[0], T, 64), dtype)
+    _check(device, q, qd, kp, vp, table, lens, cur, 64, clean)
