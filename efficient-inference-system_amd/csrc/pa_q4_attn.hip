@@ -455,6 +455,11 @@ __device__ __forceinline__ float* q4_lse(const Q4Args& a, int b, int hk, int row
   return a.lse + ((int64_t)b * a.Hk + hk) * a.T * a.group + row;
 }
 
+// log2 of a row's denominator: infinite (its weights 2^-inf are 0) where the row sees no key, NaN where it met one.
+__device__ __forceinline__ float q4_log_sum(float M, float l) {
+  return l > 0.f || l != l ? M + __builtin_amdgcn_logf(l) : INFINITY;
+}
+
 // Workgroup -> (request, KV head, tile, split): KV heads innermost, so that workgroups of one moment
 // read neighbouring slabs of the same blocks; later (longer) tiles first.
 struct Q4Unit { int b, hk, tile, split; };
@@ -650,7 +655,7 @@ __global__ __launch_bounds__(64 * kQ4WideWaves * HALVES, HALVES == 2 ? 2 : 3) vo
     const float f = l > 0.f || l != l ? 1.f / l : 0.f;
 #pragma unroll
     for (int k = 0; k < G; ++k) q4_store16<IO>(out + 64 * k + 16 * g, o[k], f);
-    if (a.lse != nullptr && g == 0) *q4_lse(a, u.b, u.hk, row) = l > 0.f ? w.M + __builtin_amdgcn_logf(l) : INFINITY;
+    if (a.lse != nullptr && g == 0) *q4_lse(a, u.b, u.hk, row) = q4_log_sum(w.M, l);
   }
 }
 
@@ -1026,7 +1031,7 @@ __global__ __launch_bounds__(64 * kQ4Waves, 2) void q4_narrow_kernel(const Q4Arg
       IO* out = static_cast<IO*>(a.out) + (int64_t)u.b * a.o_sb + (int64_t)(u.hk * a.group + j) * a.o_sh + (int64_t)i * a.o_st;
       Elem<IO>::store(out + d, den > 0.f || den != den ? s / den : 0.f);
       if (a.lse != nullptr && d == 0) {
-        const float e = den > 0.f ? top + __builtin_amdgcn_logf(den) : INFINITY;
+        const float e = q4_log_sum(top, den);
         lse_of[r] = e;
         *q4_lse(a, u.b, u.hk, m) = e;
       }
@@ -1104,7 +1109,7 @@ __global__ __launch_bounds__(256) void q4_finish_kernel(const Q4Args a, int64_t 
     IO* out = static_cast<IO*>(a.out) + (int64_t)b * a.o_sb + (int64_t)(hk * a.group + j) * a.o_sh + (int64_t)i * a.o_st;
 #pragma unroll
     for (int e = 0; e < E; ++e) Elem<IO>::store(out + lane + 64 * e, l > 0.f || l != l ? o[e] / l : 0.f);
-    if (a.lse != nullptr && lane == 0) *q4_lse(a, b, hk, row) = l > 0.f ? M + __builtin_amdgcn_logf(l) : INFINITY;
+    if (a.lse != nullptr && lane == 0) *q4_lse(a, b, hk, row) = q4_log_sum(M, l);
     return;
   }
   __shared__ float lse[kQ4MaxNarrow];
@@ -1122,7 +1127,7 @@ __global__ __launch_bounds__(256) void q4_finish_kernel(const Q4Args a, int64_t 
     for (int j = wave; j < a.group; j += 4) {
       float M, l;
       q4_row_state<HD>(q4_record<HD>(a, b, hk, j, 0), splits, lane, M, l);
-      if (lane == 0) lse[j] = l > 0.f ? M + __builtin_amdgcn_logf(l) : INFINITY;
+      if (lane == 0) lse[j] = q4_log_sum(M, l);
     }
   } else if ((int)threadIdx.x < a.group) {
     lse[threadIdx.x] = *q4_lse(a, b, hk, threadIdx.x);

@@ -1,5 +1,5 @@
 """Running totals of 4-bit attention where they can go wrong: workspaces full of rubbish, rows that see nothing beside
-long requests, keys that no row sees."""
+long requests, keys that no row sees, rows that are NaN."""
 import numpy as np
 import pytest
 import torch
@@ -91,5 +91,46 @@ def test_keys_behind_the_last_rows_view_may_hold_anything(device, dtype, heads, 
         for t in range(n - over[b], n):
             for pool in (kp, vp):
                 poison(pool, 64, table[b, t // 16], t % 16)
+    q, qd = to_q(rng, (2, heads[0], T, 64), dtype)
+    _check(device, q, qd, kp, vp, table, lens, cur, 64, clean)
+
+
+@DTYPES
+@pytest.mark.parametrize("heads, T, width", [((4, 2), 1, 8), ((4, 2), 1, 300), ((16, 2), 1, 300), ((40, 1), 1, 40), ((4, 2), 3, 8),
+                                             ((4, 2), 3, 300), ((2, 2), 40, 8), ((2, 2), 40, 130), ((8, 1), 80, 130)], ids=str)
+def test_a_row_that_is_nan_makes_the_totals_of_its_keys_nan(device, dtype, heads, T, width):
+    rng = np.random.default_rng(T + width)
+    lens, cur = [T + 50, T + 30], [T, T]
+    blocks = sum(-(-n // 16) for n in lens) + 2
+    kp, vp = filled_pools(rng, blocks, heads[1], 64)
+    table = tables(rng, lens, blocks, width=width)
+    q, _ = to_q(rng, (2, heads[0], T, 64), dtype)
+    q[0, 1, T // 2, 5] = float("nan")
+    clean = q.clone()
+    clean[0, 1, T // 2, 5] = 0
+    dk, dv = torch.from_numpy(kp).to(device), torch.from_numpy(vp).to(device)
+    want, added = q4.attention(q.double().numpy(), q4.values(kp, 64, True), q4.values(vp, 64, False), table, lens, cur)
+    _, rel = bounds(clean.double().numpy(), kp, vp, 64, np.nan_to_num(want), dtype)
+    totals = torch.zeros(blocks, heads[1], 16, device=device)
+    got = _call(device, q, dk, dv, table, lens, cur, totals).double().cpu().numpy()
+    sums = totals.double().cpu().numpy()
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    assert np.isnan(added).any() and np.array_equal(np.isnan(sums), np.isnan(added))
+    there = ~np.isnan(added)
+    assert (np.abs(sums - added) <= 2.0 ** -23 * added + added * (rel + 2.0 ** -14))[there].all()
+
+
+@DTYPES
+@pytest.mark.parametrize("heads, T, width", [((4, 2), 1, 8), ((4, 2), 1, 300), ((4, 2), 5, 8), ((2, 2), 40, 130)], ids=str)
+def test_a_key_that_is_nan_makes_its_rows_totals_nan(device, dtype, heads, T, width):
+    rng = np.random.default_rng(T + width)
+    lens, cur = [T + 50, T + 30], [T, T]
+    blocks = sum(-(-n // 16) for n in lens) + 2
+    kp, vp = filled_pools(rng, blocks, heads[1], 64)
+    table = tables(rng, lens, blocks, width=width)
+    clean = kp.copy(), vp.copy()
+    at = lens[0] - max(T // 2, 1)  # seen by the chunk's later rows only
+    for pool in (kp, vp):
+        poison(pool, 64, table[0, at // 16], at % 16)
     q, qd = to_q(rng, (2, heads[0], T, 64), dtype)
     _check(device, q, qd, kp, vp, table, lens, cur, 64, clean)
