@@ -1399,6 +1399,55 @@ static void launch_q4(const Q4Args& a, const Q4Plan& p, hipStream_t stream) {
 
 using namespace pa;
 
+namespace {
+// The bytes of [batch, heads, tokens] rows: sizes, strides and a row's length.
+struct Q4Rows {
+  int64_t n[3], stride[3], row;
+};
+
+// Whether offset d is a difference of two rows' places, within a row's length: of its dimensions the one of the
+// largest stride first, whose multiples that leave a remainder in reach of the others are few.
+bool q4_row_apart(const Q4Rows& r, const int (&order)[3], int at, int64_t d) {
+  if (at == 3) return d > -r.row && d < r.row;
+  int64_t reach = r.row - 1;
+  for (int k = at + 1; k < 3; ++k) reach += (r.n[order[k]] - 1) * r.stride[order[k]];
+  const int64_t n = r.n[order[at]], s = r.stride[order[at]];
+  if (n == 1 || s == 0) return q4_row_apart(r, order, at + 1, d);
+  int64_t first = (d - reach) / s - 1, last = (d + reach) / s + 1;
+  first = first > 1 - n ? first : 1 - n;
+  last = last < n - 1 ? last : n - 1;
+  if (last - first > 64) return true;  // (strides that no tensor of separate rows has)
+  for (int64_t k = first; k <= last; ++k)
+    if (q4_row_apart(r, order, at + 1, d - k * s)) return true;
+  return false;
+}
+
+// Whether two sets of rows share a byte. Of sets whose extents meet, those of the same strides are compared
+// exactly (q and out may be interleaved in one tensor); others count as meeting.
+bool q4_rows_meet(const void* a, Q4Rows ra, const void* b, Q4Rows rb) {
+  const auto extent = [](const void* p, const Q4Rows& r, int64_t& lo, int64_t& hi) {
+    lo = hi = (int64_t)reinterpret_cast<uintptr_t>(p);
+    for (int k = 0; k < 3; ++k) (r.stride[k] < 0 ? lo : hi) += (r.n[k] - 1) * r.stride[k];
+    hi += r.row;
+  };
+  int64_t a0, a1, b0, b1;
+  extent(a, ra, a0, a1);
+  extent(b, rb, b0, b1);
+  if (a1 <= b0 || b1 <= a0) return false;
+  for (int k = 0; k < 3; ++k)
+    if (ra.n[k] > 1 && (ra.stride[k] != rb.stride[k] || ra.stride[k] < 0)) return true;
+  int order[3] = {0, 1, 2};
+  for (int i = 0; i < 2; ++i)
+    for (int k = 0; k < 2; ++k)
+      if (ra.stride[order[k]] < ra.stride[order[k + 1]]) {
+        const int t = order[k];
+        order[k] = order[k + 1];
+        order[k + 1] = t;
+      }
+  return q4_row_apart(ra, order, 0, (int64_t)reinterpret_cast<uintptr_t>(b) - (int64_t)reinterpret_cast<uintptr_t>(a));
+}
+}  // namespace
+
 extern "C" size_t pa_q4_attention_workspace_size(int io_dtype, int32_t batch, int32_t num_heads, int32_t kv_heads,
                                                  int32_t query_len, int32_t head_dim, int32_t max_pages, int32_t weights) {
   if (batch <= 0 || num_heads <= 0 || kv_heads <= 0 || num_heads % kv_heads || query_len <= 0 || max_pages <= 0 ||
@@ -1440,7 +1489,12 @@ extern "C" int pa_q4_attention(const void* q, int64_t q_stride_b, int64_t q_stri
   if (p.bytes && (workspace == nullptr || workspace_bytes < p.bytes))
     PA_FAIL(PA_ERR_WORKSPACE, "pa_q4_attention: workspace too small: need %zu bytes, have %zu", p.bytes, workspace_bytes);
   PA_CHECK_ARG((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "pa_q4_attention: the workspace must be 16-byte aligned");
-  PA_CHECK_ARG(q != out, "pa_q4_attention: out must not be q (a chunk's totals read q after the rows are written)");
+  const int64_t elem = io_dtype == PA_DTYPE_F32 ? 4 : 2;
+  const Q4Rows rows_q{{batch, num_heads, query_len}, {q_stride_b * elem, q_stride_h * elem, q_stride_t * elem}, head_dim * elem};
+  const Q4Rows rows_out{{batch, num_heads, query_len}, {out_stride_b * elem, out_stride_h * elem, out_stride_t * elem},
+                        head_dim * elem};
+  PA_CHECK_ARG(!q4_rows_meet(q, rows_q, out, rows_out),
+               "pa_q4_attention: out must not be q or overlap it (other rows, and a chunk's totals, read q after a row is written)");
 
   Q4Args a{};
   a.q = q; a.q_sb = q_stride_b; a.q_sh = q_stride_h; a.q_st = q_stride_t;

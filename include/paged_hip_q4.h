@@ -51,7 +51,8 @@ int pa_q4_read(const void* k_pool, const void* v_pool, int64_t num_blocks, const
  * weights in two fp16 parts each), with bf16 q the softmax weights are rounded to fp16. weights: for every
  * key, the sum of its softmax weights over the KV head's query heads and the real rows (i < C) is added to
  * its slot's total (a block in several rows of the page table gets the sum of all, in no fixed order).
- * scale must be positive, and out must not overlap q. The workspace (16-byte aligned, pa_q4_attention_workspace_size bytes for the
+ * scale must be positive. out must not overlap q: calls whose rows share a byte are refused, and so are those
+ * whose extents meet with other strides (rows of q and out interleaved in one tensor have the same). The workspace (16-byte aligned, pa_q4_attention_workspace_size bytes for the
  * same arguments, weights != 0 where totals are asked for) needs no initial state and keeps none. Calls on one
  * stream may share one, from several threads too (a call's launches follow each other undivided); calls
  * on several streams must not.

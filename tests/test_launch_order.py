@@ -2,27 +2,21 @@
 the other call between them would overwrite what the first hands on to its second. On the CPU, the HIP launch
 replaced by a stub that records the launching thread."""
 import json
-import shutil
 import subprocess
 import sys
 from pathlib import Path
 
 import pytest
 
+import launch_stub
+
 HERE = Path(__file__).resolve().parent
-LIB = HERE.parent / "efficient-inference-system_amd" / "libpaged_hip.so"
 CALLS = 4  # of each thread
 
 
 @pytest.fixture(scope="module")
 def stub(tmp_path_factory):
-    gxx = shutil.which("g++")
-    if gxx is None or not LIB.exists() or not Path("/opt/rocm/include/hip/hip_runtime_api.h").exists():
-        pytest.skip("needs g++, the HIP headers and the built library")
-    out = tmp_path_factory.mktemp("stub") / "libstub.so"
-    subprocess.run([gxx, "-shared", "-fPIC", "-O1", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include",
-                    str(HERE / "launch_order_stub.cpp"), "-o", str(out), "-pthread"], check=True, timeout=120)
-    return out
+    return launch_stub.build(tmp_path_factory.mktemp("stub"))
 
 
 @pytest.mark.parametrize("name, launches", [
