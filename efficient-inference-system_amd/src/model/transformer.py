@@ -20,6 +20,7 @@ except ImportError:
     _host = None
 from src.cache.q4_kv import Q4BlockPool
 from src.config import ATTENTION_BACKENDS, KVEviction
+from src.kernels import reference_q4
 from src.model.attention import CausalSelfAttention
 
 
@@ -69,6 +70,10 @@ class TinyTransformerLM(nn.Module):
             raise ValueError(f"kv_cache_dtype is a torch dtype, \"int4\" or None, got {kv_cache_dtype!r}")
         if track_attention_weights and kv_cache_dtype != "int4":
             raise ValueError("track_attention_weights needs kv_cache_dtype \"int4\"")
+        if kv_cache_dtype == "int4":
+            reference_q4.page_bytes(d_model // num_heads)  # (refuses other head_dims)
+            if kv_block_size != reference_q4.BLOCK:
+                raise ValueError(f"4-bit pages hold {reference_q4.BLOCK} tokens, got kv_block_size {kv_block_size}")
         self.vocab_size = vocab_size
         self.max_seq_len = max_seq_len
         self.attention_backend = attention_backend
