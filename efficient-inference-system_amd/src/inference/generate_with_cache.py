@@ -99,6 +99,8 @@ def _memory(device: torch.device) -> tuple[int, int]:
 @torch.no_grad()
 def generate_with_cache(model, prompt_ids: torch.Tensor, max_new_tokens, prompt_lengths: torch.Tensor | None = None,
                         eviction: KVEviction | None = None):
+    if eviction is not None:
+        model.check_eviction(eviction)
     device = prompt_ids.device
     B, width = prompt_ids.shape
     gen = _Generation(prompt_ids, _per_request(prompt_lengths, B, width), _per_request(max_new_tokens, B, 0))

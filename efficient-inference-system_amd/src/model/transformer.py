@@ -190,6 +190,11 @@ class TinyTransformerLM(nn.Module):
             if isinstance(cache, PagedKVCacheState):
                 cache.release()
 
+    def check_eviction(self, eviction: KVEviction | None) -> None:
+        """Refuse an eviction that this model's caches cannot serve, before a run starts."""
+        if eviction is not None and not self.track_attention_weights:
+            raise ValueError("eviction needs a model with kv_cache_dtype \"int4\" and track_attention_weights")
+
     def evict_kv_caches(self, kv_caches, eviction: KVEviction) -> int:
         """Cut the requests of the per-layer batched caches (or single states) back as `eviction` says;
         returns how many (request, layer) caches were cut."""

@@ -127,6 +127,8 @@ class StepExecutor:
     keeps attention weights)."""
 
     def __init__(self, model, device, keep_logits: bool = False, observer=None, eviction: KVEviction | None = None):
+        if eviction is not None:
+            model.check_eviction(eviction)
         self.model = model
         self.device = device
         self.keep_logits = keep_logits
