@@ -72,6 +72,16 @@ constexpr float kQ4Start = 4.f;         // log2 of p * max(s) when M is set
 constexpr float kQ4Limit = 32768.f;     // p * max(s, 2^-14) beyond which M is set again
 constexpr short kQ4LimitBits = 0x7800;    // kQ4Limit as a half
 constexpr float kQ4Floor = 6.103515625e-5f;  // 2^-14
+// M of a row that has met no key: of all finite floats the lowest, since any finite score may be the first.
+constexpr float kQ4None = -3.402823466e+38f;
+// Scores (log2) from here on are steep: whole numbers, 1 apart and more. The wide kernel's p is 2^(sc S - M) with
+// the product exact, so M, a float, would miss the largest by half of its step, and p leave fp16 from 2^28
+// on. A column whose M is steep takes the next power of two for sc: its products are floats, M is one of them, and
+// keys that are not the largest keep a weight of 0 as before. (The order of M between columns' parts stays:
+// steep ones move away from zero, others stay below kQ4Steep.)
+constexpr float kQ4Steep = 16777216.f;
+__device__ __forceinline__ bool q4_steep(float M) { return fabsf(M) >= kQ4Steep && M > kQ4None; }
+__device__ __forceinline__ float q4_steep_unit(float sc) { return ldexpf(1.f, __builtin_amdgcn_frexp_expf(sc)); }
 // A zero that the compiler does not know: half * float + zero is one v_fma_mix_f32, which reads the half in
 // place, where a product alone is a conversion and a multiplication.
 __device__ __forceinline__ float q4_zero() {
@@ -114,6 +124,7 @@ struct Q4Wave {
   f16x8 q[W];
   float qs[G];  // sum of the group's q operands (units of code 1)
   float sc;     // log2-domain score of such a unit
+  float unit;   // what stands for it: sc, or while M is steep the power of two above
   int n;        // keys the column sees (a column without a row: 0x7fffffff)
   f32x4 o[G][4];
   float y[G], M, l;
@@ -179,7 +190,7 @@ __device__ __forceinline__ void q4_row_operands(const IO* src, bool there, bool 
   }
 #pragma unroll
   for (int k = 0; k < G; ++k) qs[k] = sum_xor32(sum_xor16(sum[k])) * (1.f / kQ4Unit<PARTS>);
-  sc = fminf(ldexpf(scale_log2, kQ4UnitLog2<PARTS> - up), 1e38f);
+  sc = fmaxf(fminf(ldexpf(scale_log2, kQ4UnitLog2<PARTS> - up), 1e38f), 1e-37f);  // (0 times a score of -inf is NaN)
 }
 
 // Column tile `tile` of (request b, KV head hk).
@@ -196,7 +207,8 @@ __device__ __forceinline__ void q4_setup(const Q4Args& a, int b, int hk, int til
   int n = valid_keys(L, C, i);
   n = n < keys ? n : keys;
   w.n = there ? n : 0x7fffffff;
-  w.M = kNegBig;
+  w.unit = w.sc;
+  w.M = kQ4None;
   w.l = 0.f;
 #pragma unroll
   for (int k = 0; k < G; ++k) {
@@ -323,7 +335,7 @@ __device__ __forceinline__ void q4_step(const uint8_t* pg, Q4Wave<HD, PARTS>& w,
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        p[h][i] = fast_exp2(fmaf(S[h][i], w.sc, -w.M));
+        p[h][i] = fast_exp2(fmaf(S[h][i], w.unit, -w.M));
         big = fmaxf(big, p[h][i]);
       }
 #pragma unroll
@@ -349,20 +361,25 @@ __device__ __forceinline__ void q4_step(const uint8_t* pg, Q4Wave<HD, PARTS>& w,
     }
     const bool far = top[0] > kQ4LimitBits || top[1] > kQ4LimitBits || big > kQ4Limit / kQ4Floor;
     if (__builtin_expect(!__any(far), 1)) break;
-    float m = kNegBig;
+    float sc = w.sc;
+    asm volatile("" : "+v"(sc));  // (or what follows is taken before the loop, in every step)
+    const float steep_unit = q4_steep_unit(sc);
+    float m = kQ4None;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float s = kQ4Floor;
-        asm volatile("" : "+v"(s));  // (or the maxima and logarithms are taken before the loop, in every step)
+        asm volatile("" : "+v"(s));  // (the same)
 #pragma unroll
         for (int k = 0; k < G; ++k) s = fmaxf(s, q4_scale(vm[h][k][i]));
-        m = fmaxf(m, fmaf(S[h][i], w.sc, __builtin_amdgcn_logf(s)) - kQ4Start);
+        const float t = S[h][i] * sc, low = fmaf(S[h][i], sc, __builtin_amdgcn_logf(s)) - kQ4Start;
+        m = fmaxf(m, fabsf(t) >= kQ4Steep ? S[h][i] * steep_unit : __builtin_amdgcn_fmed3f(low, 1.f - kQ4Steep, kQ4Steep - 1.f));
       }
     m = max_xor32(max_xor16(m));
     const float M = fmaxf(w.M, m), f = fast_exp2(w.M - M);
     w.M = M;
+    w.unit = q4_steep(M) ? steep_unit : w.sc;
     w.l *= f;
 #pragma unroll
     for (int k = 0; k < G; ++k) {
@@ -789,7 +806,7 @@ __global__ __launch_bounds__(64 * kQ4Waves, 2) void q4_narrow_kernel(const Q4Arg
   n = there ? n : 0;
 
   f32x4 start[G], o[G][4];
-  float y[G], l = 0.f, M = kNegBig;
+  float y[G], l = 0.f, M = kQ4None;
   const float zero = q4_zero();
 #pragma unroll
   for (int k = 0; k < G; ++k) {
@@ -933,7 +950,7 @@ __global__ __launch_bounds__(64 * kQ4Waves, 2) void q4_narrow_kernel(const Q4Arg
         }
         const bool far = top[0] > kQ4LimitBits || top[1] > kQ4LimitBits || big > kQ4Limit / kQ4Floor;
         if (__builtin_expect(!__any(far), 1)) break;
-        float m = kNegBig;
+        float m = kQ4None;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -1008,7 +1025,7 @@ __global__ __launch_bounds__(64 * kQ4Waves, 2) void q4_narrow_kernel(const Q4Arg
   __syncthreads();
   for (int x = threadIdx.x; x < here * HD; x += 64 * kQ4Waves) {
     const int r = x / HD, d = x - r * HD, m = first + r;
-    float top = kNegBig;
+    float top = kQ4None;
 #pragma unroll
     for (int v = 0; v < kQ4Waves; ++v) top = fmaxf(top, part[(v * GP + r) * (HD + 2)]);
     float den = 0.f, s = 0.f;
@@ -1062,7 +1079,7 @@ __device__ __forceinline__ int q4_splits_of(const Q4Args& a, int b, int i) {
 // Returns M and l.
 template <int HD>
 __device__ __forceinline__ void q4_row_state(const float* rec, int splits, int lane, float& M, float& l) {
-  M = kNegBig;
+  M = kQ4None;
   for (int s = lane; s < splits; s += 64) M = fmaxf(M, rec[(int64_t)s * (HD + 2)]);
   M = wave_max(M);
   l = 0.f;
