@@ -60,7 +60,7 @@ struct Q4Args {
   int32_t splits;       // key ranges per tile, >= 1
   int32_t split_pages;  // pages per key range, even
   float* rec;           // splits > 1: (M, l, O[HD]) per (split, row)
-  float* lse;           // totals: log2 of each row's denominator
+  f32x2* lse;           // totals: each row's (M, log2 of its denominator beside 2^M)
   float* scores;        // decode totals: log2-domain scores [B, H, score_stride]
   int64_t score_stride;
   f16x8* q_ops;         // chunk totals: the row tiles' operands [tile][HD / 32][64 lanes], and per lane
@@ -468,13 +468,15 @@ __device__ __forceinline__ float* q4_record(const Q4Args& a, int b, int hk, int 
   const int64_t rows = (int64_t)a.T * a.group;
   return a.rec + ((((int64_t)b * a.Hk + hk) * rows + row) * a.splits + split) * (HD + 2);
 }
-__device__ __forceinline__ float* q4_lse(const Q4Args& a, int b, int hk, int row) {
+__device__ __forceinline__ f32x2* q4_lse(const Q4Args& a, int b, int hk, int row) {
   return a.lse + ((int64_t)b * a.Hk + hk) * a.T * a.group + row;
 }
 
-// log2 of a row's denominator: infinite (its weights 2^-inf are 0) where the row sees no key, NaN where it met one.
-__device__ __forceinline__ float q4_log_sum(float M, float l) {
-  return l > 0.f || l != l ? M + __builtin_amdgcn_logf(l) : INFINITY;
+// log2 of a row's denominator as (M, log2 l): a key's weight is 2^(S - M - log2 l), where S - M comes first, since
+// the sum of the two would round to M's last digit (a weight off by 1% at scores of 10^5). log2 l is infinite
+// (weights of 0) where the row sees no key, NaN where it met one.
+__device__ __forceinline__ f32x2 q4_log_sum(float M, float l) {
+  return l > 0.f || l != l ? f32x2{M, __builtin_amdgcn_logf(l)} : f32x2{0.f, INFINITY};
 }
 
 // Workgroup -> (request, KV head, tile, split): KV heads innermost, so that workgroups of one moment
@@ -767,7 +769,7 @@ __global__ __launch_bounds__(64 * kQ4Waves, 2) void q4_narrow_kernel(const Q4Arg
   constexpr int G = Batch::G, W = Batch::W, COLS = Batch::COLS, PG = Batch::PG, PAGES = Batch::PAGES, NB = Batch::NB;
   constexpr int PB = q4_page_bytes(HD), CB = q4_codes_bytes(HD);
   __shared__ float part[kQ4Waves * GP * (HD + 2)];
-  __shared__ float lse_of[GP];
+  __shared__ f32x2 lse_of[GP];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int g = lane >> 4, c = lane & 15, col = c & (COLS - 1);
   const int row_in = col % GP, page_in = col / GP % PG;  // this lane's row of the tile and page of the batch
@@ -1048,7 +1050,7 @@ __global__ __launch_bounds__(64 * kQ4Waves, 2) void q4_narrow_kernel(const Q4Arg
       IO* out = static_cast<IO*>(a.out) + (int64_t)u.b * a.o_sb + (int64_t)(u.hk * a.group + j) * a.o_sh + (int64_t)i * a.o_st;
       Elem<IO>::store(out + d, den > 0.f || den != den ? s / den : 0.f);
       if (a.lse != nullptr && d == 0) {
-        const float e = q4_log_sum(top, den);
+        const f32x2 e = q4_log_sum(top, den);
         lse_of[r] = e;
         *q4_lse(a, u.b, u.hk, m) = e;
       }
@@ -1062,7 +1064,7 @@ __global__ __launch_bounds__(64 * kQ4Waves, 2) void q4_narrow_kernel(const Q4Arg
       const int id = q4_block(a.page_table[(int64_t)u.b * a.pt_stride + t / kQ4Tokens], a.num_blocks);
       if (id < 0) continue;
       float sum = 0.f;
-      for (int j = 0; j < here; ++j) sum += fast_exp2(mine[j * a.score_stride + t] - lse_of[j]);
+      for (int j = 0; j < here; ++j) sum += fast_exp2(mine[j * a.score_stride + t] - lse_of[j][0] - lse_of[j][1]);
       atomicAdd(a.weights + ((int64_t)id * a.Hk + u.hk) * kQ4Tokens + (t & (kQ4Tokens - 1)), sum);
     }
   }
@@ -1129,7 +1131,7 @@ __global__ __launch_bounds__(256) void q4_finish_kernel(const Q4Args a, int64_t 
     if (a.lse != nullptr && lane == 0) *q4_lse(a, b, hk, row) = q4_log_sum(M, l);
     return;
   }
-  __shared__ float lse[kQ4MaxNarrow];
+  __shared__ f32x2 lse[kQ4MaxNarrow];
   int x = (int)blockIdx.x - merges;
   const int hk = x % a.Hk;
   x /= a.Hk;
@@ -1157,7 +1159,7 @@ __global__ __launch_bounds__(256) void q4_finish_kernel(const Q4Args a, int64_t 
     const int id = q4_block(a.page_table[(int64_t)b * a.pt_stride + t / kQ4Tokens], a.num_blocks);
     float sum = 0.f;
 #pragma unroll 4
-    for (int j = 0; j < a.group; ++j) sum += fast_exp2(mine[j * a.score_stride + t] - lse[j]);
+    for (int j = 0; j < a.group; ++j) sum += fast_exp2(mine[j * a.score_stride + t] - lse[j][0] - lse[j][1]);
     if (id >= 0) atomicAdd(a.weights + ((int64_t)id * a.Hk + hk) * kQ4Tokens + (t & (kQ4Tokens - 1)), sum);
   }
 }
@@ -1213,12 +1215,12 @@ __global__ __launch_bounds__(64 * kQ4SumWaves) void q4_chunk_weights_kernel(cons
   // (the next tile's operands are loaded while this one's scores are formed; past the last one, its own)
   f16x8 next[W];
   f32x4 next_aux;
-  float next_lse;
+  f32x2 next_lse;
   const int last = (real - 1) / ROWS;
   auto load = [&](int tile) {
     tile = tile < last ? tile : last;
     const int row = q4_row<PARTS>(tile, c);
-    next_lse = row < real && c < ROWS ? *q4_lse(a, b, hk, row < rows ? row : rows - 1) : INFINITY;  // (2^-inf: 0)
+    next_lse = row < real && c < ROWS ? *q4_lse(a, b, hk, row < rows ? row : rows - 1) : f32x2{0.f, INFINITY};  // (2^-inf: 0)
     if constexpr (READY) {
       const int64_t at = ((int64_t)b * a.Hk + hk) * a.op_tiles + tile;
 #pragma unroll
@@ -1232,7 +1234,7 @@ __global__ __launch_bounds__(64 * kQ4SumWaves) void q4_chunk_weights_kernel(cons
     f16x8 q[W];
     float qs[G], sc;
     int n;
-    const float lse = next_lse;
+    const float M = next_lse[0], log_l = next_lse[1], lse = M + log_l;
     if constexpr (READY) {
 #pragma unroll
       for (int s = 0; s < W; ++s) q[s] = next[s];
@@ -1253,18 +1255,22 @@ __global__ __launch_bounds__(64 * kQ4SumWaves) void q4_chunk_weights_kernel(cons
       n = pad ? 0 : w.n;
       load(tile + STEP);
     }
+    // masked: some columns do not see all the keys, or have scores that M + log2 l in one float would blur
     auto add = [&](auto masked) {
+      const float unit = READY && q4_steep(M) ? q4_steep_unit(sc) : sc;
 #pragma unroll
       for (int h = 0; h < PG; ++h) {
         const f32x4 S = q4_scores<HD, PARTS>(kf[h], km[h], q, qs);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float p = fast_exp2(fmaf(S[i], sc, -lse));
+          float x = S[i] * unit;
+          if (!READY) asm("" : "+v"(x));  // (the narrow kernel's scores are rounded, the wide one's products exact)
+          const float p = fast_exp2(decltype(masked)::value ? (READY ? fmaf(S[i], unit, -M) : x - M) - log_l : fmaf(S[i], sc, -lse));
           sum[h][i] += decltype(masked)::value && key0 + h * kQ4Tokens + 4 * g + i >= n ? 0.f : p;
         }
       }
     };
-    if (__any(n < key0 + PG * kQ4Tokens)) add(std::true_type()); else add(std::false_type());
+    if (__any(n < key0 + PG * kQ4Tokens || !(fabsf(M) < 256.f))) add(std::true_type()); else add(std::false_type());
   }
 #pragma unroll
   for (int h = 0; h < PG; ++h)
@@ -1346,7 +1352,7 @@ static Q4Plan q4_plan(int io_dtype, int32_t batch, int32_t heads, int32_t kv_hea
   // eight wavefronts to a workgroup while there are fewer than two workgroups a CU
   p.halves = p.wide && units * p.splits < 2 * (int64_t)pa_host::device_cu_count();
   p.rec = p.splits > 1 ? (size_t)batch * kv_heads * p.rows * p.splits * (head_dim + 2) : 0;
-  p.lse = weights ? (size_t)batch * kv_heads * p.rows : 0;
+  p.lse = weights ? (size_t)batch * kv_heads * p.rows * 2 : 0;
   p.score_stride = (size_t)(max_pages + (max_pages & 1)) * kQ4Tokens;
   p.scores = weights && query_len == 1 && !p.wide ? (size_t)batch * heads * p.score_stride : 0;
   p.op_tiles = p.tiles * kQ4WideWaves;
@@ -1526,7 +1532,7 @@ extern "C" int pa_q4_attention(const void* q, int64_t q_stride_b, int64_t q_stri
   a.tiles = p.tiles; a.splits = p.splits; a.split_pages = p.split_pages;
   float* ws = static_cast<float*>(workspace);
   a.rec = p.splits > 1 ? ws : nullptr;
-  a.lse = p.lse ? ws + p.rec : nullptr;
+  a.lse = p.lse ? reinterpret_cast<f32x2*>(ws + p.rec) : nullptr;
   a.scores = p.scores ? ws + p.rec + p.lse : nullptr;
   a.score_stride = (int64_t)p.score_stride;
   float* ops = ws + p.rec + p.lse + p.scores;

@@ -74,3 +74,20 @@ def test_outputs_stay_between_the_values(device, dtype, hd, v_scale, name):
                         magnitude, b, h, i, len(near))
         if magnitude >= 1e6:
             assert one_hot > 0.4 * B * H * T  # (most rows have one key that counts)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("name", SHAPES)
+def test_a_rows_weights_add_up_to_one(device, dtype, hd, name):
+    """The totals of a request's keys add up to the rows that gave weights, at every size of the scores."""
+    for magnitude in (0.0, 1.0, 30.0, 300.0, 1e4, 1e5, 1e6, 2e7, 1e8, 3e8, 1e9, 1e12, 1e20, 1e30, 1e35):
+        q, kp, vp, table, lens = make(name, hd, dtype, magnitude)
+        totals = torch.zeros(60, kp.shape[1], 16, device=device)
+        call(device, q, kp, vp, table, lens, totals)
+        totals = totals.double().cpu().numpy()
+        for b in range(2):
+            got = totals[table[b][table[b] >= 0]].sum((0, 2))
+            want = q.shape[1] // kp.shape[1] * q.shape[2]
+            # exponents of up to 2^8 rounded to fp32, a few sums of a few hundred terms
+            assert (np.abs(got - want) <= 2.0 ** -14 * want).all(), (magnitude, got, want)
