@@ -335,6 +335,19 @@ extern "C" int pa_q4_evict(void* k_pool, void* v_pool, float* weights, int64_t n
     PA_CHECK_ARG(page_table && pt_stride >= max_pages && new_page_table && new_pt_stride >= new_max_pages,
                  "pa_q4_evict: page table missing or stride below its width");
   }
+  // what a workgroup writes, others still read
+  const auto meet = [](const int32_t* x, int64_t nx, const int32_t* y, int64_t ny) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(y);
+    return a < b + 4 * (uintptr_t)ny && b < a + 4 * (uintptr_t)nx;
+  };
+  const int64_t n_kept = (int64_t)batch * kv_heads * keep, n_old = max_pages > 0 ? (batch - 1) * pt_stride + max_pages : 0,
+                n_new = max_pages > 0 ? (batch - 1) * new_pt_stride + new_max_pages : 0;
+  PA_CHECK_ARG(!meet(new_seq_lens, batch, seq_lens, batch) && !meet(new_seq_lens, batch, page_table, n_old) &&
+                   !meet(new_seq_lens, batch, new_page_table, n_new) && !meet(new_seq_lens, batch, kept, n_kept) &&
+                   !meet(kept, n_kept, seq_lens, batch) && !meet(kept, n_kept, page_table, n_old) &&
+                   !meet(kept, n_kept, new_page_table, n_new),
+               "pa_q4_evict: kept and new_seq_lens must not overlap each other, the lengths or the page tables");
+  PA_CHECK_ARG(max_pages == 0 || page_table != new_page_table, "pa_q4_evict: the new pages must be none of the old ones");
   const int pages = (int)((most + kQ4Tokens - 1) / kQ4Tokens);
   PA_CHECK_ARG((int64_t)batch * kv_heads * (pages + 1) <= 0x7fffff00LL, "pa_q4_evict: grid too large");
   Q4EvictArgs a{};

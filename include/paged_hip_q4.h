@@ -76,7 +76,8 @@ size_t pa_q4_attention_workspace_size(int io_dtype, int32_t batch, int32_t num_h
  * the last), their rows and totals in that order into the pages of new_page_table[b, :], whose other rows
  * stay as they are, and min(n, keep) to new_seq_lens[b]. A kept key without a page moves as zeros; new
  * pages that are no blocks of the pool are skipped. The new pages must be none of the batch's old ones,
- * and hold min(keep, 16 * max_pages) keys.
+ * and hold min(keep, 16 * max_pages) keys; kept and new_seq_lens must not overlap each other, the lengths
+ * or the page tables.
  */
 int pa_q4_evict(void* k_pool, void* v_pool, float* weights, int64_t num_blocks,
                 const int32_t* page_table, int64_t pt_stride, int32_t max_pages, const int32_t* seq_lens,
