@@ -14,7 +14,7 @@
 // The codes never leave the matrix cores' operands and no cross-lane move feeds them (see pa_q4.h).
 //
 // Precision. bf16 q is exact in fp16 once scaled by a power of two per row (below 2^-23 of the row's
-// largest element bits are lost); w is rounded to fp16 (2^-12), the 7.5 w beside it is the rounded
+// largest element bits are lost); w is rounded to fp16 (2^-11), the 7.5 w beside it is the rounded
 // one, so the error is that of a code within +-7.5. For fp32 q (PARTS = 2) q and w are each the sum
 // of two fp16 values, 2^-23 or better: the columns of a tile are 8 rows twice, column c the high parts
 // of row c, column c + 8 the low ones, both parts' products summed with one DPP rotation. The second
@@ -504,8 +504,8 @@ constexpr int kQ4MaxNarrow = 32;  // rows that the narrow kernel takes (two tile
 //
 // Bound by vector instructions: a step of 32 keys takes some 200 (the codes' ANDs and shifts 80, the pairs' scales
 // and centres 64, exponentials and sums the rest) to 18 matrix instructions, 82% of the cycles that a CU has
-// work (4 x 512 rows of 32 heads x 128 bf16 over 1024 to 4096 keys: 215 us, 460 TFLOP/s; 200 rows of 32 over 8 heads
-// over 16k keys: 140 us, 380). Two tiles a wavefront, which share the codes' part, take 256 registers: 240 us.
+// work (4 x 512 rows of 32 heads x 128 bf16 over 1024 to 4096 keys: 215 to 235 us from one process to another, 420 to 460
+// TFLOP/s; 200 rows of 32 over 8 heads over 16k keys: 138 us, 390). Two tiles a wavefront, which share the codes' part, take 256 registers: 240 us.
 //
 // HALVES = 2, for grids that leave the GPU room: eight wavefronts for the same four tiles, stages of 128 keys,
 // each half of the wavefronts taking its half of every stage, joined in LDS at the end. A step is a chain of
@@ -1097,7 +1097,8 @@ __device__ __forceinline__ void q4_row_state(const float* rec, int splits, int l
 // adds kQ4FinishKeys keys' weights of one KV head, having formed its rows' denominators from the records by itself (a
 // launch less than in two steps). A block that two rows of the page table share is added to by both, hence
 // the atomic; otherwise each slot gets one addition. 64 requests of 32 over 8 heads of 512 to 16384 keys: 42 MB of
-// scores and 10 MB of totals, 21 us, bound by the records that every workgroup reads again.
+// scores and 10 MB of totals, 21 us, 2.4 TB/s, with the vector units busy 31% of the time: latency, of the lengths, the
+// records and the denominators that each workgroup takes one after the other before its scores.
 constexpr int kQ4FinishKeys = 1024;  // (256, a key per thread, repeated the denominators too often: 34 -> 20 us)
 
 template <typename IO, int HD>
@@ -1170,7 +1171,7 @@ __global__ __launch_bounds__(256) void q4_finish_kernel(const Q4Args a, int64_t 
 // the tiles' q operands are in the workspace, left by the wide kernel (formed here they cost as much as the
 // scores). A block that two rows of the page table share is added to by both, hence the atomic; otherwise
 // each slot gets one addition. Bound by vector instructions, 170 to 16 matrix instructions a tile: 200 rows of 32
-// over 8 heads x 128 bf16 over 16.5k keys 72 us (370 TFLOP/s).
+// over 8 heads x 128 bf16 over 16.5k keys 73 us (370 TFLOP/s).
 constexpr int kQ4SumWaves = 8;
 
 template <typename IO, int HD, int PARTS, bool READY, int PG, bool EACH>

@@ -78,7 +78,7 @@ __device__ __forceinline__ void q4_load8(const T* p, bool vec, float (&x)[8]) {
   }
 }
 
-// The codes of a lane's eight values: (x - z) / s + 7.5 to the nearest, ties to even, in 0..15, formed as
+// The codes of a lane's eight values: (x - z) / s + 7.5 of fp64 to the nearest, ties to even, in 0..15, formed as
 // x / s + (7.5 - z / s) in one fma a value. Where the quotient is below 16 the fp32 value is within
 // 2.5e-6 + |z / s| 2^-24 of the real one (8 x 2^-23 of the reciprocal, 2^-24 each of the sum, below 16, and
 // of its constant), so it decides unless it lies that close (taken twice as wide) to a border between two

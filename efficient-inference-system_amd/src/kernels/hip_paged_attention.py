@@ -114,7 +114,7 @@ def _capture_id(stream: int) -> int:
 
 def _call_workspace(device: torch.device, nbytes: int, kind: str) -> torch.Tensor:
     """The workspace of a call on `device`'s current stream: calls that follow each other on one stream
-    share one, calls on several streams and replays of several graphs never do (they would add to the
+    share one (from whichever threads: the library keeps a call's launches together), calls on several streams and replays of several graphs never do (they would add to the
     same arrival counters and overwrite each other's records). Under capture it comes from the graph's
     memory, one per capture and stream, cleared by the first call that the graph replays. The stream
     that allocated a workspace is the only one that uses it, so that one dropped here (at most

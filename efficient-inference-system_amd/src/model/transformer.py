@@ -138,7 +138,8 @@ class TinyTransformerLM(nn.Module):
         max_batch, one prefill chunk per length bucket and one decode step, on throwaway
         requests that are released afterwards. want_logits selects the graphs of steps that return
         logits (forward, greedy_step(return_logits=True)) instead of those that return only the
-        greedy tokens. Leaves fresh pools; returns the captures made."""
+        greedy tokens. Leaves fresh pools; returns the captures made, 0 for models whose steps run eagerly
+        (another device or backend, 4-bit pools)."""
         from src.model.graph_decode import T_BUCKETS
 
         device = torch.device(device)

@@ -28,8 +28,11 @@ size_t pa_q4_page_bytes(int32_t head_dim);
  * (as pa_kv_append; negative slots and blocks outside the pool are skipped, two rows of one slot in
  * a call leave parts of both). Per group, values clamped to +-65504: s = half((hi - lo) / 15), z = half((hi + lo) / 2), the
  * difference, the sum and their products with 1/15 and 1/2 rounded to fp32 first; c = (x - z) / s + 7.5
- * rounded to the nearest, ties to even, exactly, in 0..15 (0 where s is 0). A centre of zero is +0. A group with a NaN gets NaN
- * for s and z. weights: the written slots' totals are cleared.
+ * in 64 bits (difference, quotient and sum each rounded to them), then to the nearest, ties to even, in 0..15 (0
+ * where s is 0). So a value stands for its own within s / 2, but for what the halves lose: a group whose spread is
+ * small beside its centre (1000 +- 0.1, where z's step is 1/2) is off by up to half of z's step, all codes at one
+ * end. A centre of zero is +0. A group with a NaN gets NaN for s and z. weights: the written slots' totals are
+ * cleared.
  */
 int pa_q4_append(const void* k_new, const void* v_new, int64_t new_stride_b, int64_t new_stride_h,
                  int64_t new_stride_t, int new_dtype,
