@@ -126,7 +126,7 @@ class TinyTransformerLM(nn.Module):
 
     def _graph_runner(self):
         """Lazily created HIP-graph runner for cached steps (see graph_decode.py)."""
-        if self._graph_step is None:
+        if self._graph_step is None or self._graph_step.model is not self:  # (a shallow copy holds the original's)
             from src.model.graph_decode import GraphedStep
 
             self._graph_step = GraphedStep(self)

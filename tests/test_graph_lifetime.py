@@ -112,3 +112,15 @@ def test_a_collector_that_was_off_stays_off(monkeypatch):
     with _collector(False):
         runner._capture(SimpleNamespace(ids=torch.zeros(1), graph=None, logits=None), [])
         assert not gc.isenabled()
+
+
+def test_a_shallow_copy_makes_its_own_runner():
+    """A shallow copy (module replication makes such) holds the original's runner, whose model may be gone."""
+    model = _model()
+    model._graph_runner()
+    other = copy.copy(model)
+    assert other._graph_runner().model is other
+    assert model._graph_runner().model is model
+    del model
+    gc.collect()
+    assert other._graph_runner().model is other
